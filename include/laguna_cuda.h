@@ -233,9 +233,50 @@ int lc_mha_attn(lc_ctx *ctx, const float *q, const float *k, const float *v,
                 float *out, uint32_t m, uint32_t n_q_heads, uint32_t n_kv_heads,
                 uint32_t head_dim, uint32_t seq_len, float scale,
                 uint32_t q_pos0, uint32_t causal);
+/* Rotary positions of q [m, n_q_heads, head_dim] and k [m, n_kv_heads,
+ * head_dim] in one launch, beside lc_qk_norm_rope, for a batch of rows that sit
+ * at positions of their own.  Pair i of a head (i < rope_dim / 2) is turned by
+ * a = pos[row] * freq[i]:
+ *   y1 = scale (x1 cos a - x2 sin a),  y2 = scale (x2 cos a + x1 sin a);
+ * dims from rope_dim on are copied (rope_dim 0 copies and converts whole rows).
+ * LC_ROPE_HALF pairs dim i with i + rope_dim / 2, LC_ROPE_PAIRS dim 2i with
+ * 2i + 1.  The angle is exact for every int32 position; -pos with 1 / scale
+ * undoes pos.  x is of type dtype and y of out_dtype (LC_F32, LC_F16 or LC_BF16
+ * each; f32 arithmetic, one rounding), so k can go straight into a 16-bit cache.
+ * ld*: elements between rows (0: rows follow each other; q and k may be columns
+ * of one buffer).  An output may be its own input (same type and stride); any
+ * other overlap with an output is LC_ERR_INVALID.  n_q_heads or n_kv_heads may
+ * be 0.  pos [m] and freq [rope_dim / 2] are device pointers; pointers need
+ * only the alignment of their type, 16-byte alignment is faster.  The reference
+ * rotates whole f32 heads in the half layout (kernels/qk_norm_rope.comp:29-67). */
+enum { LC_ROPE_HALF = 0, LC_ROPE_PAIRS = 1 };
+int lc_rope(lc_ctx *ctx, int dtype, int out_dtype, int layout, const void *q, uint64_t ldq, void *q_out,
+            uint64_t ldq_out, uint32_t n_q_heads, const void *k, uint64_t ldk, void *k_out, uint64_t ldk_out,
+            uint32_t n_kv_heads, const int32_t *pos, const float *freq, uint32_t m, uint32_t head_dim,
+            uint32_t rope_dim, float scale);
 /* RoPE frequency table (src/dflash.rs:901-907) on the host:
  * freq[i] = 1 / base^(2i/rope_dim), i < rope_dim/2. */
 int lc_rope_freq(float *freq_host, uint32_t rope_dim, float base);
+/* Frequency table stretched for contexts `factor` times as long (on the host;
+ * each value formed in 64 bits and rounded once), and the factor lc_rope takes
+ * as `scale` with it:
+ *   LC_ROPE_SCALE_NONE    base^(-2i/rope_dim)
+ *   LC_ROPE_SCALE_LINEAR  the same / factor
+ *   LC_ROPE_SCALE_NTK     base * factor^(rope_dim / (rope_dim - 2)) as the base
+ *   LC_ROPE_SCALE_YARN    pairs that turn more than beta_fast times in orig_ctx
+ *                         positions as they are, those that turn less than
+ *                         beta_slow times / factor, a linear ramp between;
+ *                         *scale = 0.1 ln(factor) + 1
+ * factor >= 1 (ignored by NONE); orig_ctx, beta_fast (32 is usual) and beta_slow
+ * (1) are read by YARN only.  *scale is 1 but for YARN. */
+enum {
+    LC_ROPE_SCALE_NONE = 0,
+    LC_ROPE_SCALE_LINEAR = 1,
+    LC_ROPE_SCALE_NTK = 2,
+    LC_ROPE_SCALE_YARN = 3
+};
+int lc_rope_freq_scaled(float *freq_host, uint32_t rope_dim, float base, int kind, float factor, uint32_t orig_ctx,
+                        float beta_fast, float beta_slow, float *scale);
 
 /* ---- lm_head + argmax ----------------------------------------------------- */
 

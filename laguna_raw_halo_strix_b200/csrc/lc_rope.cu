@@ -1,0 +1,346 @@
+// lc_rope.cu -- rotary positions of q and k: half and interleaved pairs, part
+// of the head, a position per row, any row stride, f32 / f16 / bf16 in and out.
+//
+// Pair i of a head (rope_dim / 2 pairs) is turned by a = pos * freq[i]:
+//   y1 = s (x1 cos a - x2 sin a),  y2 = s (x2 cos a + x1 sin a),
+// the remaining dims are copied.  The angle of a far position needs more than
+// 24 bits (pos 1e6 at freq 1 is 0.06 rad off in f32): the product of two
+// numbers of at most 31 and 24 bits is exact to 2^-53 in a double, and is
+// reduced mod 2 pi there; sincosf then sees |a| <= pi.  The rotation itself is
+// f32 with one rounding to the output type.
+//
+// Bound by the bytes of x and y.  One CTA takes a row (or a share of its heads
+// when there are few rows): the row's table of (cos, sin) is formed once in
+// shared memory for every head, while each thread's first loads are in flight.
+#include <math.h>
+
+#include <algorithm>
+
+#include <cuda_bf16.h>
+
+#include "lc_internal.cuh"
+
+namespace {
+
+constexpr int kRpThreads = 128;
+// Items a thread loads before the table is ready.  A 40-head row of 128 in
+// 16-bit types is 320 items, 2.5 a thread.
+constexpr int kRpItems = 3;
+constexpr uint32_t kRpMaxDim = 8192;  // table of 32 KB
+
+template <class T>
+struct RpVec;  // 16 bytes of T
+template <>
+struct RpVec<float> {
+    static constexpr int kN = 4;
+};
+template <>
+struct RpVec<__half> {
+    static constexpr int kN = 8;
+};
+template <>
+struct RpVec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+};
+
+__device__ __forceinline__ float rp_f32(float v) { return v; }
+__device__ __forceinline__ float rp_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float rp_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void rp_round(float v, float &o) { o = v; }
+__device__ __forceinline__ void rp_round(float v, __half &o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void rp_round(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
+
+// N consecutive elements, as one access of N * sizeof(T) bytes where VEC.
+template <class T, int N>
+struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) RpPack {
+    T v[N];
+};
+template <class T, int N, bool VEC>
+__device__ __forceinline__ RpPack<T, N> rp_load(const T *p) {
+    RpPack<T, N> r;
+    if constexpr (VEC) {
+        r = *reinterpret_cast<const RpPack<T, N> *>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) r.v[i] = p[i];
+    }
+    return r;
+}
+template <class T, int N, bool VEC>
+__device__ __forceinline__ void rp_store(T *p, const float (&y)[N]) {
+    RpPack<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; i++) rp_round(y[i], r.v[i]);
+    if constexpr (VEC) {
+        *reinterpret_cast<RpPack<T, N> *>(p) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) p[i] = r.v[i];
+    }
+}
+
+struct RpArgs {
+    const void *x[2];   // q, k
+    void *y[2];
+    uint64_t ldx[2], ldy[2];  // elements between rows
+    int same[2];              // y is x: dims past rope_dim stay as they are
+    int n_q, n_heads;         // heads of q, of q and k together
+    int head_dim, rope_dim;
+    int rot, items;           // rotated items of a head, all items of a head
+    int heads_per_cta;
+    const int32_t *pos;
+    const float *freq;
+    float scale;
+};
+
+// PAIRS false: an item is V dims at i and the V at i + rope_dim / 2; true: the
+// V / 2 pairs of V neighbouring dims.  Items rot.. are V copied dims.
+template <class TI, class TO, bool PAIRS, int V, bool VEC>
+__global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
+    extern __shared__ float2 cs[];  // [rope_dim / 2]
+    const size_t row = blockIdx.x;
+    const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.n_heads, h0 + a.heads_per_cta);
+    const int total = (h1 - h0) * a.items, half = a.rope_dim >> 1;
+
+    auto place = [&](int idx, int &t, int &head, int &item) {
+        const int h = idx / a.items;
+        item = idx - h * a.items;
+        t = h0 + h >= a.n_q;
+        head = h0 + h - (t ? a.n_q : 0);
+    };
+    auto first = [&](int item) { return item < a.rot ? item * V : a.rope_dim + (item - a.rot) * V; };
+    auto load = [&](int idx, RpPack<TI, V> &p0, RpPack<TI, V> &p1) {
+        int t, head, item;
+        place(idx, t, head, item);
+        const TI *x = static_cast<const TI *>(t ? a.x[1] : a.x[0]) + row * (t ? a.ldx[1] : a.ldx[0]) +
+                      (size_t)head * a.head_dim + first(item);
+        if (item >= a.rot && (t ? a.same[1] : a.same[0])) return;
+        p0 = rp_load<TI, V, VEC>(x);
+        if (!PAIRS && item < a.rot) p1 = rp_load<TI, V, VEC>(x + half);
+    };
+    auto finish = [&](int idx, const RpPack<TI, V> &p0, const RpPack<TI, V> &p1) {
+        int t, head, item;
+        place(idx, t, head, item);
+        TO *y = static_cast<TO *>(t ? a.y[1] : a.y[0]) + row * (t ? a.ldy[1] : a.ldy[0]) +
+                (size_t)head * a.head_dim + first(item);
+        float o0[V], o1[V];
+        if (item >= a.rot) {
+            if (t ? a.same[1] : a.same[0]) return;
+#pragma unroll
+            for (int i = 0; i < V; i++) o0[i] = rp_f32(p0.v[i]);
+            rp_store<TO, V, VEC>(y, o0);
+        } else if constexpr (PAIRS) {
+#pragma unroll
+            for (int i = 0; i + 1 < V; i += 2) {
+                const float2 c = cs[(item * V + i) >> 1];
+                const float u = rp_f32(p0.v[i]), w = rp_f32(p0.v[i + 1]);
+                o0[i] = u * c.x - w * c.y;
+                o0[i + 1] = w * c.x + u * c.y;
+            }
+            rp_store<TO, V, VEC>(y, o0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float2 c = cs[item * V + i];
+                const float u = rp_f32(p0.v[i]), w = rp_f32(p1.v[i]);
+                o0[i] = u * c.x - w * c.y;
+                o1[i] = w * c.x + u * c.y;
+            }
+            rp_store<TO, V, VEC>(y, o0);
+            rp_store<TO, V, VEC>(y + half, o1);
+        }
+    };
+
+    RpPack<TI, V> p0[kRpItems], p1[kRpItems];
+#pragma unroll
+    for (int j = 0; j < kRpItems; j++)
+        if ((int)threadIdx.x + j * kRpThreads < total) load(threadIdx.x + j * kRpThreads, p0[j], p1[j]);
+    if (half) {
+        const double pos = (double)a.pos[row];
+        for (int i = threadIdx.x; i < half; i += kRpThreads) {
+            const double t = pos * (double)a.freq[i];
+            const double n = rint(t * 0.15915494309189533577);      // 1 / (2 pi)
+            double r = fma(-n, 6.28318530717958623200, t);           // 2 pi, rounded to a double,
+            r = fma(-n, 2.44929359829470635445e-16, r);              // and what it lacks
+            float sn, cn;
+            sincosf((float)r, &sn, &cn);
+            cs[i] = make_float2(cn * a.scale, sn * a.scale);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kRpItems; j++)
+        if ((int)threadIdx.x + j * kRpThreads < total) finish(threadIdx.x + j * kRpThreads, p0[j], p1[j]);
+    for (int idx = threadIdx.x + kRpItems * kRpThreads; idx < total; idx += kRpThreads) {
+        load(idx, p0[0], p1[0]);
+        finish(idx, p0[0], p1[0]);
+    }
+}
+
+int type_bytes(int dtype) { return dtype == LC_F32 ? 4 : dtype == LC_F16 || dtype == LC_BF16 ? 2 : 0; }
+
+// Do the m rows of wa bytes, pa apart, at a share a byte with the m rows of wb
+// bytes, pb apart, at b?  Exact for equal pitches (columns of one buffer);
+// otherwise whole extents are compared.
+bool rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
+    const intptr_t d = (intptr_t)b - (intptr_t)a;
+    if (pa != pb || m == 1) {
+        const uint64_t ea = (m - 1) * pa + wa, eb = (m - 1) * pb + wb;
+        return d < (intptr_t)ea && -d < (intptr_t)eb;
+    }
+    // row i of a and row i + j of b start d + j * pa apart: overlap if that is in (-wb, wa)
+    const intptr_t p = (intptr_t)pa;
+    const intptr_t j0 = d >= 0 ? -(d / p) : (-d + p - 1) / p;  // d + j0 * p in [0, p)
+    for (intptr_t j = j0 - 1; j <= j0; j++) {
+        const intptr_t at = d + j * p;
+        if (j < (intptr_t)m && -j < (intptr_t)m && at < (intptr_t)wa && -at < (intptr_t)wb) return true;
+    }
+    return false;
+}
+
+template <class TI, class TO>
+int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
+    constexpr int V = RpVec<TI>::kN;
+    RpArgs a = base;
+    const int half = a.rope_dim / 2;
+    // 16-byte input vectors (and the same element count out) where every row,
+    // head and half starts on a multiple of them; single elements otherwise
+    bool vec = a.head_dim % V == 0 && (pairs ? a.rope_dim : half) % V == 0;
+    for (int t = 0; t < 2; t++)
+        if (t ? a.n_heads > a.n_q : a.n_q > 0) {
+            const uintptr_t need_y = V * sizeof(TO) > 16 ? 16 : V * sizeof(TO);
+            vec = vec && (uintptr_t)a.x[t] % 16 == 0 && a.ldx[t] % V == 0 && (uintptr_t)a.y[t] % need_y == 0 &&
+                  a.ldy[t] % V == 0;
+        }
+    const int v = vec ? V : pairs ? 2 : 1;
+    const bool q_copies = a.n_q > 0 && !a.same[0], k_copies = a.n_heads > a.n_q && !a.same[1];
+    // (head_dim and rope_dim are even, so the copied dims divide by 2 as well)
+    a.rot = pairs ? a.rope_dim / v : half / v;
+    a.items = a.rot + ((q_copies || k_copies) ? (a.head_dim - a.rope_dim) / v : 0);
+    if (a.items == 0) return LC_OK;
+    // Few rows: a row's heads go to several CTAs, each with at least one item a
+    // thread; every CTA forms the table again (a 16-row, 40-head block of 128:
+    // 6 CTAs a row instead of 1).
+    const int per_head = a.items;
+    int splits = 1;
+    if (m < 2u * ctx->num_sms) {
+        const int most = std::max(1, a.n_heads * per_head / kRpThreads);
+        splits = std::min<int>(most, std::max(1, 2 * ctx->num_sms / (int)m));
+    }
+    a.heads_per_cta = (a.n_heads + splits - 1) / splits;
+    splits = (a.n_heads + a.heads_per_cta - 1) / a.heads_per_cta;
+    const dim3 grid(m, splits);
+    const size_t smem = (size_t)half * sizeof(float2);
+    auto go = [&](auto kernel) -> int {
+        kernel<<<grid, kRpThreads, smem, ctx->stream>>>(a);
+        return lc_after_launch(ctx, "lc_rope");
+    };
+    if (pairs) return vec ? go(rope_kernel<TI, TO, true, V, true>) : go(rope_kernel<TI, TO, true, 2, false>);
+    return vec ? go(rope_kernel<TI, TO, false, V, true>) : go(rope_kernel<TI, TO, false, 1, false>);
+}
+
+template <class TI>
+int rope_out(lc_ctx *ctx, int out_dtype, const RpArgs &a, uint32_t m, bool pairs) {
+    switch (out_dtype) {
+    case LC_F16: return rope_launch<TI, __half>(ctx, a, m, pairs);
+    case LC_BF16: return rope_launch<TI, __nv_bfloat16>(ctx, a, m, pairs);
+    default: return rope_launch<TI, float>(ctx, a, m, pairs);
+    }
+}
+
+}  // namespace
+
+extern "C" int lc_rope(lc_ctx *ctx, int dtype, int out_dtype, int layout, const void *q, uint64_t ldq, void *q_out,
+                       uint64_t ldq_out, uint32_t n_q_heads, const void *k, uint64_t ldk, void *k_out,
+                       uint64_t ldk_out, uint32_t n_kv_heads, const int32_t *pos, const float *freq, uint32_t m,
+                       uint32_t head_dim, uint32_t rope_dim, float scale) {
+    LC_REQUIRE(ctx, LC_ERR_INVALID, "lc_rope: null ctx");
+    const uint64_t bi = type_bytes(dtype), bo = type_bytes(out_dtype);
+    LC_REQUIRE(bi && bo, LC_ERR_UNSUPPORTED, "lc_rope: types %d -> %d (LC_F32, LC_F16 and LC_BF16 only)", dtype,
+               out_dtype);
+    LC_REQUIRE(layout == LC_ROPE_HALF || layout == LC_ROPE_PAIRS, LC_ERR_INVALID, "lc_rope: bad layout %d", layout);
+    LC_REQUIRE(head_dim > 0 && head_dim % 2 == 0, LC_ERR_INVALID, "lc_rope: head_dim %u must be even", head_dim);
+    LC_REQUIRE(rope_dim % 2 == 0 && rope_dim <= head_dim, LC_ERR_INVALID,
+               "lc_rope: rope_dim %u must be even and at most head_dim %u", rope_dim, head_dim);
+    LC_REQUIRE(rope_dim <= kRpMaxDim, LC_ERR_UNSUPPORTED, "lc_rope: rope_dim %u above %u", rope_dim, kRpMaxDim);
+    LC_REQUIRE(((uint64_t)n_q_heads + n_kv_heads) * head_dim < (1u << 30), LC_ERR_UNSUPPORTED,
+               "lc_rope: rows of %u + %u heads of %u are too long", n_q_heads, n_kv_heads, head_dim);
+    LC_REQUIRE(m < (1u << 31), LC_ERR_UNSUPPORTED, "lc_rope: %u rows", m);
+    const uint64_t wq = (uint64_t)n_q_heads * head_dim, wk = (uint64_t)n_kv_heads * head_dim;
+    if (m == 0 || wq + wk == 0) return LC_OK;
+    if (!ldq) ldq = wq;
+    if (!ldq_out) ldq_out = wq;
+    if (!ldk) ldk = wk;
+    if (!ldk_out) ldk_out = wk;
+    LC_REQUIRE((!wq || (q && q_out)) && (!wk || (k && k_out)) && (!rope_dim || (pos && freq)), LC_ERR_INVALID,
+               "lc_rope: null pointer");
+    const uint64_t ld_max = std::max(std::max(ldq, ldq_out), std::max(ldk, ldk_out));
+    LC_REQUIRE(ld_max <= ((uint64_t)1 << 60) / m, LC_ERR_INVALID, "lc_rope: row stride %llu too large",
+               (unsigned long long)ld_max);
+    LC_REQUIRE(ldq >= wq && ldq_out >= wq && ldk >= wk && ldk_out >= wk, LC_ERR_INVALID,
+               "lc_rope: a row stride is shorter than its row");
+    LC_REQUIRE((!wq || ((uintptr_t)q % bi == 0 && (uintptr_t)q_out % bo == 0)) &&
+                   (!wk || ((uintptr_t)k % bi == 0 && (uintptr_t)k_out % bo == 0)) && (uintptr_t)pos % 4 == 0 &&
+                   (uintptr_t)freq % 4 == 0,
+               LC_ERR_INVALID, "lc_rope: a pointer is not aligned to its type");
+    const bool q_same = wq && q == q_out && ldq == ldq_out && bi == bo && dtype == out_dtype;
+    const bool k_same = wk && k == k_out && ldk == ldk_out && bi == bo && dtype == out_dtype;
+    const bool meet = (wq && !q_same && rows_meet(q, ldq * bi, wq * bi, q_out, ldq_out * bo, wq * bo, m)) ||
+                      (wk && !k_same && rows_meet(k, ldk * bi, wk * bi, k_out, ldk_out * bo, wk * bo, m)) ||
+                      (wq && wk &&
+                       (rows_meet(q_out, ldq_out * bo, wq * bo, k_out, ldk_out * bo, wk * bo, m) ||
+                        rows_meet(q, ldq * bi, wq * bi, k_out, ldk_out * bo, wk * bo, m) ||
+                        rows_meet(k, ldk * bi, wk * bi, q_out, ldq_out * bo, wq * bo, m)));
+    LC_REQUIRE(!meet, LC_ERR_INVALID, "lc_rope: an output overlaps another tensor (only y = x in place is possible)");
+    RpArgs a = {};
+    a.x[0] = q, a.x[1] = k, a.y[0] = q_out, a.y[1] = k_out;
+    a.ldx[0] = ldq, a.ldx[1] = ldk, a.ldy[0] = ldq_out, a.ldy[1] = ldk_out;
+    a.same[0] = q_same, a.same[1] = k_same;
+    a.n_q = (int)n_q_heads, a.n_heads = (int)(n_q_heads + n_kv_heads);
+    a.head_dim = (int)head_dim, a.rope_dim = (int)rope_dim;
+    a.pos = pos, a.freq = freq, a.scale = scale;
+    const bool pairs = layout == LC_ROPE_PAIRS;
+    if (int s = lc_use_device(ctx)) return s;
+    switch (dtype) {
+    case LC_F16: return rope_out<__half>(ctx, out_dtype, a, m, pairs);
+    case LC_BF16: return rope_out<__nv_bfloat16>(ctx, out_dtype, a, m, pairs);
+    default: return rope_out<float>(ctx, out_dtype, a, m, pairs);
+    }
+}
+
+extern "C" int lc_rope_freq_scaled(float *freq, uint32_t rope_dim, float base, int kind, float factor,
+                                   uint32_t orig_ctx, float beta_fast, float beta_slow, float *scale) {
+    LC_REQUIRE(scale && (freq || rope_dim < 2), LC_ERR_INVALID, "lc_rope_freq_scaled: null out");
+    LC_REQUIRE(rope_dim % 2 == 0, LC_ERR_INVALID, "lc_rope_freq_scaled: rope_dim %u must be even", rope_dim);
+    LC_REQUIRE(base > 1.f && base < INFINITY, LC_ERR_INVALID, "lc_rope_freq_scaled: base %g must be above 1", base);
+    LC_REQUIRE(kind >= LC_ROPE_SCALE_NONE && kind <= LC_ROPE_SCALE_YARN, LC_ERR_INVALID,
+               "lc_rope_freq_scaled: bad kind %d", kind);
+    LC_REQUIRE(kind == LC_ROPE_SCALE_NONE || (factor >= 1.f && factor < INFINITY), LC_ERR_INVALID,
+               "lc_rope_freq_scaled: factor %g must be at least 1", factor);
+    LC_REQUIRE(kind != LC_ROPE_SCALE_NTK || rope_dim > 2, LC_ERR_INVALID,
+               "lc_rope_freq_scaled: the NTK base needs rope_dim above 2");
+    LC_REQUIRE(kind != LC_ROPE_SCALE_YARN || (orig_ctx > 0 && beta_slow > 0.f && beta_fast >= beta_slow &&
+                                              beta_fast < INFINITY),
+               LC_ERR_INVALID, "lc_rope_freq_scaled: YaRN needs orig_ctx > 0 and beta_fast >= beta_slow > 0");
+    *scale = 1.f;
+    const double d = rope_dim, b = base, f = factor;
+    const double used = kind == LC_ROPE_SCALE_NTK ? b * pow(f, d / (d - 2)) : b;
+    // YaRN: the pair whose wavelength fits `beta` times into the original context
+    double low = 0, high = 0;
+    if (kind == LC_ROPE_SCALE_YARN) {
+        auto pair_of = [&](double beta) { return d * log(orig_ctx / (beta * 2 * M_PI)) / (2 * log(b)); };
+        low = std::max(floor(pair_of(beta_fast)), 0.0);
+        high = std::min(ceil(pair_of(beta_slow)), d - 1);
+        *scale = (float)(0.1 * log(f) + 1);
+    }
+    for (uint32_t i = 0; i < rope_dim / 2; i++) {
+        double w = pow(used, -2.0 * i / d);
+        if (kind == LC_ROPE_SCALE_LINEAR) w /= f;
+        if (kind == LC_ROPE_SCALE_YARN) {
+            const double t = std::min(1.0, std::max(0.0, (i - low) / std::max(high - low, 1e-3)));
+            w = w * (1 - t) + w / f * t;  // t = 0: short wavelengths, as they are
+        }
+        freq[i] = (float)w;
+    }
+    return LC_OK;
+}

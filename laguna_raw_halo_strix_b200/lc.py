@@ -37,6 +37,14 @@ Q4_K_DFLASH_CPU = 1012
 HALF_REF = 0
 HALF_IEEE = 1
 
+ROPE_HALF = 0  # lc_rope layouts
+ROPE_PAIRS = 1
+
+ROPE_SCALE_NONE = 0  # lc_rope_freq_scaled kinds
+ROPE_SCALE_LINEAR = 1
+ROPE_SCALE_NTK = 2
+ROPE_SCALE_YARN = 3
+
 LOAD_BF16_NATIVE = 1  # lc_dflash_load_gguf_ex flag
 
 _STATUS = {0: "LC_OK", 1: "LC_ERR_INVALID", 2: "LC_ERR_UNSUPPORTED", 3: "LC_ERR_CUDA", 4: "LC_ERR_OOM",
@@ -54,6 +62,7 @@ _lib = None
 
 _vp = C.c_void_p
 _u32 = C.c_uint32
+_u64 = C.c_uint64
 _f = C.c_float
 _sz = C.c_size_t
 _i = C.c_int
@@ -107,7 +116,10 @@ SIGNATURES = {
     "lc_softplus": (_i, [_vp, _vp, _vp, _u32]),
     "lc_enc_aux_norm": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _f]),
     "lc_mha_attn": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _f, _u32, _u32]),
+    "lc_rope": (_i, [_vp, _i, _i, _i, _vp, _u64, _vp, _u64, _u32, _vp, _u64, _vp, _u64, _u32, _vp, _vp, _u32, _u32,
+                     _u32, _f]),
     "lc_rope_freq": (_i, [C.POINTER(_f), _u32, _f]),
+    "lc_rope_freq_scaled": (_i, [C.POINTER(_f), _u32, _f, _i, _f, _u32, _f, _f, C.POINTER(_f)]),
     "lc_pack_key": (C.c_uint64, [_f, _u32]),
     "lc_key_value": (_f, [C.c_uint64]),
     "lc_key_index": (_u32, [C.c_uint64]),
@@ -346,6 +358,13 @@ class Context:
         check(self.L.lc_qk_norm_rope(self.h, ptr(x), ptr(w), ptr(freq), ptr(out), m, n_heads, head_dim, rope_dim,
                                      eps, pos0), "lc_qk_norm_rope")
 
+    def rope(self, dtype, out_dtype, layout, q, q_out, n_q_heads, k, k_out, n_kv_heads, pos, freq, m, head_dim,
+             rope_dim, scale=1.0, ldq=0, ldq_out=0, ldk=0, ldk_out=0):
+        """lc_rope: q and k (either may be None with 0 heads) rotated at pos[row]; strides in elements, 0 = packed."""
+        check(self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k), ldk,
+                             ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale),
+              "lc_rope")
+
     def activation(self, gate, up, h, n):
         check(self.L.lc_activation(self.h, ptr(gate), ptr(up), ptr(h), n), "lc_activation")
 
@@ -419,3 +438,15 @@ def rope_freq(rope_dim: int, base: float = 500000.0):
     f = np.empty(max(rope_dim // 2, 1), np.float32)
     check(lib().lc_rope_freq(f.ctypes.data_as(C.POINTER(C.c_float)), rope_dim, base), "lc_rope_freq")
     return f[: rope_dim // 2]
+
+
+def rope_freq_scaled(rope_dim: int, base: float = 500000.0, kind: int = ROPE_SCALE_NONE, factor: float = 1.0,
+                     orig_ctx: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """(frequencies [rope_dim / 2], the scale Context.rope takes with them); see lc_rope_freq_scaled."""
+    import numpy as np
+
+    f = np.empty(max(rope_dim // 2, 1), np.float32)
+    scale = C.c_float(0.0)
+    check(lib().lc_rope_freq_scaled(f.ctypes.data_as(C.POINTER(C.c_float)), rope_dim, base, kind, factor, orig_ctx,
+                                    beta_fast, beta_slow, C.byref(scale)), "lc_rope_freq_scaled")
+    return f[: rope_dim // 2], float(scale.value)
