@@ -233,6 +233,46 @@ int lc_mha_attn(lc_ctx *ctx, const float *q, const float *k, const float *v,
                 float *out, uint32_t m, uint32_t n_q_heads, uint32_t n_kv_heads,
                 uint32_t head_dim, uint32_t seq_len, float scale,
                 uint32_t q_pos0, uint32_t causal);
+/* The K/V rows that a batch of sequences attends to (device pointers): those of
+ * a prefix that all sequences share, and each sequence's own behind it.  A row
+ * holds n_kv_heads * head_dim elements; ld_* are elements between rows and
+ * own_stride those between sequences (0: packed).  Rows start on 16-byte
+ * boundaries.  Own rows from own_len[i] on may hold anything; rows below it, and
+ * the prefix, are finite numbers (a masked weight is 0, and 0 * inf is NaN). */
+typedef struct {
+    const void *k_prefix;  /* [prefix_len] rows */
+    const void *v_prefix;
+    uint64_t ld_prefix;
+    uint32_t prefix_len;
+    uint32_t own_cap;      /* rows of a sequence's own part, at most: bounds own_len and the launch */
+    const void *k_own;     /* [n_seqs][own_cap] rows */
+    const void *v_own;
+    uint64_t ld_own;
+    uint64_t own_stride;
+    const int32_t *own_len;   /* [n_seqs] own rows in use (held to 0..own_cap); not read if own_cap is 0 */
+    const int32_t *seq_start; /* [n_seqs + 1] query rows of sequence i: [seq_start[i], seq_start[i + 1]) */
+    uint32_t n_seqs;
+} lc_prefix_kv;
+/* Attention of the batch, beside lc_mha_attn: for each query row of q [rows,
+ * n_q_heads * head_dim] and each head, softmax(scale q . k) v over the prefix
+ * and its sequence's own rows, the query heads of a group sharing a KV head.  A
+ * sequence of c query rows holds its last c own positions: with causal, row t
+ * of it sees own rows 0 .. own_len - c + t (none where that is negative),
+ * without, all own_len.  A row that sees no key gets 0.  The prefix's products
+ * are formed once for the batch.  q, k, v are of type dtype (LC_F16 or LC_BF16),
+ * out of that type or LC_F32; softmax and sums in f32, weights rounded to dtype
+ * (to twice its digits for LC_F32 outputs).  seq_start is non-decreasing within
+ * 0..rows (values outside are held inside); rows of no sequence stay as they
+ * are in out.  Lengths and starts are read on the device, so a captured call
+ * can be replayed as sequences grow up to own_cap.  head_dim 64 or 128, scale
+ * >= 0, ldq / ldo elements between rows (0: packed), 16-byte aligned rows.
+ * Partial states live in the context's scratch: graphs captured on one context
+ * are not replayed at the same time, and capture needs a call of the same size
+ * before it.  The reference attends one sequence at a time
+ * (kernels/mha_attn.comp:31-72). */
+int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void *q, uint64_t ldq, const lc_prefix_kv *kv,
+                   void *out, uint64_t ldo, uint32_t rows, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                   float scale, uint32_t causal);
 /* Rotary positions of q [m, n_q_heads, head_dim] and k [m, n_kv_heads,
  * head_dim] in one launch, beside lc_qk_norm_rope, for a batch of rows that sit
  * at positions of their own.  Pair i of a head (i < rope_dim / 2) is turned by
@@ -299,6 +339,41 @@ int lc_argmax_rows(lc_ctx *ctx, const float *logits, uint32_t m, uint32_t n,
 int lc_lm_head_argmax(lc_ctx *ctx, int dtype, const float *x, const void *w,
                       uint32_t m, uint32_t k, uint32_t n_local,
                       uint32_t row_offset, uint64_t *keys, float *logits);
+
+/* What lc_logits_process applies to a batch of rows; every pointer is a device
+ * pointer, and NULL switches its rule off.  Lists are ragged: row i's entries
+ * are [start[i], start[i + 1]) of an array of *_len entries (starts outside it
+ * are held inside it). */
+typedef struct {
+    const int32_t *hist;       /* past tokens: prompt, then generated */
+    const int32_t *hist_start; /* [m + 1] */
+    const int32_t *gen_start;  /* [m] where row i's generated tokens begin in hist; NULL: all are generated */
+    uint64_t hist_len;
+    const float *repetition;   /* [m] > 0, 1 = none: seen tokens x > 0 ? x / r : x * r */
+    const float *frequency;    /* [m] times the generated count, subtracted */
+    const float *presence;     /* [m] subtracted once from generated tokens */
+    const int32_t *bias_tok;   /* tokens with a bias; of a row's entries for one token the last counts */
+    const float *bias;         /* their biases, added */
+    const int32_t *bias_start; /* [m + 1] */
+    uint64_t bias_len;
+    const uint32_t *mask;      /* [n_masks][mask_ld] words, bit t of a mask (bit t % 32 of word t / 32): token t allowed */
+    const int32_t *mask_row;   /* [m] which mask a row takes, none if outside 0..n_masks - 1; NULL: mask i for row i */
+    uint64_t mask_ld;          /* words between masks */
+    uint32_t n_masks;
+} lc_logits_rules;
+/* Penalties for repeated tokens, biases and grammar masks on logits [m, n], and
+ * the row's best token, beside lc_argmax_rows; in this order, each operation
+ * rounded once to f32: repetition, frequency * count, presence, bias, masked
+ * tokens to -inf.  ld / ld_out: floats between rows (0: n).  out may be logits
+ * itself (same stride), or NULL when only keys are wanted; other overlaps are
+ * LC_ERR_INVALID.  keys[m] (optional) get lc_pack_key(max, token), ties to the
+ * larger token; a row with every token masked has (-inf, its last token).
+ * Vocab shards: the rows hold tokens row_offset .. row_offset + n - 1; token ids
+ * in lists and mask bits stay global, ids outside the shard are skipped, and
+ * the shards' keys combine by lc_comm_allreduce_max_keys.  One launch, no
+ * scratch.  The reference takes the plain argmax (src/lib.rs:456-464). */
+int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, float *out, uint64_t ld_out, uint32_t m,
+                      uint32_t n, uint32_t row_offset, const lc_logits_rules *rules, uint64_t *keys);
 
 /* ---- vocab-sharded lm_head over several GPUs (NCCL owned by the library) -- */
 

@@ -30,6 +30,8 @@ struct lc_ctx {
     // Grow-only scratch slots (see LC_SCRATCH_*).
     void *scratch[8] = {};
     size_t scratch_bytes[8] = {};
+    // Blocks that lc_scratch_kept replaced, freed by lc_destroy.
+    std::vector<void *> kept;
     // Device word that kernels set (atomicOr of LC_DEV_*) when a bounded wait
     // gives up; read and cleared by lc_device_status().  Allocated at init.
     unsigned *dev_status = nullptr;
@@ -63,6 +65,7 @@ enum {
     LC_SCRATCH_FIXUP = 4,
     LC_SCRATCH_FFN = 5,
     LC_SCRATCH_HOSTIO = 6,
+    LC_SCRATCH_PREFIX = 7,  // lc_scratch_kept
     LC_SCRATCH_COUNT = 8
 };
 // Grow-only scratch slot of at least `bytes` (256-byte aligned).  Returns
@@ -71,6 +74,12 @@ enum {
 void *lc_scratch(lc_ctx *ctx, int slot, size_t bytes);
 // Same, and a newly allocated slot is zero-filled (on the context's stream).
 void *lc_scratch_zeroed(lc_ctx *ctx, int slot, size_t bytes);
+// Scratch slot that a captured graph may go on using after the slot has grown:
+// a replaced block stays allocated until lc_destroy, and each block is at least
+// twice the last, so all of them together hold less than twice the largest.
+// Growing during a stream capture is LC_ERR_UNSUPPORTED (allocate by a call of
+// the same size before).
+int lc_scratch_kept(lc_ctx *ctx, int slot, size_t bytes, void **out);
 // Resolve ctx->static_pack with ctx->device current (lc_proj.cu; called by lc_init).
 int lc_static_pack_resolve(lc_ctx *ctx);
 // Make ctx->device current on this thread.
@@ -80,6 +89,11 @@ int lc_use_device(lc_ctx *ctx);
 // made while a stream is being captured into a CUDA graph) do not touch the
 // driver again.
 int lc_set_smem_attr(const void *kernel, size_t bytes);
+
+// Do the m rows of wa bytes, pa apart, at a share a byte with the m rows of wb
+// bytes, pb apart, at b?  Exact for equal pitches (columns of one buffer);
+// otherwise whole extents are compared.
+bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m);
 
 #define LC_REQUIRE(cond, code, ...)             \
     do {                                        \

@@ -1,0 +1,257 @@
+// lc_logits.cu -- penalties for repeated tokens, biases and grammar masks on
+// logits, with the row's argmax key.
+//
+// For token j of a row (r, f, p its repetition, frequency and presence
+// penalties, c_j how often the row generated j):
+//   x = logit;  seen in the row's history: x = x > 0 ? x / r : x * r
+//   c_j > 0:    x = (x - f * c_j) - p
+//   biased:     x = x + bias (the last of the row's entries for j)
+//   masked:     x = -inf
+// each operation rounded once, in this order, so that equal inputs give equal
+// bits whatever the launch shape.
+//
+// Bound by reading and writing the logits once.  The history and the bias list
+// are scattered: a CTA owns a slice of the vocabulary, counts the row's tokens
+// that fall into it in shared memory (integer adds, and a maximum over list
+// positions for biases: no order changes a result), then streams the slice.
+// A row is one cluster of CTAs, so the row's key is reduced over distributed
+// shared memory and the whole call is one launch without a workspace.
+#include <math.h>
+
+#include <algorithm>
+
+#include "lc_internal.cuh"
+#include "lc_sm100.cuh"
+
+namespace {
+
+constexpr int kLgThreads = 512;
+constexpr int kLgSlice = 8192;  // tokens counted at a time
+constexpr uint32_t kLgListMax = 0x7FFF0000u;  // list positions + kLgThreads stay int32
+constexpr uint32_t kSeen = 0x80000000u;  // of a counter: in the history (low bits: generated count)
+
+struct LgArgs {
+    const float *x;
+    float *y;
+    uint64_t ldx, ldy;
+    uint32_t n, row_offset, part;  // part: tokens of a CTA of the cluster, a multiple of 128
+    lc_logits_rules r;
+    uint64_t *keys;
+    int vec_x, vec_y;  // rows 16-byte aligned
+};
+
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t v;
+    asm("mov.u32 %0, %%cluster_nctaid.x;\n" : "=r"(v));
+    return v;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t v;
+    asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(v));
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+// Store to the same shared variable of CTA `rank` of the cluster.
+__device__ __forceinline__ void cluster_store(uint64_t *p, uint32_t rank, uint64_t v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(at), "l"(v) : "memory");
+}
+
+__device__ __forceinline__ int clamp_index(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+__global__ void __launch_bounds__(kLgThreads) logits_kernel(const LgArgs a) {
+    extern __shared__ __align__(16) uint32_t lg_smem[];
+    __shared__ long long best_warp[kLgThreads / 32];
+    __shared__ uint64_t best_cta[16];
+    uint32_t *cnt = lg_smem;             // [kLgSlice]
+    uint32_t *slot = lg_smem + kLgSlice;  // [kLgSlice], only with a bias list: 1 + list position
+    const uint32_t cl = cluster_size(), rank = cluster_rank();
+    const uint32_t row = blockIdx.x / cl;
+    const float *x = a.x + (size_t)row * a.ldx;
+    float *y = a.y ? a.y + (size_t)row * a.ldy : nullptr;
+    const lc_logits_rules &r = a.r;
+
+    // the row's lists; indexes from the device are held inside the arrays
+    int h0 = 0, h1 = 0, g0 = 0, b0 = 0, b1 = 0;
+    if (r.hist_start) {
+        h0 = clamp_index(r.hist_start[row], 0, (int)r.hist_len);
+        h1 = clamp_index(r.hist_start[row + 1], h0, (int)r.hist_len);
+        g0 = r.gen_start ? r.gen_start[row] : h0;
+    }
+    if (r.bias_start) {
+        b0 = clamp_index(r.bias_start[row], 0, (int)r.bias_len);
+        b1 = clamp_index(r.bias_start[row + 1], b0, (int)r.bias_len);
+    }
+    const float rep = r.repetition ? r.repetition[row] : 1.f;
+    const float freq = r.frequency ? r.frequency[row] : 0.f;
+    const float pres = r.presence ? r.presence[row] : 0.f;
+    const uint32_t *mask = nullptr;
+    if (r.mask) {
+        const int mr = r.mask_row ? r.mask_row[row] : (int)row;
+        if (mr >= 0 && (uint32_t)mr < r.n_masks) mask = r.mask + (size_t)mr * r.mask_ld;
+    }
+    const bool listed = h1 > h0 || b1 > b0;
+
+    const uint32_t p0 = min(a.n, rank * a.part), p1 = min(a.n, p0 + a.part);
+    int best_ord = INT_MIN;
+    uint32_t best_j = 0;
+    bool any = false;
+    auto value = [&](float v, uint32_t j, uint32_t c, uint32_t s) {
+        if (c) {
+            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            c &= ~kSeen;
+            if (c) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres);
+        }
+        if (s) v = __fadd_rn(v, r.bias[b0 + s - 1]);
+        if (mask) {
+            const uint32_t g = a.row_offset + j;
+            if (!(mask[g >> 5] >> (g & 31) & 1)) v = -INFINITY;
+        }
+        // the order of lc_pack_key: value bits as a signed integer
+        const int b = __float_as_int(v), ord = b ^ ((b >> 31) & 0x7FFFFFFF);
+        if (ord >= best_ord) best_ord = ord, best_j = j, any = true;
+        return v;
+    };
+    for (uint32_t s0 = p0; s0 < p1; s0 += kLgSlice) {
+        const uint32_t len = min((uint32_t)kLgSlice, p1 - s0);
+        if (listed) {
+            for (uint32_t i = threadIdx.x * 4; i < len; i += kLgThreads * 4) {
+                *reinterpret_cast<uint4 *>(cnt + i) = make_uint4(0, 0, 0, 0);
+                if (b1 > b0) *reinterpret_cast<uint4 *>(slot + i) = make_uint4(0, 0, 0, 0);
+            }
+            __syncthreads();
+            const uint32_t first = a.row_offset + s0;  // tokens outside [first, first + len) wrap past len
+            for (int i = h0 + (int)threadIdx.x; i < h1; i += kLgThreads) {
+                const uint32_t t = (uint32_t)r.hist[i] - first;
+                if (t < len) {
+                    if (i >= g0)
+                        atomicAdd(cnt + t, 1u);
+                    else
+                        atomicOr(cnt + t, kSeen);
+                }
+            }
+            for (int i = b0 + (int)threadIdx.x; i < b1; i += kLgThreads) {
+                const uint32_t t = (uint32_t)r.bias_tok[i] - first;
+                if (t < len) atomicMax(slot + t, (uint32_t)(i - b0) + 1u);
+            }
+            __syncthreads();
+        }
+        for (uint32_t i = threadIdx.x * 4; i < len; i += kLgThreads * 4) {
+            const uint32_t j = s0 + i, have = min(4u, len - i);
+            float v[4];
+            if (a.vec_x && have == 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(x + j);
+                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = e < (int)have ? x[j + e] : 0.f;
+            }
+            uint4 c = make_uint4(0, 0, 0, 0), s = c;
+            if (listed) {
+                c = *reinterpret_cast<const uint4 *>(cnt + i);
+                if (b1 > b0) s = *reinterpret_cast<const uint4 *>(slot + i);
+            }
+            const uint32_t cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < (int)have) v[e] = value(v[e], j + e, cc[e], ss[e]);
+            if (y) {
+                if (a.vec_y && have == 4) {
+                    *reinterpret_cast<float4 *>(y + j) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (e < (int)have) y[j + e] = v[e];
+                }
+            }
+        }
+        __syncthreads();  // the counters are read before the next slice clears them
+    }
+    if (!a.keys) return;  // uniform over the cluster
+    // (order, global token) as the signed key of lc_pack_key
+    long long best = any ? (long long)(((uint64_t)(uint32_t)best_ord << 32) | (a.row_offset + best_j)) : LLONG_MIN;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if ((threadIdx.x & 31) == 0) best_warp[threadIdx.x >> 5] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kLgThreads / 32; w++) best = max(best, best_warp[w]);
+        cluster_store(best_cta + rank, 0, (uint64_t)best);
+    }
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0 && threadIdx.x == 0) {
+        for (uint32_t c = 0; c < cl; c++) best = max(best, (long long)best_cta[c]);
+        a.keys[row] = (uint64_t)best;
+    }
+}
+
+}  // namespace
+
+extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, float *out, uint64_t ld_out,
+                                 uint32_t m, uint32_t n, uint32_t row_offset, const lc_logits_rules *rules,
+                                 uint64_t *keys) {
+    LC_REQUIRE(ctx, LC_ERR_INVALID, "lc_logits_process: null ctx");
+    if (m == 0) return LC_OK;
+    LC_REQUIRE(logits && rules && (out || keys), LC_ERR_INVALID, "lc_logits_process: null pointer");
+    LC_REQUIRE(n > 0 && n <= (1u << 30), LC_ERR_INVALID, "lc_logits_process: n %u not in 1..2^30", n);
+    LC_REQUIRE(row_offset <= 0x7FFFFFFFu - n, LC_ERR_INVALID,
+               "lc_logits_process: tokens %u .. + %u do not fit an int32", row_offset, n);
+    LC_REQUIRE(m <= (1u << 24), LC_ERR_UNSUPPORTED, "lc_logits_process: %u rows", m);
+    const lc_logits_rules &r = *rules;
+    LC_REQUIRE(r.hist_len <= kLgListMax && r.bias_len <= kLgListMax, LC_ERR_UNSUPPORTED,
+               "lc_logits_process: token lists above %u entries", kLgListMax);
+    LC_REQUIRE((!r.hist_len || r.hist) && (!r.hist || r.hist_start), LC_ERR_INVALID,
+               "lc_logits_process: hist and hist_start go together");
+    LC_REQUIRE((!r.bias_len || (r.bias_tok && r.bias)) && (!r.bias_tok || r.bias_start), LC_ERR_INVALID,
+               "lc_logits_process: bias_tok, bias and bias_start go together");
+    const uint64_t words = ((uint64_t)row_offset + n + 31) / 32;
+    LC_REQUIRE(!r.mask || r.mask_ld >= words, LC_ERR_INVALID,
+               "lc_logits_process: masks of %llu words do not reach token %llu", (unsigned long long)r.mask_ld,
+               (unsigned long long)row_offset + n);
+    LC_REQUIRE(!r.mask || r.mask_row || r.n_masks >= m, LC_ERR_INVALID,
+               "lc_logits_process: %u masks for %u rows and no mask_row", r.n_masks, m);
+    LC_REQUIRE(!r.mask || r.mask_ld <= (1ull << 40), LC_ERR_INVALID, "lc_logits_process: mask stride too large");
+    if (!ld) ld = n;
+    if (!ld_out) ld_out = n;
+    LC_REQUIRE(ld >= n && (!out || ld_out >= n), LC_ERR_INVALID, "lc_logits_process: a row stride is shorter than n");
+    LC_REQUIRE(ld <= (1ull << 58) / m && ld_out <= (1ull << 58) / m, LC_ERR_INVALID,
+               "lc_logits_process: row stride too large");
+    LC_REQUIRE((((uintptr_t)logits | (uintptr_t)out | (uintptr_t)r.hist | (uintptr_t)r.hist_start |
+                 (uintptr_t)r.gen_start | (uintptr_t)r.repetition | (uintptr_t)r.frequency | (uintptr_t)r.presence |
+                 (uintptr_t)r.bias_tok | (uintptr_t)r.bias | (uintptr_t)r.bias_start | (uintptr_t)r.mask |
+                 (uintptr_t)r.mask_row) & 3) == 0 && ((uintptr_t)keys & 7) == 0,
+               LC_ERR_INVALID, "lc_logits_process: a pointer is not aligned to its type");
+    LC_REQUIRE(!out || (out == logits && ld == ld_out) ||
+                   !lc_rows_meet(logits, ld * 4, n * 4ull, out, ld_out * 4, n * 4ull, m),
+               LC_ERR_INVALID, "lc_logits_process: out overlaps logits (only out = logits in place is possible)");
+    if (int s = lc_use_device(ctx)) return s;
+    LgArgs a = {};
+    a.x = logits, a.y = out, a.ldx = ld, a.ldy = ld_out, a.n = n, a.row_offset = row_offset, a.r = r, a.keys = keys;
+    a.vec_x = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
+    a.vec_y = ((uintptr_t)out & 15) == 0 && ld_out % 4 == 0;
+    // CTAs of a row's cluster: at most 8 (the portable size), each with at least
+    // 2048 tokens
+    uint32_t cl = 8;
+    while (cl > 1 && n / cl < 2048) cl /= 2;
+    a.part = ((n + cl - 1) / cl + 127) / 128 * 128;
+    const size_t smem = (size_t)kLgSlice * 4 * (r.bias_len ? 2 : 1);
+    if (int s = lc_set_smem_attr((const void *)logits_kernel, smem)) return s;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(m * cl);
+    cfg.blockDim = dim3(kLgThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cl;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    LC_CUDA(cudaLaunchKernelEx(&cfg, logits_kernel, (const LgArgs)a));
+    return lc_after_launch(ctx, "lc_logits_process");
+}

@@ -1,0 +1,758 @@
+// lc_prefix_attn.cu -- attention of a batch of sequences that share the K/V rows
+// of a prefix and have rows of their own behind it.
+//
+// out_r = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q_r . k_j), j over the
+// prefix and the row's visible own keys.  The softmax of the joined axis splits
+// into partial states (m, l, O) that merge exactly, so the prefix is computed
+// once for the query rows of the whole batch (every sequence and every query
+// head of a KV head are rows of one matrix product against it), the own parts
+// per sequence, and a small kernel merges.
+//
+// One CTA takes an item: up to 128 query rows of one KV head against a range of
+// the virtual key axis [prefix | own rows of its sequence].  Per tile of 128 keys
+//   S = Q K^T   tcgen05, Q and K K-major in shared memory, S in TMEM 0..127
+//   P           softmax warps, one thread a row, written over S as 16-bit pairs
+//               (and a second plane of what the rounding lost, for f32 outputs)
+//   O += P V    tcgen05, P from TMEM, V read MN-major as it lies in memory
+// K and V tiles come by TMA.  Roles: warps 0-3 softmax, 4 loads, 5 MMA.  S and P
+// share their TMEM columns, so within a CTA a tile's products and its softmax
+// alternate; two CTAs share an SM (256 TMEM columns and 98 KB each) and fill
+// each other's gaps.
+#include <math.h>
+
+#include <algorithm>
+
+#include <cuda_bf16.h>
+
+#include "lc_internal.cuh"
+#include "lc_sm100.cuh"
+
+namespace {
+
+constexpr int kPaRows = 128, kPaKeys = 128;
+constexpr int kPaThreads = 192;
+constexpr int kPaBoxRows = 32;             // key rows of one TMA copy
+constexpr uint32_t kPaPlane = 128 * 128;   // 128 rows x 64 16-bit elements (one swizzle span)
+constexpr uint32_t kPaColS = 0, kPaColO = 128, kPaTmemCols = 256;
+constexpr uint32_t kPaMaxLen = 0x3FFFF000u;  // prefix_len + own_cap: ranges of the key axis stay int32
+
+// Shared memory: Q, K, V tiles of HD / 64 planes each, then the barriers.
+template <int HD>
+struct PaSmem {
+    static constexpr uint32_t kTile = HD / 64 * kPaPlane;
+    static constexpr uint32_t kQ = 0, kK = kTile, kV = 2 * kTile, kBar = 3 * kTile;
+    static constexpr uint32_t kBytes = kBar + 64 + 1024;  // + slack to 1024-align the base
+};
+
+struct PaArgs {
+    const void *q;
+    void *out;
+    uint64_t ldq, ldo;
+    int rows, n_q, n_kv, group;
+    int prefix_len, own_cap, n_seqs;
+    const int32_t *own_len, *seq_start;
+    float scale_log2;  // scale * log2(e)
+    int causal;
+    // plan: items 0 .. prefix_items - 1 take the prefix for rows of all
+    // sequences, the rest rows of one sequence over [seq_from, end) of the
+    // virtual axis
+    int prefix_items, row_tiles, prefix_keys;
+    int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
+    int direct;         // one split covers everything: items write out
+    float *o_part;      // [split][row][head][HD], unnormalised
+    float2 *ml_part;    // [split][row][head]: (m in log2 units, l)
+    unsigned *status;
+};
+
+// Rows r0 .. r0 + nrows - 1 (row = token * group + head within the group) of
+// one KV head against prefix keys [p0, p1) and keys [o0, o1) of sequence seq.
+struct PaJob {
+    int r0, nrows, p0, p1, o0, o1, seq;
+    int pos0;  // own position of token t is pos0 + t
+    __device__ __forceinline__ int prefix_tiles() const { return (p1 - p0 + kPaKeys - 1) / kPaKeys; }
+    __device__ __forceinline__ int tiles() const { return prefix_tiles() + (o1 - o0 + kPaKeys - 1) / kPaKeys; }
+    // tile i: first key, keys, own or prefix
+    __device__ __forceinline__ void tile(int i, int &key, int &nk, bool &own) const {
+        const int np = prefix_tiles();
+        own = i >= np;
+        key = own ? o0 + (i - np) * kPaKeys : p0 + i * kPaKeys;
+        nk = min(kPaKeys, (own ? o1 : p1) - key);
+    }
+};
+
+struct PaItem {
+    int hk, split, rt, rt_step, rt_end;  // row tiles rt, rt + rt_step, .. < rt_end
+    int start, count, len, seq, v0, v1;
+};
+
+__device__ __forceinline__ PaItem pa_item(const PaArgs &a) {
+    PaItem t;
+    int i = blockIdx.x;
+    if (i < a.prefix_items) {
+        t.hk = i % a.n_kv;
+        i /= a.n_kv;
+        t.rt = i % a.row_tiles;
+        t.split = i / a.row_tiles;
+        t.rt_step = 1 << 24;
+        t.start = 0, t.count = a.rows, t.len = 0, t.seq = 0;
+        t.v0 = t.split * a.prefix_keys;
+        t.v1 = min(a.prefix_len, t.v0 + a.prefix_keys);
+    } else {
+        i -= a.prefix_items;
+        t.hk = i % a.n_kv;
+        i /= a.n_kv;
+        t.seq = i % a.n_seqs;
+        i /= a.n_seqs;
+        t.rt = i % a.seq_lanes;
+        const int sp = i / a.seq_lanes;
+        t.split = a.prefix_splits + sp;
+        t.rt_step = a.seq_lanes;
+        // values from the device are held inside the arrays
+        t.start = min(max(a.seq_start[t.seq], 0), a.rows);
+        t.count = min(max(a.seq_start[t.seq + 1], t.start), a.rows) - t.start;
+        t.len = a.own_len ? min(max(a.own_len[t.seq], 0), a.own_cap) : 0;
+        t.v0 = a.seq_from + sp * a.seq_keys;
+        t.v1 = min(a.prefix_len + a.own_cap, t.v0 + a.seq_keys);
+    }
+    t.rt_end = (t.count * a.group + kPaRows - 1) / kPaRows;
+    return t;
+}
+
+__device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int rt) {
+    PaJob j;
+    const int first = rt * kPaRows;  // within the item's rows
+    j.r0 = t.start * a.group + first;
+    j.nrows = min(kPaRows, t.count * a.group - first);
+    j.seq = t.seq;
+    j.pos0 = t.len - t.count - t.start;
+    j.p0 = min(t.v0, a.prefix_len), j.p1 = min(t.v1, a.prefix_len);
+    j.o0 = max(t.v0, a.prefix_len) - a.prefix_len;
+    j.o1 = min(max(t.v1, a.prefix_len) - a.prefix_len, t.len);
+    if (a.causal) j.o1 = min(j.o1, j.pos0 + (j.r0 + j.nrows - 1) / a.group + 1);  // the last row's reach
+    j.o1 = max(j.o1, j.o0);
+    return j;
+}
+
+// A bounded wait that, once it has given up, is not repeated: the launch is
+// reported as failed, so what follows only has to end.
+struct PaWait {
+    unsigned *status;
+    bool ok = true;
+    __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity)) {
+            ok = false;
+            atomicOr(status, LC_DEV_WAIT_TIMEOUT);
+        }
+    }
+};
+
+__device__ __forceinline__ void tma_load_2d_plain(void *dst, const CUtensorMap *tm, int x, int y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];\n" ::"r"(smem_addr(dst)),
+        "l"(tm), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_plain(void *dst, const CUtensorMap *tm, int x, int y, int z,
+                                                  uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];\n" ::"r"(smem_addr(dst)),
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// MN-major operand with the 128-byte swizzle: 64 MN elements (128 bytes) a row,
+// one row per K, groups of 8 K 1024 bytes apart (SBO), the next 64 MN elements
+// `mn_stride` bytes on (LBO).
+__device__ __forceinline__ uint64_t pa_desc_mn(uint32_t saddr, uint32_t mn_stride) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((mn_stride >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+template <class T>
+__host__ __device__ constexpr uint32_t pa_idesc(int n, bool b_mn) {
+    constexpr uint32_t bf = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
+    return umma_idesc_f16(128, n) | (bf << 7) | (bf << 10) | (b_mn ? 1u << 16 : 0u);
+}
+
+// 32 consecutive TMEM columns of this thread's lane (complete after tmem_ld_wait).
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+#define LC_U(i) "r"(__float_as_uint(v[i]))
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+        LC_U(0), LC_U(1), LC_U(2), LC_U(3), LC_U(4), LC_U(5), LC_U(6), LC_U(7), LC_U(8), LC_U(9), LC_U(10), LC_U(11),
+        LC_U(12), LC_U(13), LC_U(14), LC_U(15), LC_U(16), LC_U(17), LC_U(18), LC_U(19), LC_U(20), LC_U(21), LC_U(22),
+        LC_U(23), LC_U(24), LC_U(25), LC_U(26), LC_U(27), LC_U(28), LC_U(29), LC_U(30), LC_U(31)
+        : "memory");
+#undef LC_U
+}
+
+// 2^x to about 2 ulp, 0 below the normal range.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// (a, b) as a pair of T, and what that lost.
+template <class T>
+__device__ __forceinline__ uint32_t pa_pack(float a, float b, float &la, float &lb);
+template <>
+__device__ __forceinline__ uint32_t pa_pack<__half>(float a, float b, float &la, float &lb) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    la = a - f.x, lb = b - f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pa_pack<__nv_bfloat16>(float a, float b, float &la, float &lb) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const float2 f = __bfloat1622float2(h);
+    la = a - f.x, lb = b - f.y;
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 4 consecutive outputs.
+__device__ __forceinline__ void pa_store4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+template <class T>
+__device__ __forceinline__ void pa_store4(T *p, float4 v) {
+    float l;
+    uint2 u;
+    u.x = pa_pack<T>(v.x, v.y, l, l), u.y = pa_pack<T>(v.z, v.w, l, l);
+    *reinterpret_cast<uint2 *>(p) = u;
+}
+
+template <class T, class TO, int HD>
+__global__ void __launch_bounds__(kPaThreads, 2)
+    prefix_attn_kernel(const __grid_constant__ CUtensorMap kp, const __grid_constant__ CUtensorMap vp,
+                       const __grid_constant__ CUtensorMap ko, const __grid_constant__ CUtensorMap vo,
+                       const __grid_constant__ PaArgs a) {
+    using L = PaSmem<HD>;
+    constexpr bool kTwoPlanes = std::is_same<TO, float>::value;  // P as hi + lo
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *k_full = bar, *v_full = bar + 1, *s_full = bar + 2, *p_ready = bar + 3, *pv_done = bar + 4,
+             *q_ready = bar + 5;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 6);
+    const uint32_t sbase = smem_addr(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    griddep_launch_dependents();  // the merge kernel may be scheduled once the last items run
+    if (threadIdx.x == 0) {
+        mbar_init(k_full, 1);
+        mbar_init(v_full, 1);
+        mbar_init(s_full, 1);
+        mbar_init(p_ready, kPaRows);
+        mbar_init(pv_done, 1);
+        mbar_init(q_ready, kPaRows);
+        mbar_init_fence();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
+                     "r"(kPaTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = *tslot;
+    const PaItem item = pa_item(a);
+    PaWait wait{a.status};
+    uint32_t it = 0;  // tiles so far: every barrier completes once per tile (q_ready once per job)
+
+    if (warp == 4) {  // ---- loads
+        if (lane == 0) {
+            for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
+                const PaJob j = pa_job(a, item, rt);
+                const int n = j.tiles();
+                for (int i = 0; i < n; i++, it++) {
+                    int key, nk;
+                    bool own;
+                    j.tile(i, key, nk, own);
+                    const int boxes = (nk + kPaBoxRows - 1) / kPaBoxRows;
+                    const uint32_t bytes = boxes * kPaBoxRows * HD * 2;
+                    const int x = item.hk * HD;
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        // the slot is free once the products that read it are done
+                        if (it) wait(kv ? pv_done : s_full, (it - 1) & 1);
+                        if (!wait.ok) break;
+                        uint64_t *b = kv ? v_full : k_full;
+                        unsigned char *dst = smem + (kv ? L::kV : L::kK);
+                        mbar_expect_tx(b, bytes);
+                        for (int c = 0; c < HD / 64; c++)
+                            for (int r = 0; r < boxes; r++) {
+                                unsigned char *d = dst + c * kPaPlane + r * (kPaBoxRows * 128);
+                                if (own)
+                                    tma_load_3d_plain(d, kv ? &vo : &ko, x + 64 * c, key + kPaBoxRows * r, j.seq, b);
+                                else
+                                    tma_load_2d_plain(d, kv ? &vp : &kp, x + 64 * c, key + kPaBoxRows * r, b);
+                            }
+                    }
+                    if (!wait.ok) break;
+                }
+                if (!wait.ok) break;
+            }
+            if (!wait.ok) {  // copies of this CTA still in flight
+                mbar_wait(k_full, it & 1);
+                mbar_wait(v_full, it ? (it - 1) & 1 : 0);
+            }
+        }
+    } else if (warp == 5) {  // ---- products
+        uint32_t jobs = 0;
+        for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
+            const PaJob j = pa_job(a, item, rt);
+            const int n = j.tiles();
+            if (n == 0) continue;
+            wait(q_ready, jobs++ & 1);
+            for (int i = 0; i < n && wait.ok; i++, it++) {
+                int key, nk;
+                bool own;
+                j.tile(i, key, nk, own);
+                wait(k_full, it & 1);
+                if (!wait.ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
+#pragma unroll
+                    for (int s = 0; s < HD / 16; s++) {
+                        const uint64_t o = ((s >> 2) * kPaPlane + (s & 3) * 32) >> 4;
+                        umma_f16_ss(tbase + kPaColS, qd + o, kd + o, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
+                    }
+                    umma_commit(s_full);
+                }
+                __syncwarp();
+                wait(v_full, it & 1);
+                // keys of the tile's last 16-key step that do not exist: their P is 0,
+                // and 0 times whatever lies there must not be NaN
+                const int steps = (nk + 15) >> 4, gone = steps * 16 - nk;
+                if (gone && wait.ok) {
+                    for (int e = lane; e < gone * (HD / 8); e += 32) {
+                        const int row = nk + e / (HD / 8), ch = e % (HD / 8);
+                        *reinterpret_cast<uint4 *>(smem + L::kV + (ch >> 3) * kPaPlane + row * 128 + (ch & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                wait(p_ready, it & 1);
+                if (!wait.ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
+                    constexpr uint32_t id = pa_idesc<T>(HD, true);
+                    for (int s = 0; s < steps; s++) {
+                        umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 8 * s, vd + ((s * 2048) >> 4), id,
+                                    (i | s) ? 1u : 0u);
+                        if constexpr (kTwoPlanes)
+                            umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 64 + 8 * s, vd + ((s * 2048) >> 4), id, 1u);
+                    }
+                    umma_commit(pv_done);
+                }
+                __syncwarp();
+            }
+            if (!wait.ok) break;
+        }
+        if (!wait.ok && it) mbar_wait(pv_done, (it - 1) & 1);
+    } else {  // ---- softmax: thread = row = TMEM lane
+        const int row = threadIdx.x;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO;
+        for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
+            const PaJob j = pa_job(a, item, rt);
+            const int n = j.tiles();
+            const bool real = row < j.nrows, busy = 32 * warp < j.nrows;
+            const int gq = j.r0 + min(row, j.nrows - 1), tok = gq / a.group;
+            const int head = item.hk * a.group + gq - tok * a.group;
+            const int pos = j.pos0 + tok;
+            float m_ref = -INFINITY, l = 0.f;
+            if (n) {
+                // Q rows (the last job's products have been waited for below)
+                for (int e = row; e < kPaRows * (HD / 8); e += kPaRows) {
+                    const int r = e / (HD / 8), ch = e % (HD / 8);
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < j.nrows) {
+                        const int g = j.r0 + r, t = g / a.group, h = item.hk * a.group + g - t * a.group;
+                        v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (size_t)t * a.ldq +
+                                                             (size_t)h * HD + 8 * ch);
+                    }
+                    *reinterpret_cast<uint4 *>(smem + L::kQ + (ch >> 3) * kPaPlane + r * 128 +
+                                               (((ch & 7) ^ (r & 7)) << 4)) = v;
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(q_ready);
+            }
+            for (int i = 0; i < n; i++, it++) {
+                int key, nk;
+                bool own;
+                j.tile(i, key, nk, own);
+                wait(s_full, it & 1);
+                __syncwarp();
+                tc_fence_after();
+                if (busy) {
+                    // keys [0, lim) of the tile are visible to the row
+                    const int lim = own && a.causal ? min(max(pos + 1 - key, 0), nk) : nk;
+                    const bool all = __all_sync(0xffffffffu, lim == kPaKeys);
+                    float top = -INFINITY;
+                    float s[32];
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld32(ts + 32 * c, s);
+                        tmem_ld_wait();
+                        tmem_regs_ready(s);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (all || 32 * c + e < lim) top = fmaxf(top, s[e]);
+                    }
+                    const float m_new = fmaxf(m_ref, top * a.scale_log2);
+                    // O is rescaled only when the maximum has grown by more than 2^8 since
+                    // the last time: weights up to 256 are as exact, and fit f16
+                    if (i == 0) {
+                        m_ref = m_new;
+                    } else if (__any_sync(0xffffffffu, m_new > m_ref + 8.f)) {
+                        const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
+                        wait(pv_done, (it - 1) & 1);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; c++) {
+                            tmem_ld32(to + 32 * c, s);
+                            tmem_ld_wait();
+                            tmem_regs_ready(s);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) s[e] *= f;
+                            tmem_st32(to + 32 * c, s);
+                        }
+                        tmem_st_wait();
+                        l *= f;
+                        m_ref = m_new;
+                    }
+                    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+                    auto weights = [&](float (&x)[32], int c) {
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            float p0 = exp2_fast(fmaf(x[2 * e], a.scale_log2, -m_use));
+                            float p1 = exp2_fast(fmaf(x[2 * e + 1], a.scale_log2, -m_use));
+                            if (!all) {
+                                if (32 * c + 2 * e >= lim) p0 = 0.f;
+                                if (32 * c + 2 * e + 1 >= lim) p1 = 0.f;
+                            }
+                            l += p0 + p1;
+                            float r0, r1;
+                            hi[e] = pa_pack<T>(p0, p1, r0, r1);
+                            if constexpr (kTwoPlanes) {
+                                float u0, u1;
+                                lo[e] = pa_pack<T>(r0, r1, u0, u1);
+                            }
+                        }
+                        tmem_st16(ts + 16 * c, hi);
+                        if constexpr (kTwoPlanes) tmem_st16(ts + 64 + 16 * c, lo);
+                    };
+                    // P overwrites S from the left; the second plane starts at column 64, so
+                    // that half of S is taken into registers first
+                    float u[2][32];
+                    if constexpr (kTwoPlanes) {
+                        tmem_ld32(ts + 64, u[0]);
+                        tmem_ld32(ts + 96, u[1]);
+                        tmem_ld_wait();
+                        tmem_regs_ready(u[0]);
+                        tmem_regs_ready(u[1]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if (kTwoPlanes && c >= 2) {
+                            weights(u[c & 1], c);
+                        } else {
+                            tmem_ld32(ts + 32 * c, s);
+                            tmem_ld_wait();
+                            tmem_regs_ready(s);
+                            weights(s, c);
+                        }
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                mbar_arrive(p_ready);
+            }
+            if (n) {
+                wait(pv_done, (it - 1) & 1);
+                __syncwarp();
+                tc_fence_after();
+            }
+            if (busy) {
+                const size_t at = ((size_t)item.split * a.rows + tok) * a.n_q + head;
+                if (real && !a.direct) a.ml_part[at] = make_float2(m_ref, l);
+                const float f = a.direct ? 1.f / l : 1.f;
+                float o[32];
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    if (n) {
+                        tmem_ld32(to + 32 * c, o);
+                        tmem_ld_wait();
+                        tmem_regs_ready(o);
+                    }
+                    if (real && (a.direct || n)) {
+                        const bool none = !n || l == 0.f;  // no visible key: 0
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                  : make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+                            if (a.direct)
+                                pa_store4(static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)head * HD + 32 * c + e,
+                                          v);
+                            else
+                                pa_store4(a.o_part + at * HD + 32 * c + e, v);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();  // O has been read before the next job's products overwrite it
+        }
+    }
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"(kPaTmemCols)
+                     : "memory");
+    }
+}
+
+template <int W>
+struct alignas(4 * W) PaVec {
+    float v[W];
+};
+
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits that saw a
+// key, 0 if none did; one warp per (row, head).  Rows outside
+// [seq_start[0], seq_start[n_seqs]) belong to no sequence and stay as they are.
+template <class TO, int HD>
+__global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_constant__ PaArgs a) {
+    griddep_wait();  // the partial states
+    const int rh = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int row = rh / a.n_q;
+    if (row >= a.rows || row < a.seq_start[0] || row >= a.seq_start[a.n_seqs]) return;
+    const int splits = a.prefix_splits + a.seq_splits;
+    const size_t stride = (size_t)a.rows * a.n_q;
+    constexpr int W = HD / 32;  // dims of a lane
+    float M = -INFINITY;
+    for (int s = lane; s < splits; s += 32) M = fmaxf(M, a.ml_part[s * stride + rh].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float Lsum = 0.f, O[W];
+#pragma unroll
+    for (int d = 0; d < W; d++) O[d] = 0.f;
+    for (int s0 = 0; s0 < splits; s0 += 32) {
+        float w = 0.f;
+        if (s0 + lane < splits) {
+            const float2 ml = a.ml_part[(s0 + lane) * stride + rh];
+            w = ml.y != 0.f ? exp2f(ml.x - M) : 0.f;
+            Lsum += ml.y * w;
+        }
+        const int ns = min(32, splits - s0);
+#pragma unroll 8
+        for (int j = 0; j < ns; j++) {
+            const float b = __shfl_sync(0xffffffffu, w, j);
+            if (b == 0.f) continue;  // that state's O may be unwritten
+            const PaVec<W> p =
+                *reinterpret_cast<const PaVec<W> *>(a.o_part + ((s0 + j) * stride + rh) * HD + W * lane);
+#pragma unroll
+            for (int d = 0; d < W; d++) O[d] += p.v[d] * b;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) Lsum += __shfl_xor_sync(0xffffffffu, Lsum, o);
+    const float f = Lsum != 0.f ? 1.f / Lsum : 0.f;
+    TO *out = static_cast<TO *>(a.out) + (size_t)row * a.ldo + (size_t)(rh - row * a.n_q) * HD + W * lane;
+#pragma unroll
+    for (int d = 0; d < W; d++) {
+        if constexpr (std::is_same<TO, float>::value) out[d] = O[d] * f;
+        else if constexpr (std::is_same<TO, __half>::value) out[d] = __float2half_rn(O[d] * f);
+        else out[d] = __float2bfloat16_rn(O[d] * f);
+    }
+}
+
+// Rows of `inner` elements, ld apart, [rows] or [seqs][rows]; box of 64 elements
+// x kPaBoxRows rows in the 128-byte swizzle; rows past the end read as zero.
+int pa_map(CUtensorMap *tm, const void *p, int dtype, uint64_t inner, uint64_t rows, uint64_t ld, uint64_t seqs,
+           uint64_t seq_ld) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+    if (int s = lc_tensor_map_encoder(&enc)) return s;
+    cuuint64_t dims[3] = {inner, rows, seqs};
+    cuuint64_t strides[2] = {ld * 2, seq_ld * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)kPaBoxRows, 1}, es[3] = {1, 1, 1};
+    const CUresult r =
+        enc(tm, dtype == LC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, seqs ? 3 : 2,
+            const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    LC_REQUIRE(r == CUDA_SUCCESS, LC_ERR_CUDA, "lc_prefix_attn: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LC_OK;
+}
+
+int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// How the work is cut into items.
+void pa_plan(PaArgs &a, int num_sms) {
+    const int slots = 2 * num_sms;  // CTAs resident at once
+    const int64_t R = (int64_t)a.rows * a.group;
+    const int per_seq = div_up(div_up(R, a.n_seqs), kPaRows);  // row tiles of an average sequence
+    a.seq_lanes = std::max(1, per_seq);
+    // A sequence whose rows fill tiles by themselves gains nothing from sharing
+    // the prefix with others: its items run over [prefix | own] in one go.
+    const bool joint = a.prefix_len == 0 || a.n_seqs == 1 || R >= (int64_t)kPaRows * a.n_seqs;
+    a.prefix_items = 0, a.prefix_splits = 0, a.row_tiles = 1, a.prefix_keys = kPaKeys;
+    a.seq_from = joint ? 0 : a.prefix_len;
+    if (!joint) {
+        a.row_tiles = div_up(R, kPaRows);
+        const int base = a.n_kv * a.row_tiles, tiles = div_up(a.prefix_len, kPaKeys);
+        const int per = div_up(tiles, std::min(tiles, std::max(1, slots / base)));
+        a.prefix_keys = per * kPaKeys;
+        a.prefix_splits = div_up(tiles, per);
+        a.prefix_items = base * a.prefix_splits;
+    }
+    const int axis = a.prefix_len + a.own_cap - a.seq_from;
+    const int tiles = div_up(axis, kPaKeys);
+    a.seq_splits = 0, a.seq_keys = kPaKeys;
+    if (tiles) {
+        const int64_t base = (int64_t)a.n_kv * a.n_seqs * a.seq_lanes;
+        const int per = div_up(tiles, std::min<int64_t>(tiles, std::max<int64_t>(1, slots / base)));
+        a.seq_keys = per * kPaKeys;
+        a.seq_splits = div_up(tiles, per);
+    }
+    a.direct = joint && a.seq_splits == 1;
+}
+
+template <class T, class TO, int HD>
+int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[4]) {
+    auto kernel = prefix_attn_kernel<T, TO, HD>;
+    if (items) {
+        if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
+        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], a);
+    }
+    if (!a.direct) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(div_up((int64_t)a.rows * a.n_q, 4));
+        cfg.blockDim = dim3(128);
+        cfg.stream = ctx->stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = items ? 1 : 0;
+        LC_CUDA(cudaLaunchKernelEx(&cfg, prefix_attn_merge_kernel<TO, HD>, a));
+    }
+    return lc_after_launch(ctx, "lc_prefix_attn");
+}
+
+template <class T>
+int pa_types(lc_ctx *ctx, int out_dtype, uint32_t hd, const PaArgs &a, int items, const CUtensorMap (&tm)[4]) {
+    if (out_dtype == LC_F32)
+        return hd == 128 ? pa_launch<T, float, 128>(ctx, a, items, tm) : pa_launch<T, float, 64>(ctx, a, items, tm);
+    return hd == 128 ? pa_launch<T, T, 128>(ctx, a, items, tm) : pa_launch<T, T, 64>(ctx, a, items, tm);
+}
+
+}  // namespace
+
+extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void *q, uint64_t ldq,
+                              const lc_prefix_kv *kv, void *out, uint64_t ldo, uint32_t rows, uint32_t n_q_heads,
+                              uint32_t n_kv_heads, uint32_t head_dim, float scale, uint32_t causal) {
+    LC_REQUIRE(ctx, LC_ERR_INVALID, "lc_prefix_attn: null ctx");
+    LC_REQUIRE(dtype == LC_F16 || dtype == LC_BF16, LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: type %d (q, k and v are LC_F16 or LC_BF16)", dtype);
+    LC_REQUIRE(out_dtype == dtype || out_dtype == LC_F32, LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: output type %d (the input's or LC_F32)", out_dtype);
+    LC_REQUIRE(head_dim == 64 || head_dim == 128, LC_ERR_UNSUPPORTED, "lc_prefix_attn: head_dim %u (64 or 128)",
+               head_dim);
+    LC_REQUIRE(n_kv_heads > 0 && n_q_heads % n_kv_heads == 0, LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: n_q_heads %u must be a multiple of n_kv_heads %u", n_q_heads, n_kv_heads);
+    LC_REQUIRE(scale >= 0.f && scale < INFINITY, LC_ERR_INVALID,
+               "lc_prefix_attn: scale %g must be finite and not negative", scale);
+    if (rows == 0 || n_q_heads == 0) return LC_OK;
+    LC_REQUIRE(kv, LC_ERR_INVALID, "lc_prefix_attn: null kv");
+    if (kv->n_seqs == 0) return LC_OK;
+    LC_REQUIRE(q && out && kv->seq_start && (!kv->prefix_len || (kv->k_prefix && kv->v_prefix)) &&
+                   (!kv->own_cap || (kv->k_own && kv->v_own && kv->own_len)),
+               LC_ERR_INVALID, "lc_prefix_attn: null pointer");
+    LC_REQUIRE(kv->n_seqs <= (1u << 20), LC_ERR_UNSUPPORTED, "lc_prefix_attn: %u sequences", kv->n_seqs);
+    const uint64_t wq = (uint64_t)n_q_heads * head_dim, wk = (uint64_t)n_kv_heads * head_dim;
+    LC_REQUIRE((uint64_t)rows * n_q_heads <= 0x7FFFF000u && wq < (1u << 24), LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: %u rows of %u heads", rows, n_q_heads);
+    LC_REQUIRE((uint64_t)kv->prefix_len + kv->own_cap <= kPaMaxLen, LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: %u + %u keys", kv->prefix_len, kv->own_cap);
+    if (!ldq) ldq = wq;
+    if (!ldo) ldo = wq;
+    const uint64_t ldp = kv->ld_prefix ? kv->ld_prefix : wk, ldw = kv->ld_own ? kv->ld_own : wk;
+    const uint64_t seq_ld = kv->own_stride ? kv->own_stride : ldw * kv->own_cap;
+    LC_REQUIRE(ldq >= wq && ldo >= wq && ldp >= wk && ldw >= wk, LC_ERR_INVALID,
+               "lc_prefix_attn: a row stride is shorter than its row");
+    LC_REQUIRE(!kv->own_cap || kv->n_seqs == 1 || seq_ld >= (kv->own_cap - 1) * ldw + wk, LC_ERR_INVALID,
+               "lc_prefix_attn: own_stride is shorter than own_cap rows");
+    // strides of a tensor map are below 2^40 bytes
+    LC_REQUIRE(ldq < (1ull << 38) && ldo < (1ull << 38) && ldp < (1ull << 38) && ldw < (1ull << 38) &&
+                   seq_ld < (1ull << 39),
+               LC_ERR_INVALID, "lc_prefix_attn: stride too large");
+    const uint64_t out_vec = out_dtype == LC_F32 ? 4 : 8;
+    LC_REQUIRE((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ldq % 8 == 0 && ldo % out_vec == 0 &&
+                   (!kv->prefix_len || ((((uintptr_t)kv->k_prefix | (uintptr_t)kv->v_prefix) & 15) == 0 && ldp % 8 == 0)) &&
+                   (!kv->own_cap || ((((uintptr_t)kv->k_own | (uintptr_t)kv->v_own) & 15) == 0 && ldw % 8 == 0 &&
+                                     seq_ld % 8 == 0)) &&
+                   (((uintptr_t)kv->seq_start | (uintptr_t)kv->own_len) & 3) == 0,
+               LC_ERR_INVALID, "lc_prefix_attn: rows must start on 16-byte boundaries");
+    const uint64_t bo = out_dtype == LC_F32 ? 4 : 2;
+    LC_REQUIRE(!lc_rows_meet(q, ldq * 2, wq * 2, out, ldo * bo, wq * bo, rows), LC_ERR_INVALID,
+               "lc_prefix_attn: out overlaps q");
+    if (int s = lc_use_device(ctx)) return s;
+
+    PaArgs a = {};
+    a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
+    a.rows = (int)rows, a.n_q = (int)n_q_heads, a.n_kv = (int)n_kv_heads, a.group = a.n_q / a.n_kv;
+    a.prefix_len = (int)kv->prefix_len, a.own_cap = (int)kv->own_cap, a.n_seqs = (int)kv->n_seqs;
+    a.own_len = kv->own_cap ? kv->own_len : nullptr, a.seq_start = kv->seq_start;
+    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.causal = causal != 0;
+    a.status = ctx->dev_status;
+    pa_plan(a, ctx->num_sms);
+    const int64_t items = (int64_t)a.prefix_items + (int64_t)a.n_kv * a.n_seqs * a.seq_lanes * a.seq_splits;
+    LC_REQUIRE(items <= 0x7FFFFFFF, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
+    if (!a.direct) {
+        const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * rows * n_q_heads;
+        void *scr = nullptr;
+        if (int s = lc_scratch_kept(ctx, LC_SCRATCH_PREFIX, states * (head_dim * 4 + 8) + 256, &scr)) return s;
+        a.ml_part = (float2 *)scr;
+        a.o_part = (float *)((char *)scr + ((states * 8 + 255) & ~(size_t)255));
+    }
+    CUtensorMap tm[4] = {};
+    if (a.prefix_len) {
+        if (int s = pa_map(&tm[0], kv->k_prefix, dtype, wk, kv->prefix_len, ldp, 0, 0)) return s;
+        if (int s = pa_map(&tm[1], kv->v_prefix, dtype, wk, kv->prefix_len, ldp, 0, 0)) return s;
+    }
+    if (a.own_cap) {
+        if (int s = pa_map(&tm[2], kv->k_own, dtype, wk, kv->own_cap, ldw, kv->n_seqs, seq_ld)) return s;
+        if (int s = pa_map(&tm[3], kv->v_own, dtype, wk, kv->own_cap, ldw, kv->n_seqs, seq_ld)) return s;
+    }
+    return dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, tm)
+                           : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, tm);
+}

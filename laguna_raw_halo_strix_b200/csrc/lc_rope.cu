@@ -179,25 +179,6 @@ __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
 
 int type_bytes(int dtype) { return dtype == LC_F32 ? 4 : dtype == LC_F16 || dtype == LC_BF16 ? 2 : 0; }
 
-// Do the m rows of wa bytes, pa apart, at a share a byte with the m rows of wb
-// bytes, pb apart, at b?  Exact for equal pitches (columns of one buffer);
-// otherwise whole extents are compared.
-bool rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
-    const intptr_t d = (intptr_t)b - (intptr_t)a;
-    if (pa != pb || m == 1) {
-        const uint64_t ea = (m - 1) * pa + wa, eb = (m - 1) * pb + wb;
-        return d < (intptr_t)ea && -d < (intptr_t)eb;
-    }
-    // row i of a and row i + j of b start d + j * pa apart: overlap if that is in (-wb, wa)
-    const intptr_t p = (intptr_t)pa;
-    const intptr_t j0 = d >= 0 ? -(d / p) : (-d + p - 1) / p;  // d + j0 * p in [0, p)
-    for (intptr_t j = j0 - 1; j <= j0; j++) {
-        const intptr_t at = d + j * p;
-        if (j < (intptr_t)m && -j < (intptr_t)m && at < (intptr_t)wa && -at < (intptr_t)wb) return true;
-    }
-    return false;
-}
-
 template <class TI, class TO>
 int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     constexpr int V = RpVec<TI>::kN;
@@ -285,12 +266,12 @@ extern "C" int lc_rope(lc_ctx *ctx, int dtype, int out_dtype, int layout, const 
                LC_ERR_INVALID, "lc_rope: a pointer is not aligned to its type");
     const bool q_same = wq && q == q_out && ldq == ldq_out && bi == bo && dtype == out_dtype;
     const bool k_same = wk && k == k_out && ldk == ldk_out && bi == bo && dtype == out_dtype;
-    const bool meet = (wq && !q_same && rows_meet(q, ldq * bi, wq * bi, q_out, ldq_out * bo, wq * bo, m)) ||
-                      (wk && !k_same && rows_meet(k, ldk * bi, wk * bi, k_out, ldk_out * bo, wk * bo, m)) ||
+    const bool meet = (wq && !q_same && lc_rows_meet(q, ldq * bi, wq * bi, q_out, ldq_out * bo, wq * bo, m)) ||
+                      (wk && !k_same && lc_rows_meet(k, ldk * bi, wk * bi, k_out, ldk_out * bo, wk * bo, m)) ||
                       (wq && wk &&
-                       (rows_meet(q_out, ldq_out * bo, wq * bo, k_out, ldk_out * bo, wk * bo, m) ||
-                        rows_meet(q, ldq * bi, wq * bi, k_out, ldk_out * bo, wk * bo, m) ||
-                        rows_meet(k, ldk * bi, wk * bi, q_out, ldq_out * bo, wq * bo, m)));
+                       (lc_rows_meet(q_out, ldq_out * bo, wq * bo, k_out, ldk_out * bo, wk * bo, m) ||
+                        lc_rows_meet(q, ldq * bi, wq * bi, k_out, ldk_out * bo, wk * bo, m) ||
+                        lc_rows_meet(k, ldk * bi, wk * bi, q_out, ldq_out * bo, wq * bo, m)));
     LC_REQUIRE(!meet, LC_ERR_INVALID, "lc_rope: an output overlaps another tensor (only y = x in place is possible)");
     RpArgs a = {};
     a.x[0] = q, a.x[1] = k, a.y[0] = q_out, a.y[1] = k_out;

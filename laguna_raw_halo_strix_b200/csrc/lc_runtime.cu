@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 
@@ -111,6 +112,7 @@ extern "C" int lc_destroy(lc_ctx *ctx) {
     if (ctx->stream && ctx->stream != ctx->own_stream) cudaStreamSynchronize(ctx->stream);
     for (int i = 0; i < LC_SCRATCH_COUNT; i++)
         if (ctx->scratch[i]) cudaFree(ctx->scratch[i]);
+    for (void *p : ctx->kept) cudaFree(p);
     if (ctx->dev_status) cudaFree(ctx->dev_status);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     delete ctx;
@@ -166,6 +168,22 @@ int lc_set_smem_attr(const void *kernel, size_t bytes) {
     return LC_OK;
 }
 
+bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
+    const intptr_t d = (intptr_t)b - (intptr_t)a;
+    if (pa != pb || m == 1) {
+        const uint64_t ea = (m - 1) * pa + wa, eb = (m - 1) * pb + wb;
+        return d < (intptr_t)ea && -d < (intptr_t)eb;
+    }
+    // row i of a and row i + j of b start d + j * pa apart: overlap if that is in (-wb, wa)
+    const intptr_t p = (intptr_t)pa;
+    const intptr_t j0 = d >= 0 ? -(d / p) : (-d + p - 1) / p;  // d + j0 * p in [0, p)
+    for (intptr_t j = j0 - 1; j <= j0; j++) {
+        const intptr_t at = d + j * p;
+        if (j < (intptr_t)m && -j < (intptr_t)m && at < (intptr_t)wa && -at < (intptr_t)wb) return true;
+    }
+    return false;
+}
+
 int lc_after_launch(lc_ctx *ctx, const char *what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return lc_fail(LC_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
@@ -213,6 +231,29 @@ void *lc_scratch_zeroed(lc_ctx *ctx, int slot, size_t bytes) {
         }
     }
     return p;
+}
+
+int lc_scratch_kept(lc_ctx *ctx, int slot, size_t bytes, void **out) {
+    if (bytes > ctx->scratch_bytes[slot]) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        LC_CUDA(cudaStreamIsCapturing(ctx->stream, &st));
+        LC_REQUIRE(st == cudaStreamCaptureStatusNone, LC_ERR_UNSUPPORTED,
+                   "scratch: %zu bytes needed during a stream capture, %zu held; make a call of this size before it",
+                   bytes, ctx->scratch_bytes[slot]);
+        size_t want = (std::max(bytes, 2 * ctx->scratch_bytes[slot]) + 255) & ~(size_t)255;
+        if (want < ((size_t)1 << 20)) want = (size_t)1 << 20;
+        void *p = nullptr;
+        cudaError_t e = cudaMalloc(&p, want);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return lc_fail(LC_ERR_OOM, "scratch: cudaMalloc(%zu): %s", want, cudaGetErrorString(e));
+        }
+        if (ctx->scratch[slot]) ctx->kept.push_back(ctx->scratch[slot]);
+        ctx->scratch[slot] = p;
+        ctx->scratch_bytes[slot] = want;
+    }
+    *out = ctx->scratch[slot];
+    return LC_OK;
 }
 
 // ---- buffers ---------------------------------------------------------------

@@ -116,6 +116,7 @@ SIGNATURES = {
     "lc_softplus": (_i, [_vp, _vp, _vp, _u32]),
     "lc_enc_aux_norm": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _f]),
     "lc_mha_attn": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _f, _u32, _u32]),
+    "lc_prefix_attn": (_i, [_vp, _i, _i, _vp, _u64, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _f, _u32]),
     "lc_rope": (_i, [_vp, _i, _i, _i, _vp, _u64, _vp, _u64, _u32, _vp, _u64, _vp, _u64, _u32, _vp, _vp, _u32, _u32,
                      _u32, _f]),
     "lc_rope_freq": (_i, [C.POINTER(_f), _u32, _f]),
@@ -124,6 +125,7 @@ SIGNATURES = {
     "lc_key_value": (_f, [C.c_uint64]),
     "lc_key_index": (_u32, [C.c_uint64]),
     "lc_argmax_rows": (_i, [_vp, _vp, _u32, _u32, _u32, _vp]),
+    "lc_logits_process": (_i, [_vp, _vp, _u64, _vp, _u64, _u32, _u32, _u32, _vp, _vp]),
     "lc_lm_head_argmax": (_i, [_vp, _i, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp]),
     # GGUF reader
     "lc_type_block_bytes": (C.c_uint64, [_i]),
@@ -192,6 +194,45 @@ class TargetHParams(C.Structure):
 
     def as_dict(self) -> dict:
         return {k: getattr(self, k) for k, _ in self._fields_}
+
+
+class PrefixKV(C.Structure):
+    """lc_prefix_kv (include/laguna_cuda.h): the shared prefix and the sequences' own K/V rows.  Holds the tensors."""
+
+    _fields_ = [("k_prefix", _vp), ("v_prefix", _vp), ("ld_prefix", _u64), ("prefix_len", _u32), ("own_cap", _u32),
+                ("k_own", _vp), ("v_own", _vp), ("ld_own", _u64), ("own_stride", _u64), ("own_len", _vp),
+                ("seq_start", _vp), ("n_seqs", _u32)]
+
+    def __init__(self, k_prefix, v_prefix, prefix_len, k_own, v_own, own_cap, own_len, seq_start, n_seqs, ld_prefix=0,
+                 ld_own=0, own_stride=0):
+        super().__init__(ptr(k_prefix), ptr(v_prefix), ld_prefix, prefix_len, own_cap, ptr(k_own), ptr(v_own), ld_own,
+                         own_stride, ptr(own_len), ptr(seq_start), n_seqs)
+        self.held = (k_prefix, v_prefix, k_own, v_own, own_len, seq_start)
+
+
+class LogitsRules(C.Structure):
+    """lc_logits_rules (include/laguna_cuda.h), from tensors: the lengths of the
+    lists and the shape of the masks [n_masks, words] are read off them (a list
+    given as an int address needs its length beside it).  Holds the tensors."""
+
+    _fields_ = [("hist", _vp), ("hist_start", _vp), ("gen_start", _vp), ("hist_len", _u64),
+                ("repetition", _vp), ("frequency", _vp), ("presence", _vp),
+                ("bias_tok", _vp), ("bias", _vp), ("bias_start", _vp), ("bias_len", _u64),
+                ("mask", _vp), ("mask_row", _vp), ("mask_ld", _u64), ("n_masks", _u32)]
+
+    def __init__(self, hist=None, hist_start=None, gen_start=None, repetition=None, frequency=None, presence=None,
+                 bias_tok=None, bias=None, bias_start=None, mask=None, mask_row=None, hist_len=None, bias_len=None,
+                 mask_ld=None, n_masks=None):
+        def size(t, given):
+            return given if given is not None else 0 if t is None else t.numel()
+
+        if mask is not None and (mask_ld is None or n_masks is None):
+            n_masks, mask_ld = mask.shape[0], mask.stride(0)
+        super().__init__(ptr(hist), ptr(hist_start), ptr(gen_start), size(hist, hist_len), ptr(repetition),
+                         ptr(frequency), ptr(presence), ptr(bias_tok), ptr(bias), ptr(bias_start),
+                         size(bias_tok, bias_len), ptr(mask), ptr(mask_row), mask_ld or 0, n_masks or 0)
+        self.held = (hist, hist_start, gen_start, repetition, frequency, presence, bias_tok, bias, bias_start, mask,
+                     mask_row)
 
 
 TARGET_CACHED = 1  # lc_target_forward flag
@@ -385,8 +426,19 @@ class Context:
         check(self.L.lc_mha_attn(self.h, ptr(q), ptr(k), ptr(v), ptr(out), m, n_q_heads, n_kv_heads, head_dim,
                                  seq_len, scale, q_pos0, causal), "lc_mha_attn")
 
+    def prefix_attn(self, dtype, out_dtype, q, kv, out, rows, n_q_heads, n_kv_heads, head_dim, scale, causal=1, ldq=0,
+                    ldo=0):
+        """lc_prefix_attn with a PrefixKV; strides in elements, 0 = packed."""
+        check(self.L.lc_prefix_attn(self.h, dtype, out_dtype, ptr(q), ldq, C.byref(kv), ptr(out), ldo, rows, n_q_heads,
+                                    n_kv_heads, head_dim, scale, causal), "lc_prefix_attn")
+
     def argmax_rows(self, logits, m, n, row_offset, keys):
         check(self.L.lc_argmax_rows(self.h, ptr(logits), m, n, row_offset, ptr(keys)), "lc_argmax_rows")
+
+    def logits_process(self, logits, rules, out, keys, m, n, row_offset=0, ld=0, ld_out=0):
+        """lc_logits_process with a LogitsRules; out (or keys) may be None; strides in floats, 0 = n."""
+        check(self.L.lc_logits_process(self.h, ptr(logits), ld, ptr(out), ld_out, m, n, row_offset, C.byref(rules),
+                                       ptr(keys)), "lc_logits_process")
 
     def check_bounded_wait(self, spins: int = 1024) -> None:
         check(self.L.lc_check_bounded_wait(self.h, spins), "lc_check_bounded_wait")

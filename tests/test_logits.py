@@ -1,0 +1,66 @@
+"""lc_logits_process without a GPU: its refusals (decided from the arguments
+alone, before it looks into the context, so a blank one will do), and the
+restatement that the GPU tests compare with, on rows worked out by hand."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import logits_ref
+from laguna_raw_halo_strix_b200 import lc
+
+BLANK = C.create_string_buffer(4096)  # stands for an lc_ctx
+
+
+def call(rules=None, **over):
+    a = dict(logits=0x100000, ld=0, out=0x200000, ld_out=0, m=4, n=100, row_offset=0)
+    keys = over.pop("keys", 0x300000)
+    a.update(over)
+    r = lc.LogitsRules()
+    for k, v in (rules or {}).items():
+        setattr(r, k, v)
+    return lc.lib().lc_logits_process(C.cast(BLANK, C.c_void_p), *a.values(),
+                                      None if rules is False else C.byref(r), keys)
+
+
+@pytest.mark.parametrize("over", [
+    dict(logits=None), dict(rules=False), dict(out=None, keys=None), dict(n=0), dict(n=(1 << 30) + 1),
+    dict(row_offset=0x7FFFFFFF - 99), dict(row_offset=0xFFFFFFFF), dict(ld=99), dict(ld_out=99), dict(ld=2 ** 60),
+    dict(ld_out=2 ** 57), dict(logits=0x100002), dict(out=0x200001), dict(keys=0x300004), dict(out=0x100004),
+    dict(out=0x100000, ld_out=200), dict(out=0x100000 + 4 * 350),
+    dict(out=0x100000 + 4 * 60, ld=150, ld_out=150),
+    dict(rules=dict(hist_len=5)), dict(rules=dict(hist=0x400000, hist_len=5)),
+    dict(rules=dict(bias_len=5, bias_tok=0x400000, bias_start=0x500000)),
+    dict(rules=dict(bias_len=5, bias=0x400000, bias_start=0x500000)),
+    dict(rules=dict(bias_len=5, bias=0x400000, bias_tok=0x500000)),
+    dict(rules=dict(hist=0x400001, hist_start=0x500000, hist_len=1)),
+    dict(rules=dict(mask=0x400000, mask_ld=3, n_masks=4)), dict(rules=dict(mask=0x400000, mask_ld=4, n_masks=3)),
+    dict(rules=dict(mask=0x400000, mask_ld=4, n_masks=4), row_offset=29),
+    dict(rules=dict(mask=0x400000, mask_ld=1 << 41, n_masks=4)), dict(rules=dict(repetition=0x400002))], ids=str)
+def test_invalid(over):
+    assert call(**over) == lc.LC_ERR_INVALID
+    assert "lc_logits_process" in lc.last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(m=(1 << 24) + 1), dict(rules=dict(hist=0x400000, hist_start=0x500000, hist_len=1 << 31)),
+    dict(rules=dict(bias=0x400000, bias_tok=0x400000, bias_start=0x500000, bias_len=1 << 31))], ids=str)
+def test_unsupported(over):
+    assert call(**over) == lc.LC_ERR_UNSUPPORTED
+    assert "lc_logits_process" in lc.last_error()
+
+
+def test_no_rows_and_null_context():
+    assert call(m=0, logits=None, out=None, keys=None) == lc.LC_OK
+    assert lc.lib().lc_logits_process(None, None, 0, None, 0, 1, 1, 0, None, None) == lc.LC_ERR_INVALID
+
+
+def test_restatement_by_hand():
+    x = np.array([[2.0, -2.0, 1.0, 3.0, 0.5]], np.float32)
+    out, _, best = logits_ref.process(
+        x, hist=[0, 1, 0, 3, 3, 9], hist_start=[0, 6], gen_start=[2], repetition=[2.0], frequency=[0.25],
+        presence=[0.5], bias_tok=[2, 4, 2], bias=[9.0, 1.0, 0.5], bias_start=[0, 3],
+        mask=np.array([[0b10111]], np.uint32), mask_row=[0])
+    # 0: seen twice, generated once; 1: prompt only; 2: the later bias; 3: masked; 4: bias
+    assert out[0].tolist() == [2 / 2 - 0.25 - 0.5, -4.0, 1.5, -np.inf, 1.5]
+    assert best[0] == 4  # the larger of two equal ones
