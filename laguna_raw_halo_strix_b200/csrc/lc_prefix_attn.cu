@@ -8,16 +8,18 @@
 // head of a KV head are rows of one matrix product against it), the own parts
 // per sequence, and a small kernel merges.
 //
-// One CTA takes an item: up to 128 query rows of one KV head against a range of
-// the virtual key axis [prefix | own rows of its sequence].  Per tile of 128 keys
+// A work item is up to 128 query rows of one KV head (whole tokens) against a
+// range of the virtual key axis [prefix | own rows of its sequence].  Per tile
+// of 128 keys
 //   S = Q K^T   tcgen05, Q and K K-major in shared memory, S in TMEM 0..127
 //   P           softmax warps, one thread a row, written over S as 16-bit pairs
 //               (and a second plane of what the rounding lost, for f32 outputs)
 //   O += P V    tcgen05, P from TMEM, V read MN-major as it lies in memory
-// K and V tiles come by TMA.  Roles: warps 0-3 softmax, 4 loads, 5 MMA.  S and P
+// Q, K and V come by TMA.  Roles: warps 0-3 softmax, 4 loads, 5 MMA.  S and P
 // share their TMEM columns, so within a CTA a tile's products and its softmax
 // alternate; two CTAs share an SM (256 TMEM columns and 98 KB each) and fill
-// each other's gaps.
+// each other's gaps.  CTAs stay for several items: the next item's Q and K are
+// loaded while the last one's weights, values and results are worked on.
 #include <math.h>
 
 #include <algorithm>
@@ -49,25 +51,33 @@ struct PaArgs {
     void *out;
     uint64_t ldq, ldo;
     int rows, n_q, n_kv, group;
+    uint32_t group_inv;  // ceil(2^16 / group): r * group_inv >> 16 is r / group for r < 128
+    int tile_toks, box_toks;  // tokens of a row tile and of one TMA copy of Q
     int prefix_len, own_cap, n_seqs;
     const int32_t *own_len, *seq_start;
     float scale_log2;  // scale * log2(e)
     int causal;
-    // plan: items 0 .. prefix_items - 1 take the prefix for rows of all
+    // plan: CTA c runs items c, c + gridDim.x, ..; items 0 .. prefix_items - 1 take the prefix for rows of all
     // sequences, the rest rows of one sequence over [seq_from, end) of the
     // virtual axis
-    int prefix_items, row_tiles, prefix_keys;
+    int items, prefix_items, row_tiles, prefix_keys;
     int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
     int direct;         // one split covers everything: items write out
-    float *o_part;      // [split][row][head][HD], unnormalised
-    float2 *ml_part;    // [split][row][head]: (m in log2 units, l)
+    // partial states of row r = token * group + head within the group: O
+    // unnormalised as [split][KV head][r / 32][HD / 4][r % 32][4] (32 rows' 16-byte
+    // pieces side by side: the lanes of a warp hold neighbouring rows), and (m in
+    // log2 units, l) as [split][KV head][r]
+    float *o_part;
+    float2 *ml_part;
+    int row_blocks;     // 32-row blocks of a KV head
     unsigned *status;
 };
 
-// Rows r0 .. r0 + nrows - 1 (row = token * group + head within the group) of
-// one KV head against prefix keys [p0, p1) and keys [o0, o1) of sequence seq.
+// Tokens first .. first + count - 1 (rows r = token within the tile * group +
+// head within the group) of one KV head against prefix keys [p0, p1) and keys
+// [o0, o1) of sequence seq.
 struct PaJob {
-    int r0, nrows, p0, p1, o0, o1, seq;
+    int first, count, p0, p1, o0, o1, seq;
     int pos0;  // own position of token t is pos0 + t
     __device__ __forceinline__ int prefix_tiles() const { return (p1 - p0 + kPaKeys - 1) / kPaKeys; }
     __device__ __forceinline__ int tiles() const { return prefix_tiles() + (o1 - o0 + kPaKeys - 1) / kPaKeys; }
@@ -81,19 +91,18 @@ struct PaJob {
 };
 
 struct PaItem {
-    int hk, split, rt, rt_step, rt_end;  // row tiles rt, rt + rt_step, .. < rt_end
+    int hk, split, t, t_step;  // token tiles at t, t + t_step, .. below count
     int start, count, len, seq, v0, v1;
 };
 
-__device__ __forceinline__ PaItem pa_item(const PaArgs &a) {
+__device__ __forceinline__ PaItem pa_item(const PaArgs &a, int i) {
     PaItem t;
-    int i = blockIdx.x;
     if (i < a.prefix_items) {
         t.hk = i % a.n_kv;
         i /= a.n_kv;
-        t.rt = i % a.row_tiles;
+        t.t = i % a.row_tiles * a.tile_toks;
         t.split = i / a.row_tiles;
-        t.rt_step = 1 << 24;
+        t.t_step = 1 << 30;
         t.start = 0, t.count = a.rows, t.len = 0, t.seq = 0;
         t.v0 = t.split * a.prefix_keys;
         t.v1 = min(a.prefix_len, t.v0 + a.prefix_keys);
@@ -103,10 +112,10 @@ __device__ __forceinline__ PaItem pa_item(const PaArgs &a) {
         i /= a.n_kv;
         t.seq = i % a.n_seqs;
         i /= a.n_seqs;
-        t.rt = i % a.seq_lanes;
+        t.t = i % a.seq_lanes * a.tile_toks;
         const int sp = i / a.seq_lanes;
         t.split = a.prefix_splits + sp;
-        t.rt_step = a.seq_lanes;
+        t.t_step = a.seq_lanes * a.tile_toks;
         // values from the device are held inside the arrays
         t.start = min(max(a.seq_start[t.seq], 0), a.rows);
         t.count = min(max(a.seq_start[t.seq + 1], t.start), a.rows) - t.start;
@@ -114,21 +123,19 @@ __device__ __forceinline__ PaItem pa_item(const PaArgs &a) {
         t.v0 = a.seq_from + sp * a.seq_keys;
         t.v1 = min(a.prefix_len + a.own_cap, t.v0 + a.seq_keys);
     }
-    t.rt_end = (t.count * a.group + kPaRows - 1) / kPaRows;
     return t;
 }
 
-__device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int rt) {
+__device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int at) {
     PaJob j;
-    const int first = rt * kPaRows;  // within the item's rows
-    j.r0 = t.start * a.group + first;
-    j.nrows = min(kPaRows, t.count * a.group - first);
+    j.first = t.start + at;
+    j.count = min(a.tile_toks, t.count - at);
     j.seq = t.seq;
     j.pos0 = t.len - t.count - t.start;
     j.p0 = min(t.v0, a.prefix_len), j.p1 = min(t.v1, a.prefix_len);
     j.o0 = max(t.v0, a.prefix_len) - a.prefix_len;
     j.o1 = min(max(t.v1, a.prefix_len) - a.prefix_len, t.len);
-    if (a.causal) j.o1 = min(j.o1, j.pos0 + (j.r0 + j.nrows - 1) / a.group + 1);  // the last row's reach
+    if (a.causal) j.o1 = min(j.o1, j.pos0 + j.first + j.count);  // the last token's reach
     j.o1 = max(j.o1, j.o0);
     return j;
 }
@@ -139,7 +146,16 @@ struct PaWait {
     unsigned *status;
     bool ok = true;
     __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity)) {
+        if (!ok) return;
+        uint32_t left;
+        asm volatile(
+            "{\n .reg .pred p;\n mov.u32 %0, %3;\n"
+            "AGAIN: mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+            " sub.u32 %0, %0, 1;\n setp.ne.u32 p, %0, 0;\n @p bra AGAIN;\nDONE:\n}\n"
+            : "=&r"(left)
+            : "r"(smem_addr(bar)), "r"(parity), "n"(kWaitSpins)
+            : "memory");
+        if (left == 0) {
             ok = false;
             atomicOr(status, LC_DEV_WAIT_TIMEOUT);
         }
@@ -195,16 +211,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-#define LC_U(i) "r"(__float_as_uint(v[i]))
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
-        LC_U(0), LC_U(1), LC_U(2), LC_U(3), LC_U(4), LC_U(5), LC_U(6), LC_U(7), LC_U(8), LC_U(9), LC_U(10), LC_U(11),
-        LC_U(12), LC_U(13), LC_U(14), LC_U(15), LC_U(16), LC_U(17), LC_U(18), LC_U(19), LC_U(20), LC_U(21), LC_U(22),
-        LC_U(23), LC_U(24), LC_U(25), LC_U(26), LC_U(27), LC_U(28), LC_U(29), LC_U(30), LC_U(31)
-        : "memory");
-#undef LC_U
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n"
+        " add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 
 // 2^x to about 2 ulp, 0 below the normal range.
@@ -246,15 +275,15 @@ template <class T, class TO, int HD>
 __global__ void __launch_bounds__(kPaThreads, 2)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap kp, const __grid_constant__ CUtensorMap vp,
                        const __grid_constant__ CUtensorMap ko, const __grid_constant__ CUtensorMap vo,
+                       const __grid_constant__ CUtensorMap qm,
                        const __grid_constant__ PaArgs a) {
     using L = PaSmem<HD>;
     constexpr bool kTwoPlanes = std::is_same<TO, float>::value;  // P as hi + lo
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *k_full = bar, *v_full = bar + 1, *s_full = bar + 2, *p_ready = bar + 3, *pv_done = bar + 4,
-             *q_ready = bar + 5;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 6);
+    uint64_t *k_full = bar, *v_full = bar + 1, *s_full = bar + 2, *p_ready = bar + 3, *pv_done = bar + 4;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 5);
     const uint32_t sbase = smem_addr(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -265,7 +294,6 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         mbar_init(s_full, 1);
         mbar_init(p_ready, kPaRows);
         mbar_init(pv_done, 1);
-        mbar_init(q_ready, kPaRows);
         mbar_init_fence();
     }
     if (warp == 5) {
@@ -278,42 +306,56 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = *tslot;
-    const PaItem item = pa_item(a);
     PaWait wait{a.status};
-    uint32_t it = 0;  // tiles so far: every barrier completes once per tile (q_ready once per job)
+    uint32_t it = 0;  // tiles so far: every barrier completes once per tile
 
     if (warp == 4) {  // ---- loads
         if (lane == 0) {
-            for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
-                const PaJob j = pa_job(a, item, rt);
-                const int n = j.tiles();
-                for (int i = 0; i < n; i++, it++) {
-                    int key, nk;
-                    bool own;
-                    j.tile(i, key, nk, own);
-                    const int boxes = (nk + kPaBoxRows - 1) / kPaBoxRows;
-                    const uint32_t bytes = boxes * kPaBoxRows * HD * 2;
-                    const int x = item.hk * HD;
-#pragma unroll
-                    for (int kv = 0; kv < 2; kv++) {
-                        // the slot is free once the products that read it are done
-                        if (it) wait(kv ? pv_done : s_full, (it - 1) & 1);
-                        if (!wait.ok) break;
-                        uint64_t *b = kv ? v_full : k_full;
-                        unsigned char *dst = smem + (kv ? L::kV : L::kK);
-                        mbar_expect_tx(b, bytes);
-                        for (int c = 0; c < HD / 64; c++)
-                            for (int r = 0; r < boxes; r++) {
-                                unsigned char *d = dst + c * kPaPlane + r * (kPaBoxRows * 128);
-                                if (own)
-                                    tma_load_3d_plain(d, kv ? &vo : &ko, x + 64 * c, key + kPaBoxRows * r, j.seq, b);
-                                else
-                                    tma_load_2d_plain(d, kv ? &vp : &kp, x + 64 * c, key + kPaBoxRows * r, b);
+#pragma unroll 1
+            for (int w = blockIdx.x; w < a.items && wait.ok; w += gridDim.x) {
+                const PaItem item = pa_item(a, w);
+#pragma unroll 1
+                for (int at = item.t; at < item.count && wait.ok; at += item.t_step) {
+                    const PaJob j = pa_job(a, item, at);
+                    const int n = j.tiles();
+#pragma unroll 1
+                    for (int i = 0; i < n && wait.ok; i++, it++) {
+                        int key, nk;
+                        bool own;
+                        j.tile(i, key, nk, own);
+                        const int boxes = (nk + kPaBoxRows - 1) / kPaBoxRows;
+                        const uint32_t bytes = boxes * kPaBoxRows * HD * 2;
+                        const int x = item.hk * HD;
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; kv++) {
+                            // the slot is free once the products that read it are done (Q: those
+                            // of the last job's last scores)
+                            if (it) wait(kv ? pv_done : s_full, (it - 1) & 1);
+                            if (!wait.ok) break;
+                            uint64_t *b = kv ? v_full : k_full;
+                            const int qb = i == 0 && kv == 0 ? (j.count + a.box_toks - 1) / a.box_toks : 0;
+                            const int q_rows = a.box_toks * a.group;
+                            mbar_expect_tx(b, bytes + (uint32_t)(qb * q_rows * HD * 2));
+#pragma unroll 1
+                            for (int c = 0; c < HD / 64; c++) {
+#pragma unroll 1
+                                for (int r = 0; r < qb; r++)
+                                    tma_load_3d_plain(smem + L::kQ + c * kPaPlane + r * q_rows * 128, &qm, 64 * c,
+                                                      item.hk * a.group, j.first + r * a.box_toks, b);
+                                unsigned char *dst = smem + (kv ? L::kV : L::kK) + c * kPaPlane;
+#pragma unroll 1
+                                for (int r = 0; r < boxes; r++) {
+                                    const int y = key + kPaBoxRows * r;
+                                    unsigned char *d = dst + r * (kPaBoxRows * 128);
+                                    if (own)
+                                        tma_load_3d_plain(d, kv ? &vo : &ko, x + 64 * c, y, j.seq, b);
+                                    else
+                                        tma_load_2d_plain(d, kv ? &vp : &kp, x + 64 * c, y, b);
+                                }
                             }
+                        }
                     }
-                    if (!wait.ok) break;
                 }
-                if (!wait.ok) break;
             }
             if (!wait.ok) {  // copies of this CTA still in flight
                 mbar_wait(k_full, it & 1);
@@ -321,89 +363,86 @@ __global__ void __launch_bounds__(kPaThreads, 2)
             }
         }
     } else if (warp == 5) {  // ---- products
-        uint32_t jobs = 0;
-        for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
-            const PaJob j = pa_job(a, item, rt);
-            const int n = j.tiles();
-            if (n == 0) continue;
-            wait(q_ready, jobs++ & 1);
-            for (int i = 0; i < n && wait.ok; i++, it++) {
-                int key, nk;
-                bool own;
-                j.tile(i, key, nk, own);
-                wait(k_full, it & 1);
-                if (!wait.ok) break;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
-#pragma unroll
-                    for (int s = 0; s < HD / 16; s++) {
-                        const uint64_t o = ((s >> 2) * kPaPlane + (s & 3) * 32) >> 4;
-                        umma_f16_ss(tbase + kPaColS, qd + o, kd + o, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
+#pragma unroll 1
+        for (int w = blockIdx.x; w < a.items && wait.ok; w += gridDim.x) {
+            const PaItem item = pa_item(a, w);
+#pragma unroll 1
+            for (int at = item.t; at < item.count && wait.ok; at += item.t_step) {
+                const PaJob j = pa_job(a, item, at);
+                const int n = j.tiles();
+#pragma unroll 1
+                for (int i = 0; i < n; i++, it++) {
+                    int key, nk;
+                    bool own;
+                    j.tile(i, key, nk, own);
+                    wait(k_full, it & 1);
+                    if (!wait.ok) break;
+                    __syncwarp();
+                    tc_fence_after();
+                    if (lane == 0) {
+                        uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
+#pragma unroll 1
+                        for (int s = 0; s < HD / 16; s++) {
+                            umma_f16_ss(tbase + kPaColS, qd, kd, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
+                            const uint64_t step = ((s & 3) == 3 ? kPaPlane - 96 : 32) >> 4;
+                            qd += step, kd += step;
+                        }
+                        umma_commit(s_full);
                     }
-                    umma_commit(s_full);
-                }
-                __syncwarp();
-                wait(v_full, it & 1);
-                // keys of the tile's last 16-key step that do not exist: their P is 0,
-                // and 0 times whatever lies there must not be NaN
-                const int steps = (nk + 15) >> 4, gone = steps * 16 - nk;
-                if (gone && wait.ok) {
-                    for (int e = lane; e < gone * (HD / 8); e += 32) {
-                        const int row = nk + e / (HD / 8), ch = e % (HD / 8);
-                        *reinterpret_cast<uint4 *>(smem + L::kV + (ch >> 3) * kPaPlane + row * 128 + (ch & 7) * 16) =
-                            make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                    wait(v_full, it & 1);
+                    // keys of the tile's last 16-key step that do not exist: their P is 0,
+                    // and 0 times whatever lies there must not be NaN
+                    const int steps = (nk + 15) >> 4, gone = steps * 16 - nk;
+                    if (gone && wait.ok) {
+#pragma unroll 1
+                        for (int e = lane; e < gone * (HD / 8); e += 32) {
+                            const int row = nk + e / (HD / 8), ch = e % (HD / 8);
+                            *reinterpret_cast<uint4 *>(smem + L::kV + (ch >> 3) * kPaPlane + row * 128 +
+                                                       (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
                     }
-                    fence_proxy_async_smem();
+                    wait(p_ready, it & 1);
+                    if (!wait.ok) break;
+                    __syncwarp();
+                    tc_fence_after();
+                    if (lane == 0) {
+                        uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
+                        uint32_t p = tbase + kPaColS;
+                        constexpr uint32_t id = pa_idesc<T>(HD, true);
+#pragma unroll 1
+                        for (int s = 0; s < steps; s++, vd += 2048 >> 4, p += 8) {
+                            umma_f16_ts(tbase + kPaColO, p, vd, id, (i | s) ? 1u : 0u);
+                            if constexpr (kTwoPlanes) umma_f16_ts(tbase + kPaColO, p + 64, vd, id, 1u);
+                        }
+                        umma_commit(pv_done);
+                    }
                     __syncwarp();
                 }
-                wait(p_ready, it & 1);
-                if (!wait.ok) break;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
-                    constexpr uint32_t id = pa_idesc<T>(HD, true);
-                    for (int s = 0; s < steps; s++) {
-                        umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 8 * s, vd + ((s * 2048) >> 4), id,
-                                    (i | s) ? 1u : 0u);
-                        if constexpr (kTwoPlanes)
-                            umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 64 + 8 * s, vd + ((s * 2048) >> 4), id, 1u);
-                    }
-                    umma_commit(pv_done);
-                }
-                __syncwarp();
             }
-            if (!wait.ok) break;
         }
         if (!wait.ok && it) mbar_wait(pv_done, (it - 1) & 1);
     } else {  // ---- softmax: thread = row = TMEM lane
         const int row = threadIdx.x;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO;
-        for (int rt = item.rt; rt < item.rt_end; rt += item.rt_step) {
-            const PaJob j = pa_job(a, item, rt);
-            const int n = j.tiles();
-            const bool real = row < j.nrows, busy = 32 * warp < j.nrows;
-            const int gq = j.r0 + min(row, j.nrows - 1), tok = gq / a.group;
+#pragma unroll 1
+        for (int w = blockIdx.x; w < a.items; w += gridDim.x) {
+        const PaItem item = pa_item(a, w);
+#pragma unroll 1
+        for (int at = item.t; at < item.count; at += item.t_step) {
+            const PaJob j = pa_job(a, item, at);
+            const int n = j.tiles(), nrows = j.count * a.group;
+            const bool real = row < nrows, busy = 32 * warp < nrows;
+            const int in = min(row, nrows - 1), gq = j.first * a.group + in;
+            const int tok = j.first + (int)((uint32_t)in * a.group_inv >> 16);
             const int head = item.hk * a.group + gq - tok * a.group;
             const int pos = j.pos0 + tok;
-            float m_ref = -INFINITY, l = 0.f;
-            if (n) {
-                // Q rows (the last job's products have been waited for below)
-                for (int e = row; e < kPaRows * (HD / 8); e += kPaRows) {
-                    const int r = e / (HD / 8), ch = e % (HD / 8);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < j.nrows) {
-                        const int g = j.r0 + r, t = g / a.group, h = item.hk * a.group + g - t * a.group;
-                        v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (size_t)t * a.ldq +
-                                                             (size_t)h * HD + 8 * ch);
-                    }
-                    *reinterpret_cast<uint4 *>(smem + L::kQ + (ch >> 3) * kPaPlane + r * 128 +
-                                               (((ch & 7) ^ (r & 7)) << 4)) = v;
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(q_ready);
-            }
+            float m_ref = -INFINITY;
+            float2 l = make_float2(0.f, 0.f);
+#pragma unroll 1
             for (int i = 0; i < n; i++, it++) {
                 int key, nk;
                 bool own;
@@ -415,16 +454,34 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     // keys [0, lim) of the tile are visible to the row
                     const int lim = own && a.causal ? min(max(pos + 1 - key, 0), nk) : nk;
                     const bool all = __all_sync(0xffffffffu, lim == kPaKeys);
+                    // Three quarters of S stay in registers from the maximum to the weights;
+                    // the first is read again once two of them are done.
+                    float s0[32], s1[32], s2[32], s3[32];
+                    tmem_ld32(ts, s0);
+                    tmem_ld32(ts + 32, s1);
+                    tmem_ld_wait();
+                    tmem_regs_ready(s0);
+                    tmem_regs_ready(s1);
+                    tmem_ld32(ts + 64, s2);
                     float top = -INFINITY;
-                    float s[32];
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        tmem_ld32(ts + 32 * c, s);
-                        tmem_ld_wait();
-                        tmem_regs_ready(s);
+                    auto mask_and_max = [&](float (&x)[32], int c) {
+                        if (!all) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (all || 32 * c + e < lim) top = fmaxf(top, s[e]);
+                            for (int e = 0; e < 32; e++)
+                                if (32 * c + e >= lim) x[e] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(x[e], x[e + 1]));
+                    };
+                    mask_and_max(s0, 0);
+                    tmem_ld32(ts + 96, s3);
+                    mask_and_max(s1, 1);
+                    tmem_ld_wait();
+                    tmem_regs_ready(s2);
+                    tmem_regs_ready(s3);
+                    if (nk > 64) {
+                        mask_and_max(s2, 2);
+                        mask_and_max(s3, 3);
                     }
                     const float m_new = fmaxf(m_ref, top * a.scale_log2);
                     // O is rescaled only when the maximum has grown by more than 2^8 since
@@ -437,32 +494,32 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; c++) {
-                            tmem_ld32(to + 32 * c, s);
+                        for (int c = 0; c < HD / 8; c++) {
+                            float o[8];
+                            tmem_ld8(to + 8 * c, o);
                             tmem_ld_wait();
-                            tmem_regs_ready(s);
+                            tmem_regs_ready(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) s[e] *= f;
-                            tmem_st32(to + 32 * c, s);
+                            for (int e = 0; e < 8; e++) o[e] *= f;
+                            tmem_st8(to + 8 * c, o);
                         }
                         tmem_st_wait();
-                        l *= f;
+                        l.x *= f, l.y *= f;
                         m_ref = m_new;
                     }
-                    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-                    auto weights = [&](float (&x)[32], int c) {
+                    const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+                    const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
+                    // P over S: quarter c goes to columns 16 c (and 64 + 16 c), which hold
+                    // quarters that have been read
+                    auto weights = [&](const float (&x)[32], int c) {
                         uint32_t hi[16], lo[16];
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            float p0 = exp2_fast(fmaf(x[2 * e], a.scale_log2, -m_use));
-                            float p1 = exp2_fast(fmaf(x[2 * e + 1], a.scale_log2, -m_use));
-                            if (!all) {
-                                if (32 * c + 2 * e >= lim) p0 = 0.f;
-                                if (32 * c + 2 * e + 1 >= lim) p1 = 0.f;
-                            }
-                            l += p0 + p1;
+                            const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
+                            const float2 w = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                            l = fadd2(l, w);
                             float r0, r1;
-                            hi[e] = pa_pack<T>(p0, p1, r0, r1);
+                            hi[e] = pa_pack<T>(w.x, w.y, r0, r1);
                             if constexpr (kTwoPlanes) {
                                 float u0, u1;
                                 lo[e] = pa_pack<T>(r0, r1, u0, u1);
@@ -471,27 +528,18 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         tmem_st16(ts + 16 * c, hi);
                         if constexpr (kTwoPlanes) tmem_st16(ts + 64 + 16 * c, lo);
                     };
-                    // P overwrites S from the left; the second plane starts at column 64, so
-                    // that half of S is taken into registers first
-                    float u[2][32];
-                    if constexpr (kTwoPlanes) {
-                        tmem_ld32(ts + 64, u[0]);
-                        tmem_ld32(ts + 96, u[1]);
-                        tmem_ld_wait();
-                        tmem_regs_ready(u[0]);
-                        tmem_regs_ready(u[1]);
-                    }
+                    if (nk > 96) weights(s3, 3);
+                    tmem_ld32(ts, s0);
+                    if (nk > 64) weights(s2, 2);
+                    tmem_ld_wait();
+                    tmem_regs_ready(s0);
+                    if (!all) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        if (kTwoPlanes && c >= 2) {
-                            weights(u[c & 1], c);
-                        } else {
-                            tmem_ld32(ts + 32 * c, s);
-                            tmem_ld_wait();
-                            tmem_regs_ready(s);
-                            weights(s, c);
-                        }
+                        for (int e = 0; e < 32; e++)
+                            if (e >= lim) s0[e] = -INFINITY;
                     }
+                    if (nk > 32) weights(s1, 1);
+                    weights(s0, 0);
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -503,9 +551,11 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                 tc_fence_after();
             }
             if (busy) {
-                const size_t at = ((size_t)item.split * a.rows + tok) * a.n_q + head;
-                if (real && !a.direct) a.ml_part[at] = make_float2(m_ref, l);
-                const float f = a.direct ? 1.f / l : 1.f;
+                const float sum = l.x + l.y;
+                const size_t blk = (size_t)(item.split * a.n_kv + item.hk) * a.row_blocks;
+                if (real && !a.direct) a.ml_part[blk * 32 + gq] = make_float2(m_ref, sum);
+                float *part = a.o_part + (blk + (gq >> 5)) * (32 * HD) + (gq & 31) * 4;
+                const float f = a.direct ? 1.f / sum : 1.f;
                 float o[32];
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; c++) {
@@ -515,7 +565,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         tmem_regs_ready(o);
                     }
                     if (real && (a.direct || n)) {
-                        const bool none = !n || l == 0.f;  // no visible key: 0
+                        const bool none = !n || sum == 0.f;  // no visible key: 0
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
                             const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
@@ -524,13 +574,14 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                                 pa_store4(static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)head * HD + 32 * c + e,
                                           v);
                             else
-                                pa_store4(a.o_part + at * HD + 32 * c + e, v);
+                                pa_store4(part + (32 * c + e) * 32, v);
                         }
                     }
                     __syncwarp();
                 }
             }
             tc_fence_before();  // O has been read before the next job's products overwrite it
+        }
         }
     }
     __syncthreads();
@@ -541,72 +592,65 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     }
 }
 
-template <int W>
-struct alignas(4 * W) PaVec {
-    float v[W];
-};
-
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits that saw a
-// key, 0 if none did; one warp per (row, head).  Rows outside
-// [seq_start[0], seq_start[n_seqs]) belong to no sequence and stay as they are.
+// key, 0 if none did.  One warp per 32 rows of a KV head and 8 dims, a lane per
+// row: the states' pieces are read 512 bytes at a time, 8 splits in flight.
+// Rows outside [seq_start[0], seq_start[n_seqs]) belong to no sequence and stay
+// as they are.
 template <class TO, int HD>
 __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_constant__ PaArgs a) {
+    constexpr int kPer = HD / 8, kBatch = 8;  // warps of a block of rows; splits in flight
     griddep_wait();  // the partial states
-    const int rh = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int row = rh / a.n_q;
-    if (row >= a.rows || row < a.seq_start[0] || row >= a.seq_start[a.n_seqs]) return;
+    const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int piece = w % kPer, blk = w / kPer % a.row_blocks, hk = w / kPer / a.row_blocks;
+    const int gq = blk * 32 + lane, tok = gq / a.group;
+    if (hk >= a.n_kv || gq >= a.rows * a.group || tok < a.seq_start[0] || tok >= a.seq_start[a.n_seqs]) return;
     const int splits = a.prefix_splits + a.seq_splits;
-    const size_t stride = (size_t)a.rows * a.n_q;
-    constexpr int W = HD / 32;  // dims of a lane
+    const size_t stride = (size_t)a.n_kv * a.row_blocks;  // blocks of a split
+    const size_t at = (size_t)hk * a.row_blocks + blk;
+    const float2 *ml = a.ml_part + at * 32 + lane;
+    const float4 *op = reinterpret_cast<const float4 *>(a.o_part + at * (32 * HD)) + piece * 64 + lane;
     float M = -INFINITY;
-    for (int s = lane; s < splits; s += 32) M = fmaxf(M, a.ml_part[s * stride + rh].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float Lsum = 0.f, O[W];
-#pragma unroll
-    for (int d = 0; d < W; d++) O[d] = 0.f;
-    for (int s0 = 0; s0 < splits; s0 += 32) {
-        float w = 0.f;
-        if (s0 + lane < splits) {
-            const float2 ml = a.ml_part[(s0 + lane) * stride + rh];
-            w = ml.y != 0.f ? exp2f(ml.x - M) : 0.f;
-            Lsum += ml.y * w;
-        }
-        const int ns = min(32, splits - s0);
 #pragma unroll 8
-        for (int j = 0; j < ns; j++) {
-            const float b = __shfl_sync(0xffffffffu, w, j);
-            if (b == 0.f) continue;  // that state's O may be unwritten
-            const PaVec<W> p =
-                *reinterpret_cast<const PaVec<W> *>(a.o_part + ((s0 + j) * stride + rh) * HD + W * lane);
+    for (int s = 0; s < splits; s++) M = fmaxf(M, ml[s * stride * 32].x);
+    float sum = 0.f, o[8] = {};
+    for (int s0 = 0; s0 < splits; s0 += kBatch) {
+        float2 st[kBatch];
+        float4 x[kBatch][2];
 #pragma unroll
-            for (int d = 0; d < W; d++) O[d] += p.v[d] * b;
-        }
+        for (int u = 0; u < kBatch; u++)
+            if (s0 + u < splits) {
+                st[u] = ml[(s0 + u) * stride * 32];
+                x[u][0] = op[(s0 + u) * stride * (8 * HD)];
+                x[u][1] = op[(s0 + u) * stride * (8 * HD) + 32];
+            }
+#pragma unroll
+        for (int u = 0; u < kBatch; u++)
+            if (s0 + u < splits && st[u].y != 0.f) {  // O of a state that saw no key may be unwritten
+                const float f = exp2f(st[u].x - M);
+                sum += st[u].y * f;
+                o[0] += x[u][0].x * f, o[1] += x[u][0].y * f, o[2] += x[u][0].z * f, o[3] += x[u][0].w * f;
+                o[4] += x[u][1].x * f, o[5] += x[u][1].y * f, o[6] += x[u][1].z * f, o[7] += x[u][1].w * f;
+            }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) Lsum += __shfl_xor_sync(0xffffffffu, Lsum, o);
-    const float f = Lsum != 0.f ? 1.f / Lsum : 0.f;
-    TO *out = static_cast<TO *>(a.out) + (size_t)row * a.ldo + (size_t)(rh - row * a.n_q) * HD + W * lane;
-#pragma unroll
-    for (int d = 0; d < W; d++) {
-        if constexpr (std::is_same<TO, float>::value) out[d] = O[d] * f;
-        else if constexpr (std::is_same<TO, __half>::value) out[d] = __float2half_rn(O[d] * f);
-        else out[d] = __float2bfloat16_rn(O[d] * f);
-    }
+    const float f = sum != 0.f ? 1.f / sum : 0.f;
+    TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)(hk * a.group + gq - tok * a.group) * HD + 8 * piece;
+    pa_store4(out, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
+    pa_store4(out + 4, make_float4(o[4] * f, o[5] * f, o[6] * f, o[7] * f));
 }
 
-// Rows of `inner` elements, ld apart, [rows] or [seqs][rows]; box of 64 elements
-// x kPaBoxRows rows in the 128-byte swizzle; rows past the end read as zero.
-int pa_map(CUtensorMap *tm, const void *p, int dtype, uint64_t inner, uint64_t rows, uint64_t ld, uint64_t seqs,
-           uint64_t seq_ld) {
+// A tensor of dims[0] contiguous elements and strides ld[] (elements) of the
+// outer dims, copied in boxes of 64 elements x box1 (x box2) in the 128-byte
+// swizzle; what lies past an end reads as zero.
+int pa_map(CUtensorMap *tm, const void *p, int dtype, int nd, const uint64_t (&dims)[3], const uint64_t (&ld)[2],
+           uint32_t box1, uint32_t box2) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
     if (int s = lc_tensor_map_encoder(&enc)) return s;
-    cuuint64_t dims[3] = {inner, rows, seqs};
-    cuuint64_t strides[2] = {ld * 2, seq_ld * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)kPaBoxRows, 1}, es[3] = {1, 1, 1};
+    cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, strides[2] = {ld[0] * 2, ld[1] * 2};
+    cuuint32_t box[3] = {64, box1, box2}, es[3] = {1, 1, 1};
     const CUresult r =
-        enc(tm, dtype == LC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, seqs ? 3 : 2,
-            const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        enc(tm, dtype == LC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, nd,
+            const_cast<void *>(p), d, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LC_REQUIRE(r == CUDA_SUCCESS, LC_ERR_CUDA, "lc_prefix_attn: cuTensorMapEncodeTiled failed (%d)", (int)r);
     return LC_OK;
@@ -618,7 +662,18 @@ int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 void pa_plan(PaArgs &a, int num_sms) {
     const int slots = 2 * num_sms;  // CTAs resident at once
     const int64_t R = (int64_t)a.rows * a.group;
-    const int per_seq = div_up(div_up(R, a.n_seqs), kPaRows);  // row tiles of an average sequence
+    // Tokens of a row tile: as many as fit 128 rows in whole copies of Q, which hold
+    // about 32 rows and, where several make a tile, a multiple of 8 rows (the swizzle's
+    // period)
+    int unit = 1;
+    while (unit * a.group % 8) unit *= 2;
+    if (unit * a.group > kPaRows) {
+        a.box_toks = a.tile_toks = kPaRows / a.group;
+    } else {
+        a.box_toks = unit * std::max(1, 32 / (unit * a.group));
+        a.tile_toks = kPaRows / (a.box_toks * a.group) * a.box_toks;
+    }
+    const int per_seq = div_up(div_up(a.rows, a.n_seqs), a.tile_toks);  // row tiles of an average sequence
     a.seq_lanes = std::max(1, per_seq);
     // A sequence whose rows fill tiles by themselves gains nothing from sharing
     // the prefix with others: its items run over [prefix | own] in one go.
@@ -626,7 +681,7 @@ void pa_plan(PaArgs &a, int num_sms) {
     a.prefix_items = 0, a.prefix_splits = 0, a.row_tiles = 1, a.prefix_keys = kPaKeys;
     a.seq_from = joint ? 0 : a.prefix_len;
     if (!joint) {
-        a.row_tiles = div_up(R, kPaRows);
+        a.row_tiles = div_up(a.rows, a.tile_toks);
         const int base = a.n_kv * a.row_tiles, tiles = div_up(a.prefix_len, kPaKeys);
         const int per = div_up(tiles, std::min(tiles, std::max(1, slots / base)));
         a.prefix_keys = per * kPaKeys;
@@ -646,15 +701,16 @@ void pa_plan(PaArgs &a, int num_sms) {
 }
 
 template <class T, class TO, int HD>
-int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[4]) {
+int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[5]) {
     auto kernel = prefix_attn_kernel<T, TO, HD>;
     if (items) {
         if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
-        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(tm[0], tm[1], tm[2], tm[3], a);
+        kernel<<<std::min(items, 2 * ctx->num_sms), kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(
+            tm[0], tm[1], tm[2], tm[3], tm[4], a);
     }
     if (!a.direct) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(div_up((int64_t)a.rows * a.n_q, 4));
+        cfg.gridDim = dim3(div_up((int64_t)a.n_kv * a.row_blocks * (HD / 8), 4));
         cfg.blockDim = dim3(128);
         cfg.stream = ctx->stream;
         cudaLaunchAttribute attr[1];
@@ -668,7 +724,7 @@ int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[4
 }
 
 template <class T>
-int pa_types(lc_ctx *ctx, int out_dtype, uint32_t hd, const PaArgs &a, int items, const CUtensorMap (&tm)[4]) {
+int pa_types(lc_ctx *ctx, int out_dtype, uint32_t hd, const PaArgs &a, int items, const CUtensorMap (&tm)[5]) {
     if (out_dtype == LC_F32)
         return hd == 128 ? pa_launch<T, float, 128>(ctx, a, items, tm) : pa_launch<T, float, 64>(ctx, a, items, tm);
     return hd == 128 ? pa_launch<T, T, 128>(ctx, a, items, tm) : pa_launch<T, T, 64>(ctx, a, items, tm);
@@ -688,6 +744,8 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
                head_dim);
     LC_REQUIRE(n_kv_heads > 0 && n_q_heads % n_kv_heads == 0, LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: n_q_heads %u must be a multiple of n_kv_heads %u", n_q_heads, n_kv_heads);
+    LC_REQUIRE(n_q_heads / n_kv_heads <= (uint32_t)kPaRows, LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: %u query heads to a KV head (at most %d)", n_q_heads / n_kv_heads, kPaRows);
     LC_REQUIRE(scale >= 0.f && scale < INFINITY, LC_ERR_INVALID,
                "lc_prefix_attn: scale %g must be finite and not negative", scale);
     if (rows == 0 || n_q_heads == 0) return LC_OK;
@@ -698,7 +756,7 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
                LC_ERR_INVALID, "lc_prefix_attn: null pointer");
     LC_REQUIRE(kv->n_seqs <= (1u << 20), LC_ERR_UNSUPPORTED, "lc_prefix_attn: %u sequences", kv->n_seqs);
     const uint64_t wq = (uint64_t)n_q_heads * head_dim, wk = (uint64_t)n_kv_heads * head_dim;
-    LC_REQUIRE((uint64_t)rows * n_q_heads <= 0x7FFFF000u && wq < (1u << 24), LC_ERR_UNSUPPORTED,
+    LC_REQUIRE((uint64_t)rows * n_q_heads <= (1u << 29) && wq < (1u << 24), LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: %u rows of %u heads", rows, n_q_heads);
     LC_REQUIRE((uint64_t)kv->prefix_len + kv->own_cap <= kPaMaxLen, LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: %u + %u keys", kv->prefix_len, kv->own_cap);
@@ -731,27 +789,36 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     a.rows = (int)rows, a.n_q = (int)n_q_heads, a.n_kv = (int)n_kv_heads, a.group = a.n_q / a.n_kv;
     a.prefix_len = (int)kv->prefix_len, a.own_cap = (int)kv->own_cap, a.n_seqs = (int)kv->n_seqs;
     a.own_len = kv->own_cap ? kv->own_len : nullptr, a.seq_start = kv->seq_start;
+    a.group_inv = (65536 + a.group - 1) / a.group;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.causal = causal != 0;
     a.status = ctx->dev_status;
     pa_plan(a, ctx->num_sms);
     const int64_t items = (int64_t)a.prefix_items + (int64_t)a.n_kv * a.n_seqs * a.seq_lanes * a.seq_splits;
     LC_REQUIRE(items <= 0x7FFFFFFF, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
+    a.items = (int)items;
     if (!a.direct) {
-        const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * rows * n_q_heads;
+        a.row_blocks = div_up((int64_t)rows * a.group, 32);
+        const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;
         void *scr = nullptr;
         if (int s = lc_scratch_kept(ctx, LC_SCRATCH_PREFIX, states * (head_dim * 4 + 8) + 256, &scr)) return s;
         a.ml_part = (float2 *)scr;
         a.o_part = (float *)((char *)scr + ((states * 8 + 255) & ~(size_t)255));
     }
-    CUtensorMap tm[4] = {};
+    CUtensorMap tm[5] = {};
     if (a.prefix_len) {
-        if (int s = pa_map(&tm[0], kv->k_prefix, dtype, wk, kv->prefix_len, ldp, 0, 0)) return s;
-        if (int s = pa_map(&tm[1], kv->v_prefix, dtype, wk, kv->prefix_len, ldp, 0, 0)) return s;
+        const uint64_t dims[3] = {wk, kv->prefix_len, 1}, ld[2] = {ldp, 0};
+        if (int s = pa_map(&tm[0], kv->k_prefix, dtype, 2, dims, ld, kPaBoxRows, 1)) return s;
+        if (int s = pa_map(&tm[1], kv->v_prefix, dtype, 2, dims, ld, kPaBoxRows, 1)) return s;
     }
     if (a.own_cap) {
-        if (int s = pa_map(&tm[2], kv->k_own, dtype, wk, kv->own_cap, ldw, kv->n_seqs, seq_ld)) return s;
-        if (int s = pa_map(&tm[3], kv->v_own, dtype, wk, kv->own_cap, ldw, kv->n_seqs, seq_ld)) return s;
+        const uint64_t dims[3] = {wk, kv->own_cap, kv->n_seqs}, ld[2] = {ldw, seq_ld};
+        if (int s = pa_map(&tm[2], kv->k_own, dtype, 3, dims, ld, kPaBoxRows, 1)) return s;
+        if (int s = pa_map(&tm[3], kv->v_own, dtype, 3, dims, ld, kPaBoxRows, 1)) return s;
+    }
+    {  // Q as [token][head][head_dim]: a box is the heads of a group for box_toks tokens, in row order
+        const uint64_t dims[3] = {head_dim, n_q_heads, rows}, ld[2] = {head_dim, ldq};
+        if (int s = pa_map(&tm[4], q, dtype, 3, dims, ld, a.group, a.box_toks)) return s;
     }
     return dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, tm)
                            : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, tm);

@@ -133,7 +133,8 @@ def test_small(ctx, dev, src, dst, hd, prefix, cap, counts, lens):
 
 
 @pytest.mark.parametrize("src,dst", TYPES)
-@pytest.mark.parametrize("n_q,n_kv", [(1, 1), (5, 1), (8, 8), (32, 8), (24, 2), (48, 8)])
+@pytest.mark.parametrize("n_q,n_kv", [(1, 1), (5, 1), (8, 8), (32, 8), (24, 2), (48, 8), (3, 1), (9, 1), (17, 1), (40, 1),
+                                       (64, 1), (100, 1), (128, 1)])
 def test_head_layouts(ctx, dev, src, dst, n_q, n_kv):
     b = Batch(dev, src, dst, n_q, n_kv, 128, 500, 100, [1, 7, 2, 1], [33, 100, 60, 1], seed=n_q)
     b.run(ctx)

@@ -37,7 +37,7 @@ def test_invalid(over):
 
 @pytest.mark.parametrize("over", [
     dict(dtype=lc.F32, out_dtype=lc.F32), dict(dtype=lc.Q8_0), dict(out_dtype=lc.F16), dict(hd=32), dict(hd=96),
-    dict(hd=256), dict(n_kv=0), dict(n_kv=3), dict(rows=1 << 31), dict(kv=dict(prefix_len=1 << 30)),
+    dict(hd=256), dict(n_kv=0), dict(n_kv=3), dict(rows=1 << 31), dict(rows=(1 << 26) + 1), dict(n_q=258), dict(kv=dict(prefix_len=1 << 30)),
     dict(kv=dict(own_cap=0x3FFFF000), ), dict(kv=dict(n_seqs=(1 << 20) + 1))], ids=str)
 def test_unsupported(over):
     assert call(**over) == lc.LC_ERR_UNSUPPORTED
