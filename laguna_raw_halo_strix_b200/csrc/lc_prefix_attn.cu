@@ -15,11 +15,12 @@
 //   P           softmax warps, one thread a row, written over S as 16-bit pairs
 //               (and a second plane of what the rounding lost, for f32 outputs)
 //   O += P V    tcgen05, P from TMEM, V read MN-major as it lies in memory
-// Q, K and V come by TMA.  Roles: warps 0-3 softmax, 4 loads, 5 MMA.  S and P
+// Q, K and V come by TMA.  Roles: warps 0-7 softmax, 8 loads, 9 MMA.  S and P
 // share their TMEM columns, so within a CTA a tile's products and its softmax
 // alternate; two CTAs share an SM (256 TMEM columns and 98 KB each) and fill
 // each other's gaps.  CTAs stay for several items: the next item's Q and K are
 // loaded while the last one's weights, values and results are worked on.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -32,7 +33,8 @@
 namespace {
 
 constexpr int kPaRows = 128, kPaKeys = 128;
-constexpr int kPaThreads = 192;
+constexpr int kPaLoadWarp = 8, kPaMmaWarp = 9;  // 0..7 softmax
+constexpr int kPaThreads = 320;
 constexpr int kPaBoxRows = 32;             // key rows of one TMA copy
 constexpr uint32_t kPaPlane = 128 * 128;   // 128 rows x 64 16-bit elements (one swizzle span)
 constexpr uint32_t kPaColS = 0, kPaColO = 128, kPaTmemCols = 256;
@@ -43,7 +45,8 @@ template <int HD>
 struct PaSmem {
     static constexpr uint32_t kTile = HD / 64 * kPaPlane;
     static constexpr uint32_t kQ = 0, kK = kTile, kV = 2 * kTile, kBar = 3 * kTile;
-    static constexpr uint32_t kBytes = kBar + 64 + 1024;  // + slack to 1024-align the base
+    static constexpr uint32_t kSched = kBar + 80, kJobs = kSched + 48, kRed = kJobs + 128;  // kRed: maxima [2][kPaRows], sums [2][kPaRows]
+    static constexpr uint32_t kBytes = kRed + 4 * kPaRows * 4 + 1024;  // + slack to 1024-align the base
 };
 
 struct PaArgs {
@@ -57,10 +60,10 @@ struct PaArgs {
     const int32_t *own_len, *seq_start;
     float scale_log2;  // scale * log2(e)
     int causal;
-    // plan: CTA c runs items c, c + gridDim.x, ..; items 0 .. prefix_items - 1 take the prefix for rows of all
+    // plan: items 0 .. prefix_items - 1 take the prefix for rows of all
     // sequences, the rest rows of one sequence over [seq_from, end) of the
     // virtual axis
-    int items, prefix_items, row_tiles, prefix_keys;
+    int prefix_items, row_tiles, prefix_keys;
     int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
     int direct;         // one split covers everything: items write out
     // partial states of row r = token * group + head within the group: O
@@ -77,10 +80,10 @@ struct PaArgs {
 // head within the group) of one KV head against prefix keys [p0, p1) and keys
 // [o0, o1) of sequence seq.
 struct PaJob {
-    int first, count, p0, p1, o0, o1, seq;
+    int n;  // tiles; -1: no more jobs
+    int first, count, p0, p1, o0, o1, seq, hk, split;
     int pos0;  // own position of token t is pos0 + t
     __device__ __forceinline__ int prefix_tiles() const { return (p1 - p0 + kPaKeys - 1) / kPaKeys; }
-    __device__ __forceinline__ int tiles() const { return prefix_tiles() + (o1 - o0 + kPaKeys - 1) / kPaKeys; }
     // tile i: first key, keys, own or prefix
     __device__ __forceinline__ void tile(int i, int &key, int &nk, bool &own) const {
         const int np = prefix_tiles();
@@ -89,6 +92,9 @@ struct PaJob {
         nk = min(kPaKeys, (own ? o1 : p1) - key);
     }
 };
+
+// Token of row r < 128 of a tile, within the tile.
+__device__ __forceinline__ int pa_token(const PaArgs &a, int r) { return (int)((uint32_t)r * a.group_inv >> 16); }
 
 struct PaItem {
     int hk, split, t, t_step;  // token tiles at t, t + t_step, .. below count
@@ -130,13 +136,14 @@ __device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int at
     PaJob j;
     j.first = t.start + at;
     j.count = min(a.tile_toks, t.count - at);
-    j.seq = t.seq;
     j.pos0 = t.len - t.count - t.start;
     j.p0 = min(t.v0, a.prefix_len), j.p1 = min(t.v1, a.prefix_len);
     j.o0 = max(t.v0, a.prefix_len) - a.prefix_len;
     j.o1 = min(max(t.v1, a.prefix_len) - a.prefix_len, t.len);
     if (a.causal) j.o1 = min(j.o1, j.pos0 + j.first + j.count);  // the last token's reach
     j.o1 = max(j.o1, j.o0);
+    j.n = j.prefix_tiles() + (j.o1 - j.o0 + kPaKeys - 1) / kPaKeys;
+    j.seq = t.seq, j.hk = t.hk, j.split = t.split;
     return j;
 }
 
@@ -159,6 +166,89 @@ struct PaWait {
             ok = false;
             atomicOr(status, LC_DEV_WAIT_TIMEOUT);
         }
+    }
+};
+
+// The two warps of a lane quarter meet (named barriers 1..4; the id an immediate),
+// the second form telling all 64 threads whether any of them said `yes`.
+__device__ __forceinline__ void pa_meet(int quarter) {
+    switch (quarter) {
+    case 0: asm volatile("bar.sync 1, 64;\n" ::: "memory"); break;
+    case 1: asm volatile("bar.sync 2, 64;\n" ::: "memory"); break;
+    case 2: asm volatile("bar.sync 3, 64;\n" ::: "memory"); break;
+    default: asm volatile("bar.sync 4, 64;\n" ::: "memory"); break;
+    }
+}
+__device__ __forceinline__ bool pa_meet_any(int quarter, bool yes) {
+    uint32_t any;
+#define LC_MEET(ID)                                                                                      \
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, " #ID               \
+                 ", 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"                                                \
+                 : "=r"(any)                                                                             \
+                 : "r"((uint32_t)yes)                                                                    \
+                 : "memory")
+    switch (quarter) {
+    case 0: LC_MEET(1); break;
+    case 1: LC_MEET(2); break;
+    case 2: LC_MEET(3); break;
+    default: LC_MEET(4); break;
+    }
+#undef LC_MEET
+    return any != 0;
+}
+
+// Items beyond a CTA's own: a resident CTA takes over CTAs of the grid that have
+// not been launched (cluster launch control), so long and short items even out
+// without a counter in memory.  Asked for one item ahead, by the load thread; an
+// answer holds the taken CTA's index, or that none was left.
+struct PaSched {
+    unsigned char *at;  // answer, then a barrier
+    uint32_t got = 0;
+    __device__ __forceinline__ uint64_t *bar() { return reinterpret_cast<uint64_t *>(at + 16); }
+    __device__ __forceinline__ void ask() {
+        mbar_expect_tx(bar(), 16);
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(
+                         smem_addr(at)),
+                     "r"(smem_addr(bar()))
+                     : "memory");
+    }
+    __device__ __forceinline__ int next(PaWait &wait) {  // the next item, -1 if there is none
+        wait(bar(), got++ & 1);
+        if (!wait.ok) return -1;
+        int w;
+        asm volatile(
+            "{\n .reg .b128 h;\n .reg .pred p;\n mov.u32 %0, -1;\n ld.shared.b128 h, [%1];\n"
+            " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+            " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}\n"
+            : "=&r"(w)
+            : "r"(smem_addr(at))
+            : "memory");
+        fence_proxy_async_smem();  // read before the next answer is written there
+        return w;
+    }
+};
+
+// Jobs in shared memory, from the load thread to the other warps: two slots, each
+// filled once and released by the 8 softmax warps and the MMA warp.
+struct PaJobs {
+    PaJob *slot;
+    uint64_t *bar;  // full[2], empty[2]
+    uint32_t k = 0;
+    __device__ __forceinline__ void put(PaWait &wait, const PaJob &j) {
+        if (k >= 2) wait(bar + 2 + (k & 1), ((k >> 1) - 1) & 1);
+        if (!wait.ok) return;
+        slot[k & 1] = j;
+        mbar_arrive(bar + (k & 1));
+        k++;
+    }
+    __device__ __forceinline__ const PaJob &get(PaWait &wait) {
+        wait(bar + (k & 1), (k >> 1) & 1);
+        return slot[k & 1];
+    }
+    __device__ __forceinline__ void release(int lane) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar + 2 + (k & 1));
+        k++;
     }
 };
 
@@ -271,6 +361,20 @@ __device__ __forceinline__ void pa_store4(T *p, float4 v) {
     *reinterpret_cast<uint2 *>(p) = u;
 }
 
+__device__ __forceinline__ void pa_store16(float *p, const float (&v)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) pa_store4(p + e, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+}
+template <class T>
+__device__ __forceinline__ void pa_store16(T *p, const float (&v)[16]) {
+    float l;
+#pragma unroll
+    for (int e = 0; e < 16; e += 8)
+        *reinterpret_cast<uint4 *>(p + e) =
+            make_uint4(pa_pack<T>(v[e], v[e + 1], l, l), pa_pack<T>(v[e + 2], v[e + 3], l, l),
+                       pa_pack<T>(v[e + 4], v[e + 5], l, l), pa_pack<T>(v[e + 6], v[e + 7], l, l));
+}
+
 template <class T, class TO, int HD>
 __global__ void __launch_bounds__(kPaThreads, 2)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap kp, const __grid_constant__ CUtensorMap vp,
@@ -283,8 +387,10 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
     uint64_t *k_full = bar, *v_full = bar + 1, *s_full = bar + 2, *p_ready = bar + 3, *pv_done = bar + 4;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 5);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 9);
     const uint32_t sbase = smem_addr(smem);
+    PaSched sched{smem + L::kSched};
+    PaJobs jobs{reinterpret_cast<PaJob *>(smem + L::kJobs), bar + 5};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     griddep_launch_dependents();  // the merge kernel may be scheduled once the last items run
@@ -292,11 +398,16 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         mbar_init(k_full, 1);
         mbar_init(v_full, 1);
         mbar_init(s_full, 1);
-        mbar_init(p_ready, kPaRows);
+        mbar_init(p_ready, 8);
         mbar_init(pv_done, 1);
+        mbar_init(sched.bar(), 1);
+        for (int k = 0; k < 2; k++) {
+            mbar_init(jobs.bar + k, 1);
+            mbar_init(jobs.bar + 2 + k, 9);
+        }
         mbar_init_fence();
     }
-    if (warp == 5) {
+    if (warp == kPaMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
                      "r"(kPaTmemCols)
                      : "memory");
@@ -309,17 +420,18 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     PaWait wait{a.status};
     uint32_t it = 0;  // tiles so far: every barrier completes once per tile
 
-    if (warp == 4) {  // ---- loads
+    if (warp == kPaLoadWarp) {  // ---- loads
         if (lane == 0) {
 #pragma unroll 1
-            for (int w = blockIdx.x; w < a.items && wait.ok; w += gridDim.x) {
+            for (int w = blockIdx.x; w >= 0; w = sched.next(wait)) {
+                sched.ask();
                 const PaItem item = pa_item(a, w);
 #pragma unroll 1
                 for (int at = item.t; at < item.count && wait.ok; at += item.t_step) {
                     const PaJob j = pa_job(a, item, at);
-                    const int n = j.tiles();
+                    jobs.put(wait, j);
 #pragma unroll 1
-                    for (int i = 0; i < n && wait.ok; i++, it++) {
+                    for (int i = 0; i < j.n && wait.ok; i++, it++) {
                         int key, nk;
                         bool own;
                         j.tile(i, key, nk, own);
@@ -357,19 +469,21 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     }
                 }
             }
+            PaJob last = {};
+            last.n = -1;
+            jobs.put(wait, last);
             if (!wait.ok) {  // copies of this CTA still in flight
                 mbar_wait(k_full, it & 1);
                 mbar_wait(v_full, it ? (it - 1) & 1 : 0);
             }
         }
-    } else if (warp == 5) {  // ---- products
+    } else if (warp == kPaMmaWarp) {  // ---- products
 #pragma unroll 1
-        for (int w = blockIdx.x; w < a.items && wait.ok; w += gridDim.x) {
-            const PaItem item = pa_item(a, w);
-#pragma unroll 1
-            for (int at = item.t; at < item.count && wait.ok; at += item.t_step) {
-                const PaJob j = pa_job(a, item, at);
-                const int n = j.tiles();
+        while (wait.ok) {
+            const PaJob &j = jobs.get(wait);
+            const int n = wait.ok ? j.n : -1;
+            if (n < 0) break;
+            {
 #pragma unroll 1
                 for (int i = 0; i < n; i++, it++) {
                     int key, nk;
@@ -422,170 +536,171 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     __syncwarp();
                 }
             }
+            jobs.release(lane);
         }
         if (!wait.ok && it) mbar_wait(pv_done, (it - 1) & 1);
-    } else {  // ---- softmax: thread = row = TMEM lane
-        const int row = threadIdx.x;
-        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-        const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO;
+    } else {  // ---- softmax
+        // Row = TMEM lane; the two warps of a lane quarter take 64 keys of a tile, and half
+        // of O's columns, each (64 scores in registers; one warp per quarter and 128 keys
+        // left the chain of a tile 1.6x as long).  Thread pairs meet at a barrier of their
+        // two warps: `meet` also says that both have read S, which P overwrites.
+        const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO + half * (HD / 2);
+        float *mine = reinterpret_cast<float *>(smem + L::kRed) + half * kPaRows + row;
+        const float *other = reinterpret_cast<float *>(smem + L::kRed) + (half ^ 1) * kPaRows + row;
 #pragma unroll 1
-        for (int w = blockIdx.x; w < a.items; w += gridDim.x) {
-        const PaItem item = pa_item(a, w);
+        while (true) {
+            const PaJob &j = jobs.get(wait);
+            // a warp that gave up takes its partner along, which would wait for it
+            if (pa_meet_any(quarter, !wait.ok || j.n < 0)) break;
+            const int n = j.n;
+            {
+                const bool busy = 32 * quarter < j.count * a.group;
+                float m_ref = -INFINITY;
+                float2 l = make_float2(0.f, 0.f);
 #pragma unroll 1
-        for (int at = item.t; at < item.count; at += item.t_step) {
-            const PaJob j = pa_job(a, item, at);
-            const int n = j.tiles(), nrows = j.count * a.group;
-            const bool real = row < nrows, busy = 32 * warp < nrows;
-            const int in = min(row, nrows - 1), gq = j.first * a.group + in;
-            const int tok = j.first + (int)((uint32_t)in * a.group_inv >> 16);
-            const int head = item.hk * a.group + gq - tok * a.group;
-            const int pos = j.pos0 + tok;
-            float m_ref = -INFINITY;
-            float2 l = make_float2(0.f, 0.f);
-#pragma unroll 1
-            for (int i = 0; i < n; i++, it++) {
-                int key, nk;
-                bool own;
-                j.tile(i, key, nk, own);
-                wait(s_full, it & 1);
-                __syncwarp();
-                tc_fence_after();
-                if (busy) {
-                    // keys [0, lim) of the tile are visible to the row
-                    const int lim = own && a.causal ? min(max(pos + 1 - key, 0), nk) : nk;
-                    const bool all = __all_sync(0xffffffffu, lim == kPaKeys);
-                    // Three quarters of S stay in registers from the maximum to the weights;
-                    // the first is read again once two of them are done.
-                    float s0[32], s1[32], s2[32], s3[32];
-                    tmem_ld32(ts, s0);
-                    tmem_ld32(ts + 32, s1);
-                    tmem_ld_wait();
-                    tmem_regs_ready(s0);
-                    tmem_regs_ready(s1);
-                    tmem_ld32(ts + 64, s2);
-                    float top = -INFINITY;
-                    auto mask_and_max = [&](float (&x)[32], int c) {
-                        if (!all) {
+                for (int i = 0; i < n; i++, it++) {
+                    int key, nk;
+                    bool own;
+                    j.tile(i, key, nk, own);
+                    wait(s_full, it & 1);
+                    __syncwarp();
+                    if (busy) {
+                        tc_fence_after();
+                        // keys [0, lim) of this half are visible to the row
+                        int lim = nk;
+                        if (own && a.causal)
+                            lim = min(max(j.pos0 + j.first + pa_token(a, row) + 1 - key, 0), nk);
+                        lim -= 64 * half;
+                        float s0[32], s1[32];
+                        tmem_ld32(ts + 64 * half, s0);
+                        tmem_ld32(ts + 64 * half + 32, s1);
+                        tmem_ld_wait();
+                        tmem_regs_ready(s0);
+                        tmem_regs_ready(s1);
+                        if (__any_sync(0xffffffffu, lim < 64)) {
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (32 * c + e >= lim) x[e] = -INFINITY;
+                            for (int e = 0; e < 32; e++) {
+                                if (e >= lim) s0[e] = -INFINITY;
+                                if (32 + e >= lim) s1[e] = -INFINITY;
+                            }
                         }
+                        float t0 = s0[0], t1 = s0[1], t2 = s1[0], t3 = s1[1];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(x[e], x[e + 1]));
-                    };
-                    mask_and_max(s0, 0);
-                    tmem_ld32(ts + 96, s3);
-                    mask_and_max(s1, 1);
-                    tmem_ld_wait();
-                    tmem_regs_ready(s2);
-                    tmem_regs_ready(s3);
-                    if (nk > 64) {
-                        mask_and_max(s2, 2);
-                        mask_and_max(s3, 3);
+                        for (int e = 2; e < 32; e += 2) {
+                            t0 = fmaxf(t0, s0[e]), t1 = fmaxf(t1, s0[e + 1]);
+                            t2 = fmaxf(t2, s1[e]), t3 = fmaxf(t3, s1[e + 1]);
+                        }
+                        const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2;
+                        // The reference maximum moves, and O is rescaled, only when a score is
+                        // more than 2^8 above it: weights up to 256 are as exact, and fit f16
+                        if (pa_meet_any(quarter, i == 0 || top > m_ref + 8.f)) {
+                            *mine = top;
+                            pa_meet(quarter);
+                            const float m_new = fmaxf(m_ref, fmaxf(top, *other));
+                            const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
+                            if (i) {
+                                wait(pv_done, (it - 1) & 1);
+                                __syncwarp();
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < HD / 16; c++) {
+                                    float o[8];
+                                    tmem_ld8(to + 8 * c, o);
+                                    tmem_ld_wait();
+                                    tmem_regs_ready(o);
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) o[e] *= f;
+                                    tmem_st8(to + 8 * c, o);
+                                }
+                            }
+                            l.x *= f, l.y *= f;
+                            m_ref = m_new;
+                        }
+                        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+                        const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
+                        // P as pairs in columns 32 half .. + 31, what it lost 64 columns on
+                        auto weights = [&](const float (&x)[32], int c) {
+                            uint32_t hi[16], lo[16];
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
+                                const float2 p = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                                l = fadd2(l, p);
+                                float r0, r1;
+                                hi[e] = pa_pack<T>(p.x, p.y, r0, r1);
+                                if constexpr (kTwoPlanes) {
+                                    float u0, u1;
+                                    lo[e] = pa_pack<T>(r0, r1, u0, u1);
+                                }
+                            }
+                            tmem_st16(ts + 32 * half + 16 * c, hi);
+                            if constexpr (kTwoPlanes) tmem_st16(ts + 64 + 32 * half + 16 * c, lo);
+                        };
+                        if (nk > 64 * half) weights(s0, 0);  // the products stop at nk
+                        if (nk > 64 * half + 32) weights(s1, 1);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
                     }
-                    const float m_new = fmaxf(m_ref, top * a.scale_log2);
-                    // O is rescaled only when the maximum has grown by more than 2^8 since
-                    // the last time: weights up to 256 are as exact, and fit f16
-                    if (i == 0) {
-                        m_ref = m_new;
-                    } else if (__any_sync(0xffffffffu, m_new > m_ref + 8.f)) {
-                        const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
+                    if (lane == 0) mbar_arrive(p_ready);
+                }
+                if (busy) {
+                    mine[2 * kPaRows] = l.x + l.y;
+                    pa_meet(quarter);
+                    const float sum = l.x + l.y + other[2 * kPaRows];
+                    const bool real = row < j.count * a.group;
+                    const int tok = j.first + pa_token(a, row), gq = j.first * a.group + row;
+                    if (n) {
                         wait(pv_done, (it - 1) & 1);
                         __syncwarp();
                         tc_fence_after();
+                    }
+                    if (a.direct) {
+                        const bool none = n == 0 || sum == 0.f;  // no visible key: 0
+                        const float f = none ? 0.f : 1.f / sum;
+                        TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo +
+                                  (size_t)(j.hk * a.group + gq - tok * a.group) * HD + half * (HD / 2);
 #pragma unroll 1
-                        for (int c = 0; c < HD / 8; c++) {
-                            float o[8];
-                            tmem_ld8(to + 8 * c, o);
+                        for (int c = 0; c < HD / 2; c += 16, out += 16) {
+                            float o[16];
+                            tmem_ld16(to + c, o);  // without a tile whatever is there, and not used
                             tmem_ld_wait();
                             tmem_regs_ready(o);
+                            if (real) {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) o[e] *= f;
-                            tmem_st8(to + 8 * c, o);
-                        }
-                        tmem_st_wait();
-                        l.x *= f, l.y *= f;
-                        m_ref = m_new;
-                    }
-                    const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-                    const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
-                    // P over S: quarter c goes to columns 16 c (and 64 + 16 c), which hold
-                    // quarters that have been read
-                    auto weights = [&](const float (&x)[32], int c) {
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
-                            const float2 w = make_float2(exp2_fast(t.x), exp2_fast(t.y));
-                            l = fadd2(l, w);
-                            float r0, r1;
-                            hi[e] = pa_pack<T>(w.x, w.y, r0, r1);
-                            if constexpr (kTwoPlanes) {
-                                float u0, u1;
-                                lo[e] = pa_pack<T>(r0, r1, u0, u1);
+                                for (int e = 0; e < 16; e++) o[e] = none ? 0.f : o[e] * f;
+                                pa_store16(out, o);
                             }
+                            __syncwarp();
                         }
-                        tmem_st16(ts + 16 * c, hi);
-                        if constexpr (kTwoPlanes) tmem_st16(ts + 64 + 16 * c, lo);
-                    };
-                    if (nk > 96) weights(s3, 3);
-                    tmem_ld32(ts, s0);
-                    if (nk > 64) weights(s2, 2);
-                    tmem_ld_wait();
-                    tmem_regs_ready(s0);
-                    if (!all) {
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (e >= lim) s0[e] = -INFINITY;
-                    }
-                    if (nk > 32) weights(s1, 1);
-                    weights(s0, 0);
-                    tmem_st_wait();
-                }
-                tc_fence_before();
-                mbar_arrive(p_ready);
-            }
-            if (n) {
-                wait(pv_done, (it - 1) & 1);
-                __syncwarp();
-                tc_fence_after();
-            }
-            if (busy) {
-                const float sum = l.x + l.y;
-                const size_t blk = (size_t)(item.split * a.n_kv + item.hk) * a.row_blocks;
-                if (real && !a.direct) a.ml_part[blk * 32 + gq] = make_float2(m_ref, sum);
-                float *part = a.o_part + (blk + (gq >> 5)) * (32 * HD) + (gq & 31) * 4;
-                const float f = a.direct ? 1.f / sum : 1.f;
-                float o[32];
+                    } else {
+                        const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks;
+                        if (real && half == 0) a.ml_part[blk * 32 + gq] = make_float2(m_ref, sum);
+                        float *part = a.o_part + (blk + (gq >> 5)) * (32 * HD) + (gq & 31) * 4 + half * (HD * 16);
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    if (n) {
-                        tmem_ld32(to + 32 * c, o);
-                        tmem_ld_wait();
-                        tmem_regs_ready(o);
-                    }
-                    if (real && (a.direct || n)) {
-                        const bool none = !n || sum == 0.f;  // no visible key: 0
+                        for (int c = 0; c < HD / 2 && n; c += 32, part += 32 * 32) {
+                            float o[32];
+                            tmem_ld32(to + c, o);
+                            tmem_ld_wait();
+                            tmem_regs_ready(o);
+                            if (real) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                  : make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
-                            if (a.direct)
-                                pa_store4(static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)head * HD + 32 * c + e,
-                                          v);
-                            else
-                                pa_store4(part + (32 * c + e) * 32, v);
+                                for (int e = 0; e < 32; e += 4)
+                                    pa_store4(part + e * 32, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                            }
+                            __syncwarp();
                         }
                     }
-                    __syncwarp();
+                    tc_fence_before();  // O has been read before the next job's products overwrite it
                 }
             }
-            tc_fence_before();  // O has been read before the next job's products overwrite it
-        }
+            jobs.release(lane);
         }
     }
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kPaMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tbase), "r"(kPaTmemCols)
                      : "memory");
@@ -705,7 +820,7 @@ int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[5
     auto kernel = prefix_attn_kernel<T, TO, HD>;
     if (items) {
         if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
-        kernel<<<std::min(items, 2 * ctx->num_sms), kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(
+        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(
             tm[0], tm[1], tm[2], tm[3], tm[4], a);
     }
     if (!a.direct) {
@@ -746,8 +861,9 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
                "lc_prefix_attn: n_q_heads %u must be a multiple of n_kv_heads %u", n_q_heads, n_kv_heads);
     LC_REQUIRE(n_q_heads / n_kv_heads <= (uint32_t)kPaRows, LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: %u query heads to a KV head (at most %d)", n_q_heads / n_kv_heads, kPaRows);
-    LC_REQUIRE(scale >= 0.f && scale < INFINITY, LC_ERR_INVALID,
-               "lc_prefix_attn: scale %g must be finite and not negative", scale);
+    const float scale_log2 = scale * 1.44269504088896340736f;
+    LC_REQUIRE(scale >= FLT_MIN && scale_log2 < INFINITY, LC_ERR_INVALID,
+               "lc_prefix_attn: scale %g must be a positive normal number", scale);
     if (rows == 0 || n_q_heads == 0) return LC_OK;
     LC_REQUIRE(kv, LC_ERR_INVALID, "lc_prefix_attn: null kv");
     if (kv->n_seqs == 0) return LC_OK;
@@ -790,13 +906,12 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     a.prefix_len = (int)kv->prefix_len, a.own_cap = (int)kv->own_cap, a.n_seqs = (int)kv->n_seqs;
     a.own_len = kv->own_cap ? kv->own_len : nullptr, a.seq_start = kv->seq_start;
     a.group_inv = (65536 + a.group - 1) / a.group;
-    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.scale_log2 = scale_log2;
     a.causal = causal != 0;
     a.status = ctx->dev_status;
     pa_plan(a, ctx->num_sms);
     const int64_t items = (int64_t)a.prefix_items + (int64_t)a.n_kv * a.n_seqs * a.seq_lanes * a.seq_splits;
     LC_REQUIRE(items <= 0x7FFFFFFF, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
-    a.items = (int)items;
     if (!a.direct) {
         a.row_blocks = div_up((int64_t)rows * a.group, 32);
         const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;

@@ -24,7 +24,7 @@ def call(kv=None, **over):
 @pytest.mark.parametrize("over", [
     dict(q=None), dict(out=None), dict(kv=False), dict(kv=dict(k_prefix=None)), dict(kv=dict(v_prefix=None)),
     dict(kv=dict(k_own=None)), dict(kv=dict(v_own=None)), dict(kv=dict(own_len=None)), dict(kv=dict(seq_start=None)),
-    dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(ldq=511), dict(ldq=516),
+    dict(scale=-1.0), dict(scale=0.0), dict(scale=1e-39), dict(scale=3e38), dict(scale=float("nan")), dict(scale=float("inf")), dict(ldq=511), dict(ldq=516),
     dict(ldo=500), dict(ldo=516), dict(kv=dict(ld_prefix=120)), dict(kv=dict(ld_prefix=132)),
     dict(kv=dict(ld_own=120)), dict(kv=dict(ld_own=132)), dict(kv=dict(own_stride=49 * 128 + 120)),
     dict(kv=dict(own_stride=50 * 128 + 4)), dict(kv=dict(k_prefix=0x300008)), dict(kv=dict(v_own=0x600002)),
