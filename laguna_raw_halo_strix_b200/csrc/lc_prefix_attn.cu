@@ -333,6 +333,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// 2^x of two numbers on the FMA pipes, which the special function unit (16 results
+// a cycle and SM, the limit of a tile's weights) leaves idle: x = n + f with n
+// the nearest integer, read off the low mantissa bits after adding 1.5 * 2^23;
+// 2^f by a polynomial of degree N (least squares of the relative error over
+// [-1/2, 1/2]: off by 7.5e-5 for N = 3, 2.6e-6 for N = 4, against half a step of
+// 2e-3 for bf16 and 2.4e-4 for f16 weights); n added to the exponent.  Below
+// -126 the result stays at 2^-126.
+template <int N>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    constexpr float c[2][5] = {{0.99992806f, 0.69326097f, 0.24261113f, 0.05517167f, 0.f},
+                               {0.99999928f, 0.69312179f, 0.24024744f, 0.05591786f, 0.0095701f}};
+    constexpr float kMagic = 12582912.f;
+    const float2 m = make_float2(kMagic, kMagic), mm = make_float2(-kMagic, -kMagic);
+    x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
+    const float2 r = fadd2(x, m), n = fadd2(r, mm), f = ffma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = make_float2(c[N - 3][N], c[N - 3][N]);
+#pragma unroll
+    for (int i = N - 1; i >= 0; i--) p = ffma2(p, f, make_float2(c[N - 3][i], c[N - 3][i]));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+
 // (a, b) as a pair of T, and what that lost.
 template <class T>
 __device__ __forceinline__ uint32_t pa_pack(float a, float b, float &la, float &lb);
@@ -493,13 +515,13 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     if (!wait.ok) break;
                     __syncwarp();
                     tc_fence_after();
+                    // unrolled: a product runs 64 cycles, and a loop around one takes 88 to issue it
                     if (lane == 0) {
-                        uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
-#pragma unroll 1
+                        const uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
+#pragma unroll
                         for (int s = 0; s < HD / 16; s++) {
-                            umma_f16_ss(tbase + kPaColS, qd, kd, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
-                            const uint64_t step = ((s & 3) == 3 ? kPaPlane - 96 : 32) >> 4;
-                            qd += step, kd += step;
+                            const uint64_t o = ((s >> 2) * kPaPlane + (s & 3) * 32) >> 4;
+                            umma_f16_ss(tbase + kPaColS, qd + o, kd + o, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
                         }
                         umma_commit(s_full);
                     }
@@ -523,13 +545,20 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     __syncwarp();
                     tc_fence_after();
                     if (lane == 0) {
-                        uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
-                        uint32_t p = tbase + kPaColS;
-                        constexpr uint32_t id = pa_idesc<T>(HD, true);
+                        const uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
+                        auto step = [&](int s) {
+                            const uint32_t p = tbase + kPaColS + (s >> 2) * 64 + (s & 3) * 8;
+                            const uint64_t v = vd + ((s * 2048) >> 4);
+                            umma_f16_ts(tbase + kPaColO, p, v, pa_idesc<T>(HD, true), (i | s) ? 1u : 0u);
+                            if constexpr (kTwoPlanes)
+                                umma_f16_ts(tbase + kPaColO, p + 32, v, pa_idesc<T>(HD, true), 1u);
+                        };
+                        if (steps == 8) {
+#pragma unroll
+                            for (int s = 0; s < 8; s++) step(s);
+                        } else {
 #pragma unroll 1
-                        for (int s = 0; s < steps; s++, vd += 2048 >> 4, p += 8) {
-                            umma_f16_ts(tbase + kPaColO, p, vd, id, (i | s) ? 1u : 0u);
-                            if constexpr (kTwoPlanes) umma_f16_ts(tbase + kPaColO, p + 64, vd, id, 1u);
+                            for (int s = 0; s < steps; s++) step(s);
                         }
                         umma_commit(pv_done);
                     }
@@ -543,7 +572,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         // Row = TMEM lane; the two warps of a lane quarter take 64 keys of a tile, and half
         // of O's columns, each (64 scores in registers; one warp per quarter and 128 keys
         // left the chain of a tile 1.6x as long).  Thread pairs meet at a barrier of their
-        // two warps: `meet` also says that both have read S, which P overwrites.
+        // two warps to agree on a row's maximum.
         const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
         const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO + half * (HD / 2);
@@ -579,7 +608,8 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         tmem_ld_wait();
                         tmem_regs_ready(s0);
                         tmem_regs_ready(s1);
-                        if (__any_sync(0xffffffffu, lim < 64)) {
+                        const bool part = __any_sync(0xffffffffu, lim < 64);
+                        if (part) {
 #pragma unroll
                             for (int e = 0; e < 32; e++) {
                                 if (e >= lim) s0[e] = -INFINITY;
@@ -620,13 +650,17 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         }
                         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
                         const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
-                        // P as pairs in columns 32 half .. + 31, what it lost 64 columns on
-                        auto weights = [&](const float (&x)[32], int c) {
-                            uint32_t hi[16], lo[16];
+                        // P as pairs over the first half of the warp's own scores, what the rounding
+                        // lost over the second
+                        auto weights = [&](const float (&x)[32], int c, auto by_polynomial) {
+                            uint32_t hi[16];
+                            [[maybe_unused]] uint32_t lo[16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
                                 const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
-                                const float2 p = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                                const float2 p = decltype(by_polynomial)::value && e % 4 == 3
+                                                     ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(t)
+                                                     : make_float2(exp2_fast(t.x), exp2_fast(t.y));
                                 l = fadd2(l, p);
                                 float r0, r1;
                                 hi[e] = pa_pack<T>(p.x, p.y, r0, r1);
@@ -635,11 +669,16 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                                     lo[e] = pa_pack<T>(r0, r1, u0, u1);
                                 }
                             }
-                            tmem_st16(ts + 32 * half + 16 * c, hi);
-                            if constexpr (kTwoPlanes) tmem_st16(ts + 64 + 32 * half + 16 * c, lo);
+                            tmem_st16(ts + 64 * half + 16 * c, hi);
+                            if constexpr (kTwoPlanes) tmem_st16(ts + 64 * half + 32 + 16 * c, lo);
                         };
-                        if (nk > 64 * half) weights(s0, 0);  // the products stop at nk
-                        if (nk > 64 * half + 32) weights(s1, 1);
+                        if (kTwoPlanes || part) {
+                            if (nk > 64 * half) weights(s0, 0, std::false_type());  // the products stop at nk
+                            if (nk > 64 * half + 32) weights(s1, 1, std::false_type());
+                        } else {
+                            weights(s0, 0, std::true_type());
+                            weights(s1, 1, std::true_type());
+                        }
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
