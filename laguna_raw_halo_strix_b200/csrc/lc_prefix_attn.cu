@@ -64,8 +64,12 @@ struct PaArgs {
     // sequences, the rest rows of one sequence over [seq_from, end) of the
     // virtual axis
     int prefix_items, row_tiles, prefix_keys;
+    int chunk, chunk_pairs;  // prefix and sequence items alternate in chunks, chunk_pairs times
     int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
-    int direct;         // one split covers everything: items write out
+    int seq_base;  // n_kv * n_seqs * seq_lanes
+    // The first `direct` sequence items run over the whole axis and write out (their
+    // rows' first state says so: l = -1); merge: the others leave states
+    int direct, merge;
     // partial states of row r = token * group + head within the group: O
     // unnormalised as [split][KV head][r / 32][HD / 4][r % 32][4] (32 rows' 16-byte
     // pieces side by side: the lanes of a warp hold neighbouring rows), and (m in
@@ -76,11 +80,18 @@ struct PaArgs {
     unsigned *status;
 };
 
+// K/V copies: [a whole tile or kPaBoxRows of its rows][prefix or own][K or V], as
+// [sequence][row][element] (one sequence for the prefix); Q as [token][head][element].
+struct PaMaps {
+    CUtensorMap kv[2][2][2], q;
+};
+
 // Tokens first .. first + count - 1 (rows r = token within the tile * group +
 // head within the group) of one KV head against prefix keys [p0, p1) and keys
 // [o0, o1) of sequence seq.
 struct PaJob {
     int n;  // tiles; -1: no more jobs
+    int direct;
     int first, count, p0, p1, o0, o1, seq, hk, split;
     int pos0;  // own position of token t is pos0 + t
     __device__ __forceinline__ int prefix_tiles() const { return (p1 - p0 + kPaKeys - 1) / kPaKeys; }
@@ -97,39 +108,66 @@ struct PaJob {
 __device__ __forceinline__ int pa_token(const PaArgs &a, int r) { return (int)((uint32_t)r * a.group_inv >> 16); }
 
 struct PaItem {
-    int hk, split, t, t_step;  // token tiles at t, t + t_step, .. below count
+    int direct, hk, split, t, t_step;  // token tiles at t, t + t_step, .. below count
     int start, count, len, seq, v0, v1;
 };
 
-__device__ __forceinline__ PaItem pa_item(const PaArgs &a, int i) {
+// Item i in two steps: the first ends in loads whose values only the second looks
+// at, so that they can be under way while the last item's copies are waited for.
+__device__ __forceinline__ PaItem pa_item_begin(const PaArgs &a, int i) {
     PaItem t;
-    if (i < a.prefix_items) {
-        t.hk = i % a.n_kv;
-        i /= a.n_kv;
+    // prefix and sequence items in turn, a chunk of each, while there are both
+    bool prefix;
+    const int q = i / a.chunk;
+    if (q < 2 * a.chunk_pairs) {
+        prefix = !(q & 1);
+        i -= (q + 1) / 2 * a.chunk;
+    } else {
+        i -= a.chunk_pairs * a.chunk;
+        prefix = i < a.prefix_items;
+        if (!prefix) i -= a.prefix_items - a.chunk_pairs * a.chunk;
+    }
+    // sequence items: the direct ones, then the splits of the rest
+    t.direct = !prefix && i < a.direct;
+    int sp = 0;
+    if (!prefix && !t.direct) {
+        const int rest = a.seq_base - a.direct;
+        sp = (i - a.direct) / rest;
+        i -= sp * rest;
+    }
+    t.hk = i % a.n_kv;
+    i /= a.n_kv;
+    if (prefix) {
         t.t = i % a.row_tiles * a.tile_toks;
         t.split = i / a.row_tiles;
+        t.seq = -1;
+        t.start = 0, t.count = a.rows, t.len = 0;
+    } else {
+        t.seq = i % a.n_seqs;
+        i /= a.n_seqs;
+        t.t = i * a.tile_toks;
+        t.split = a.prefix_splits + sp;
+        t.start = a.seq_start[t.seq];
+        t.count = a.seq_start[t.seq + 1];
+        t.len = a.own_len ? a.own_len[t.seq] : 0;
+    }
+    return t;
+}
+__device__ __forceinline__ void pa_item_finish(const PaArgs &a, PaItem &t) {
+    if (t.seq < 0) {
         t.t_step = 1 << 30;
-        t.start = 0, t.count = a.rows, t.len = 0, t.seq = 0;
         t.v0 = t.split * a.prefix_keys;
         t.v1 = min(a.prefix_len, t.v0 + a.prefix_keys);
     } else {
-        i -= a.prefix_items;
-        t.hk = i % a.n_kv;
-        i /= a.n_kv;
-        t.seq = i % a.n_seqs;
-        i /= a.n_seqs;
-        t.t = i % a.seq_lanes * a.tile_toks;
-        const int sp = i / a.seq_lanes;
-        t.split = a.prefix_splits + sp;
         t.t_step = a.seq_lanes * a.tile_toks;
         // values from the device are held inside the arrays
-        t.start = min(max(a.seq_start[t.seq], 0), a.rows);
-        t.count = min(max(a.seq_start[t.seq + 1], t.start), a.rows) - t.start;
-        t.len = a.own_len ? min(max(a.own_len[t.seq], 0), a.own_cap) : 0;
-        t.v0 = a.seq_from + sp * a.seq_keys;
-        t.v1 = min(a.prefix_len + a.own_cap, t.v0 + a.seq_keys);
+        t.start = min(max(t.start, 0), a.rows);
+        t.count = min(max(t.count, t.start), a.rows) - t.start;
+        t.len = min(max(t.len, 0), a.own_cap);
+        t.v0 = a.seq_from + (t.split - a.prefix_splits) * a.seq_keys;
+        t.v1 = a.prefix_len + a.own_cap;
+        if (!t.direct) t.v1 = min(t.v1, t.v0 + a.seq_keys);
     }
-    return t;
 }
 
 __device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int at) {
@@ -143,7 +181,7 @@ __device__ __forceinline__ PaJob pa_job(const PaArgs &a, const PaItem &t, int at
     if (a.causal) j.o1 = min(j.o1, j.pos0 + j.first + j.count);  // the last token's reach
     j.o1 = max(j.o1, j.o0);
     j.n = j.prefix_tiles() + (j.o1 - j.o0 + kPaKeys - 1) / kPaKeys;
-    j.seq = t.seq, j.hk = t.hk, j.split = t.split;
+    j.seq = t.seq, j.hk = t.hk, j.split = t.split, j.direct = t.direct;
     return j;
 }
 
@@ -252,13 +290,6 @@ struct PaJobs {
     }
 };
 
-__device__ __forceinline__ void tma_load_2d_plain(void *dst, const CUtensorMap *tm, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];\n" ::"r"(smem_addr(dst)),
-        "l"(tm), "r"(x), "r"(y), "r"(smem_addr(bar))
-        : "memory");
-}
 __device__ __forceinline__ void tma_load_3d_plain(void *dst, const CUtensorMap *tm, int x, int y, int z,
                                                   uint64_t *bar) {
     asm volatile(
@@ -399,10 +430,7 @@ __device__ __forceinline__ void pa_store16(T *p, const float (&v)[16]) {
 
 template <class T, class TO, int HD>
 __global__ void __launch_bounds__(kPaThreads, 2)
-    prefix_attn_kernel(const __grid_constant__ CUtensorMap kp, const __grid_constant__ CUtensorMap vp,
-                       const __grid_constant__ CUtensorMap ko, const __grid_constant__ CUtensorMap vo,
-                       const __grid_constant__ CUtensorMap qm,
-                       const __grid_constant__ PaArgs a) {
+    prefix_attn_kernel(const __grid_constant__ PaMaps maps, const __grid_constant__ PaArgs a) {
     using L = PaSmem<HD>;
     constexpr bool kTwoPlanes = std::is_same<TO, float>::value;  // P as hi + lo
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -415,6 +443,11 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     PaJobs jobs{reinterpret_cast<PaJob *>(smem + L::kJobs), bar + 5};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    PaItem next;
+    if (threadIdx.x == 32 * kPaLoadWarp) {
+        next = pa_item_begin(a, blockIdx.x);
+        prefetch_tensormap(&maps.q);
+    }
     griddep_launch_dependents();  // the merge kernel may be scheduled once the last items run
     if (threadIdx.x == 0) {
         mbar_init(k_full, 1);
@@ -443,23 +476,32 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     uint32_t it = 0;  // tiles so far: every barrier completes once per tile
 
     if (warp == kPaLoadWarp) {  // ---- loads
+        // (kept short: the thread has about 1500 cycles a tile beside its waits)
         if (lane == 0) {
+            while (true) {
+                pa_item_finish(a, next);
+                bool asked = false;
 #pragma unroll 1
-            for (int w = blockIdx.x; w >= 0; w = sched.next(wait)) {
-                sched.ask();
-                const PaItem item = pa_item(a, w);
-#pragma unroll 1
-                for (int at = item.t; at < item.count && wait.ok; at += item.t_step) {
-                    const PaJob j = pa_job(a, item, at);
+                for (int at = next.t; at < next.count && wait.ok; at += next.t_step) {
+                    const PaJob j = pa_job(a, next, at);
+                    if (j.n == 0 && !j.direct && j.count * a.group <= 32) {  // nothing visible: the states here
+                        const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks;
+                        for (int r = 0; r < j.count * a.group; r++)
+                            a.ml_part[blk * 32 + j.first * a.group + r] = make_float2(-INFINITY, 0.f);
+                        continue;
+                    }
                     jobs.put(wait, j);
 #pragma unroll 1
                     for (int i = 0; i < j.n && wait.ok; i++, it++) {
+                        // The next item is asked for two tiles before this one's end (not sooner: an
+                        // item taken early would wait behind this one while other CTAs run dry).
+                        if (!asked && i >= j.n - 2 && at + next.t_step >= next.count) sched.ask(), asked = true;
                         int key, nk;
                         bool own;
                         j.tile(i, key, nk, own);
-                        const int boxes = (nk + kPaBoxRows - 1) / kPaBoxRows;
-                        const uint32_t bytes = boxes * kPaBoxRows * HD * 2;
-                        const int x = item.hk * HD;
+                        const bool full = nk == kPaKeys;
+                        const int copies = full ? 1 : (nk + kPaBoxRows - 1) / kPaBoxRows;
+                        const uint32_t bytes = (full ? kPaKeys : copies * kPaBoxRows) * HD * 2;
 #pragma unroll 1
                         for (int kv = 0; kv < 2; kv++) {
                             // the slot is free once the products that read it are done (Q: those
@@ -467,29 +509,33 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             if (it) wait(kv ? pv_done : s_full, (it - 1) & 1);
                             if (!wait.ok) break;
                             uint64_t *b = kv ? v_full : k_full;
-                            const int qb = i == 0 && kv == 0 ? (j.count + a.box_toks - 1) / a.box_toks : 0;
-                            const int q_rows = a.box_toks * a.group;
-                            mbar_expect_tx(b, bytes + (uint32_t)(qb * q_rows * HD * 2));
-#pragma unroll 1
-                            for (int c = 0; c < HD / 64; c++) {
+                            if (i == 0 && kv == 0) {
+                                const int qb = (j.count + a.box_toks - 1) / a.box_toks, q_rows = a.box_toks * a.group;
+                                mbar_expect_tx(b, bytes + (uint32_t)(qb * q_rows * HD * 2));
 #pragma unroll 1
                                 for (int r = 0; r < qb; r++)
-                                    tma_load_3d_plain(smem + L::kQ + c * kPaPlane + r * q_rows * 128, &qm, 64 * c,
-                                                      item.hk * a.group, j.first + r * a.box_toks, b);
-                                unsigned char *dst = smem + (kv ? L::kV : L::kK) + c * kPaPlane;
-#pragma unroll 1
-                                for (int r = 0; r < boxes; r++) {
-                                    const int y = key + kPaBoxRows * r;
-                                    unsigned char *d = dst + r * (kPaBoxRows * 128);
-                                    if (own)
-                                        tma_load_3d_plain(d, kv ? &vo : &ko, x + 64 * c, y, j.seq, b);
-                                    else
-                                        tma_load_2d_plain(d, kv ? &vp : &kp, x + 64 * c, y, b);
-                                }
+#pragma unroll
+                                    for (int c = 0; c < HD / 64; c++)
+                                        tma_load_3d_plain(smem + L::kQ + c * kPaPlane + r * q_rows * 128, &maps.q, 64 * c,
+                                                          j.hk * a.group, j.first + r * a.box_toks, b);
+                            } else {
+                                mbar_expect_tx(b, bytes);
                             }
+                            const CUtensorMap *m = &maps.kv[full][own][kv];
+                            unsigned char *dst = smem + (kv ? L::kV : L::kK);
+#pragma unroll 1
+                            for (int r = 0; r < copies; r++, dst += kPaBoxRows * 128)
+#pragma unroll
+                                for (int c = 0; c < HD / 64; c++)
+                                    tma_load_3d_plain(dst + c * kPaPlane, m, j.hk * HD + 64 * c, key + kPaBoxRows * r,
+                                                      own ? j.seq : 0, b);
                         }
                     }
                 }
+                if (!asked) sched.ask();
+                const int w = sched.next(wait);
+                if (w < 0) break;
+                next = pa_item_begin(a, w);
             }
             PaJob last = {};
             last.n = -1;
@@ -696,7 +742,9 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         __syncwarp();
                         tc_fence_after();
                     }
-                    if (a.direct) {
+                    const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks;
+                    if (j.direct) {
+                        if (real && half == 0 && a.merge) a.ml_part[blk * 32 + gq] = make_float2(0.f, -1.f);
                         const bool none = n == 0 || sum == 0.f;  // no visible key: 0
                         const float f = none ? 0.f : 1.f / sum;
                         TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo +
@@ -715,7 +763,6 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             __syncwarp();
                         }
                     } else {
-                        const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks;
                         if (real && half == 0) a.ml_part[blk * 32 + gq] = make_float2(m_ref, sum);
                         float *part = a.o_part + (blk + (gq >> 5)) * (32 * HD) + (gq & 31) * 4 + half * (HD * 16);
 #pragma unroll 1
@@ -758,35 +805,50 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
     const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int piece = w % kPer, blk = w / kPer % a.row_blocks, hk = w / kPer / a.row_blocks;
     const int gq = blk * 32 + lane, tok = gq / a.group;
-    if (hk >= a.n_kv || gq >= a.rows * a.group || tok < a.seq_start[0] || tok >= a.seq_start[a.n_seqs]) return;
+    if (hk >= a.n_kv || gq >= a.rows * a.group) return;
+    const int first = a.seq_start[0], last = a.seq_start[a.n_seqs];  // (looked at below, with the states)
     const int splits = a.prefix_splits + a.seq_splits;
     const size_t stride = (size_t)a.n_kv * a.row_blocks;  // blocks of a split
     const size_t at = (size_t)hk * a.row_blocks + blk;
     const float2 *ml = a.ml_part + at * 32 + lane;
     const float4 *op = reinterpret_cast<const float4 *>(a.o_part + at * (32 * HD)) + piece * 64 + lane;
-    float M = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < splits; s++) M = fmaxf(M, ml[s * stride * 32].x);
-    float sum = 0.f, o[8] = {};
+    // a batch's (m, l) and pieces in one round trip; the sums move to its maximum
+    float M = -INFINITY, sum = 0.f, o[8] = {};
+#pragma unroll 1
     for (int s0 = 0; s0 < splits; s0 += kBatch) {
         float2 st[kBatch];
         float4 x[kBatch][2];
 #pragma unroll
-        for (int u = 0; u < kBatch; u++)
-            if (s0 + u < splits) {
-                st[u] = ml[(s0 + u) * stride * 32];
-                x[u][0] = op[(s0 + u) * stride * (8 * HD)];
-                x[u][1] = op[(s0 + u) * stride * (8 * HD) + 32];
-            }
+        for (int u = 0; u < kBatch; u++) {
+            const size_t s = min(s0 + u, splits - 1);
+            st[u] = ml[s * stride * 32];
+            x[u][0] = op[s * stride * (8 * HD)];
+            x[u][1] = op[s * stride * (8 * HD) + 32];
+        }
+        if (s0 == 0 && (st[0].y < 0.f || tok < first || tok >= last)) return;  // written already, or of no sequence
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            if (s0 + u >= splits) st[u].y = 0.f;
+            if (st[u].y != 0.f) top = fmaxf(top, st[u].x);
+        }
+        if (top > M) {
+            const float f = exp2f(M - top);
+            sum *= f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] *= f;
+            M = top;
+        }
 #pragma unroll
         for (int u = 0; u < kBatch; u++)
-            if (s0 + u < splits && st[u].y != 0.f) {  // O of a state that saw no key may be unwritten
+            if (st[u].y != 0.f) {  // O of a state that saw no key may be unwritten
                 const float f = exp2f(st[u].x - M);
                 sum += st[u].y * f;
                 o[0] += x[u][0].x * f, o[1] += x[u][0].y * f, o[2] += x[u][0].z * f, o[3] += x[u][0].w * f;
                 o[4] += x[u][1].x * f, o[5] += x[u][1].y * f, o[6] += x[u][1].z * f, o[7] += x[u][1].w * f;
             }
     }
+    if (splits == 0 && (tok < first || tok >= last)) return;
     const float f = sum != 0.f ? 1.f / sum : 0.f;
     TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)(hk * a.group + gq - tok * a.group) * HD + 8 * piece;
     pa_store4(out, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
@@ -796,14 +858,14 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
 // A tensor of dims[0] contiguous elements and strides ld[] (elements) of the
 // outer dims, copied in boxes of 64 elements x box1 (x box2) in the 128-byte
 // swizzle; what lies past an end reads as zero.
-int pa_map(CUtensorMap *tm, const void *p, int dtype, int nd, const uint64_t (&dims)[3], const uint64_t (&ld)[2],
+int pa_map(CUtensorMap *tm, const void *p, int dtype, const uint64_t (&dims)[3], const uint64_t (&ld)[2],
            uint32_t box1, uint32_t box2) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
     if (int s = lc_tensor_map_encoder(&enc)) return s;
     cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, strides[2] = {ld[0] * 2, ld[1] * 2};
     cuuint32_t box[3] = {64, box1, box2}, es[3] = {1, 1, 1};
     const CUresult r =
-        enc(tm, dtype == LC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, nd,
+        enc(tm, dtype == LC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
             const_cast<void *>(p), d, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LC_REQUIRE(r == CUDA_SUCCESS, LC_ERR_CUDA, "lc_prefix_attn: cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -813,7 +875,7 @@ int pa_map(CUtensorMap *tm, const void *p, int dtype, int nd, const uint64_t (&d
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How the work is cut into items.
-void pa_plan(PaArgs &a, int num_sms) {
+void pa_plan(PaArgs &a, int num_sms, int hd) {
     const int slots = 2 * num_sms;  // CTAs resident at once
     const int64_t R = (int64_t)a.rows * a.group;
     // Tokens of a row tile: as many as fit 128 rows in whole copies of Q, which hold
@@ -827,42 +889,80 @@ void pa_plan(PaArgs &a, int num_sms) {
         a.box_toks = unit * std::max(1, 32 / (unit * a.group));
         a.tile_toks = kPaRows / (a.box_toks * a.group) * a.box_toks;
     }
-    const int per_seq = div_up(div_up(a.rows, a.n_seqs), a.tile_toks);  // row tiles of an average sequence
-    a.seq_lanes = std::max(1, per_seq);
+    const int tiles_all = div_up(a.rows, a.tile_toks), tiles_avg = div_up(div_up(a.rows, a.n_seqs), a.tile_toks);
+    // row tiles of a sequence that run side by side (a longer one goes round again)
+    a.seq_lanes = a.n_seqs == 1 ? tiles_all : std::min(tiles_all, tiles_avg > 1 ? 2 * tiles_avg : 1);
+    // Splits of the key axis for `base` items of `tiles` tiles: the fewest rounds of tiles
+    // over the resident CTAs (about 2 us a tile), against writing and reading the states
+    // (4 bytes a picosecond) and the merge's launch.
+    const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 4e6;
+    auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
+        int best = 1;
+        double best_us = 1e30;
+        for (int n = 1; n <= std::min(tiles, 128); n++) {
+            const int per = div_up(tiles, n);
+            if (n > 1 && div_up(tiles, n - 1) == per) continue;  // the same cut with an empty split more
+            const double us = 2.0 * per * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
+            if (us < best_us) best = n, best_us = us;
+        }
+        return best;
+    };
     // A sequence whose rows fill tiles by themselves gains nothing from sharing
     // the prefix with others: its items run over [prefix | own] in one go.
     const bool joint = a.prefix_len == 0 || a.n_seqs == 1 || R >= (int64_t)kPaRows * a.n_seqs;
     a.prefix_items = 0, a.prefix_splits = 0, a.row_tiles = 1, a.prefix_keys = kPaKeys;
     a.seq_from = joint ? 0 : a.prefix_len;
     if (!joint) {
-        a.row_tiles = div_up(a.rows, a.tile_toks);
+        a.row_tiles = tiles_all;
         const int base = a.n_kv * a.row_tiles, tiles = div_up(a.prefix_len, kPaKeys);
-        const int per = div_up(tiles, std::min(tiles, std::max(1, slots / base)));
+        const int per = div_up(tiles, splits_for(base, tiles, true));
         a.prefix_keys = per * kPaKeys;
         a.prefix_splits = div_up(tiles, per);
         a.prefix_items = base * a.prefix_splits;
     }
-    const int axis = a.prefix_len + a.own_cap - a.seq_from;
-    const int tiles = div_up(axis, kPaKeys);
-    a.seq_splits = 0, a.seq_keys = kPaKeys;
+    const int tiles = div_up(a.prefix_len + a.own_cap - a.seq_from, kPaKeys);
+    a.seq_base = a.n_kv * a.n_seqs * a.seq_lanes;
+    a.seq_splits = 0, a.seq_keys = kPaKeys, a.direct = 0;
     if (tiles) {
-        const int64_t base = (int64_t)a.n_kv * a.n_seqs * a.seq_lanes;
-        const int per = div_up(tiles, std::min<int64_t>(tiles, std::max<int64_t>(1, slots / base)));
+        int per;
+        const int64_t real = (int64_t)a.n_kv * tiles_all;  // about so many items have rows
+        if (!joint) {
+            // Own parts differ in length: items of at most 4 tiles keep one long sequence from
+            // being the launch's tail, unless there are many sequences to even out.
+            per = div_up(tiles, splits_for(a.seq_base, tiles, true));
+            if (a.seq_base < 16 * slots) per = std::min(per, 4);
+        } else if (real < slots) {
+            per = div_up(tiles, splits_for(real, tiles, false));
+            if (per == tiles) a.direct = a.seq_base;
+        } else {
+            // Whole rounds of the resident CTAs write out directly; what is left over for a
+            // last, thin round is split to fill it.
+            const int rest = (int)(real % slots);
+            per = div_up(tiles, rest ? std::min(tiles, std::max(1, slots / rest)) : 1);
+            a.direct = per == tiles ? a.seq_base : std::min<int64_t>(a.seq_base, real - rest);
+        }
         a.seq_keys = per * kPaKeys;
-        a.seq_splits = div_up(tiles, per);
+        a.seq_splits = a.direct == a.seq_base ? 1 : div_up(tiles, per);
     }
-    a.direct = joint && a.seq_splits == 1;
+    a.merge = a.direct < a.seq_base || !tiles;
+    // Prefix items lean on the tensor cores and sequence items on memory, so they
+    // alternate (a CTA of each per SM), unless those of the prefix are much longer:
+    // then they come first, as the others even out the end.
+    a.chunk = num_sms;
+    a.chunk_pairs = a.prefix_keys > 2 * a.seq_keys
+                        ? 0
+                        : (int)std::min<int64_t>(a.prefix_items, (int64_t)a.seq_base * a.seq_splits) / a.chunk;
 }
 
 template <class T, class TO, int HD>
-int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[5]) {
+int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const PaMaps &maps) {
     auto kernel = prefix_attn_kernel<T, TO, HD>;
     if (items) {
         if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
         kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(
-            tm[0], tm[1], tm[2], tm[3], tm[4], a);
+            maps, a);
     }
-    if (!a.direct) {
+    if (a.merge) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(div_up((int64_t)a.n_kv * a.row_blocks * (HD / 8), 4));
         cfg.blockDim = dim3(128);
@@ -878,10 +978,10 @@ int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const CUtensorMap (&tm)[5
 }
 
 template <class T>
-int pa_types(lc_ctx *ctx, int out_dtype, uint32_t hd, const PaArgs &a, int items, const CUtensorMap (&tm)[5]) {
+int pa_types(lc_ctx *ctx, int out_dtype, uint32_t hd, const PaArgs &a, int items, const PaMaps &maps) {
     if (out_dtype == LC_F32)
-        return hd == 128 ? pa_launch<T, float, 128>(ctx, a, items, tm) : pa_launch<T, float, 64>(ctx, a, items, tm);
-    return hd == 128 ? pa_launch<T, T, 128>(ctx, a, items, tm) : pa_launch<T, T, 64>(ctx, a, items, tm);
+        return hd == 128 ? pa_launch<T, float, 128>(ctx, a, items, maps) : pa_launch<T, float, 64>(ctx, a, items, maps);
+    return hd == 128 ? pa_launch<T, T, 128>(ctx, a, items, maps) : pa_launch<T, T, 64>(ctx, a, items, maps);
 }
 
 }  // namespace
@@ -913,6 +1013,8 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     const uint64_t wq = (uint64_t)n_q_heads * head_dim, wk = (uint64_t)n_kv_heads * head_dim;
     LC_REQUIRE((uint64_t)rows * n_q_heads <= (1u << 29) && wq < (1u << 24), LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: %u rows of %u heads", rows, n_q_heads);
+    LC_REQUIRE((uint64_t)n_kv_heads * (rows + 2ull * kv->n_seqs) <= (1u << 29), LC_ERR_UNSUPPORTED,
+               "lc_prefix_attn: %u sequences of %u KV heads", kv->n_seqs, n_kv_heads);
     LC_REQUIRE((uint64_t)kv->prefix_len + kv->own_cap <= kPaMaxLen, LC_ERR_UNSUPPORTED,
                "lc_prefix_attn: %u + %u keys", kv->prefix_len, kv->own_cap);
     if (!ldq) ldq = wq;
@@ -948,10 +1050,10 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     a.scale_log2 = scale_log2;
     a.causal = causal != 0;
     a.status = ctx->dev_status;
-    pa_plan(a, ctx->num_sms);
-    const int64_t items = (int64_t)a.prefix_items + (int64_t)a.n_kv * a.n_seqs * a.seq_lanes * a.seq_splits;
+    pa_plan(a, ctx->num_sms, (int)head_dim);
+    const int64_t items = a.prefix_items + a.direct + (int64_t)(a.seq_base - a.direct) * a.seq_splits;
     LC_REQUIRE(items <= 0x7FFFFFFF, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
-    if (!a.direct) {
+    if (a.merge) {
         a.row_blocks = div_up((int64_t)rows * a.group, 32);
         const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;
         void *scr = nullptr;
@@ -959,21 +1061,24 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
         a.ml_part = (float2 *)scr;
         a.o_part = (float *)((char *)scr + ((states * 8 + 255) & ~(size_t)255));
     }
-    CUtensorMap tm[5] = {};
-    if (a.prefix_len) {
-        const uint64_t dims[3] = {wk, kv->prefix_len, 1}, ld[2] = {ldp, 0};
-        if (int s = pa_map(&tm[0], kv->k_prefix, dtype, 2, dims, ld, kPaBoxRows, 1)) return s;
-        if (int s = pa_map(&tm[1], kv->v_prefix, dtype, 2, dims, ld, kPaBoxRows, 1)) return s;
+    PaMaps maps = {};
+    for (int full = 0; full < 2; full++) {
+        const uint32_t box = full ? kPaKeys : kPaBoxRows;
+        if (a.prefix_len) {
+            const uint64_t dims[3] = {wk, kv->prefix_len, 1}, ld[2] = {ldp, ldp};
+            if (int s = pa_map(&maps.kv[full][0][0], kv->k_prefix, dtype, dims, ld, box, 1)) return s;
+            if (int s = pa_map(&maps.kv[full][0][1], kv->v_prefix, dtype, dims, ld, box, 1)) return s;
+        }
+        if (a.own_cap) {
+            const uint64_t dims[3] = {wk, kv->own_cap, kv->n_seqs}, ld[2] = {ldw, seq_ld};
+            if (int s = pa_map(&maps.kv[full][1][0], kv->k_own, dtype, dims, ld, box, 1)) return s;
+            if (int s = pa_map(&maps.kv[full][1][1], kv->v_own, dtype, dims, ld, box, 1)) return s;
+        }
     }
-    if (a.own_cap) {
-        const uint64_t dims[3] = {wk, kv->own_cap, kv->n_seqs}, ld[2] = {ldw, seq_ld};
-        if (int s = pa_map(&tm[2], kv->k_own, dtype, 3, dims, ld, kPaBoxRows, 1)) return s;
-        if (int s = pa_map(&tm[3], kv->v_own, dtype, 3, dims, ld, kPaBoxRows, 1)) return s;
-    }
-    {  // Q as [token][head][head_dim]: a box is the heads of a group for box_toks tokens, in row order
+    {  // a box of Q is the heads of a group for box_toks tokens, in row order
         const uint64_t dims[3] = {head_dim, n_q_heads, rows}, ld[2] = {head_dim, ldq};
-        if (int s = pa_map(&tm[4], q, dtype, 3, dims, ld, a.group, a.box_toks)) return s;
+        if (int s = pa_map(&maps.q, q, dtype, dims, ld, a.group, a.box_toks)) return s;
     }
-    return dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, tm)
-                           : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, tm);
+    return dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, maps)
+                           : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, maps);
 }
