@@ -49,6 +49,18 @@ struct PaSmem {
     static constexpr uint32_t kBytes = kRed + 4 * kPaRows * 4 + 1024;  // + slack to 1024-align the base
 };
 
+// Division of numbers below 2^31 by a divisor known at launch, as a product with
+// ceil(2^63 / d).
+struct PaDiv {
+    uint64_t inv;
+    int d;
+    __device__ __forceinline__ int operator()(int &rest) const {  // rest <- rest % d; the quotient
+        const int q = (int)__umul64hi((uint64_t)rest << 1, inv);
+        rest -= q * d;
+        return q;
+    }
+};
+
 struct PaArgs {
     const void *q;
     void *out;
@@ -67,6 +79,7 @@ struct PaArgs {
     int chunk, chunk_pairs;  // prefix and sequence items alternate in chunks, chunk_pairs times
     int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
     int seq_base;  // n_kv * n_seqs * seq_lanes
+    PaDiv by_chunk, by_rest, by_heads, by_seqs, by_tiles;  // chunk, seq_base - direct, n_kv, n_seqs, row_tiles
     // The first `direct` sequence items run over the whole axis and write out (their
     // rows' first state says so: l = -1); merge: the others leave states
     int direct, merge;
@@ -118,10 +131,11 @@ __device__ __forceinline__ PaItem pa_item_begin(const PaArgs &a, int i) {
     PaItem t;
     // prefix and sequence items in turn, a chunk of each, while there are both
     bool prefix;
-    const int q = i / a.chunk;
-    if (q < 2 * a.chunk_pairs) {
+    if (i < 2 * a.chunk_pairs * a.chunk) {
+        int in = i;
+        const int q = a.by_chunk(in);
         prefix = !(q & 1);
-        i -= (q + 1) / 2 * a.chunk;
+        i = (q >> 1) * a.chunk + in;
     } else {
         i -= a.chunk_pairs * a.chunk;
         prefix = i < a.prefix_items;
@@ -131,25 +145,27 @@ __device__ __forceinline__ PaItem pa_item_begin(const PaArgs &a, int i) {
     t.direct = !prefix && i < a.direct;
     int sp = 0;
     if (!prefix && !t.direct) {
-        const int rest = a.seq_base - a.direct;
-        sp = (i - a.direct) / rest;
-        i -= sp * rest;
+        i -= a.direct;
+        sp = a.by_rest(i);
+        i += a.direct;
     }
-    t.hk = i % a.n_kv;
-    i /= a.n_kv;
+    int hk = i;
+    i = a.by_heads(hk);
+    t.hk = hk;
     if (prefix) {
-        t.t = i % a.row_tiles * a.tile_toks;
-        t.split = i / a.row_tiles;
+        int tile = i;
+        t.split = a.by_tiles(tile);
+        t.t = tile * a.tile_toks;
         t.seq = -1;
         t.start = 0, t.count = a.rows, t.len = 0;
     } else {
-        t.seq = i % a.n_seqs;
-        i /= a.n_seqs;
-        t.t = i * a.tile_toks;
+        int seq = i;
+        t.t = a.by_seqs(seq) * a.tile_toks;
+        t.seq = seq;
         t.split = a.prefix_splits + sp;
-        t.start = a.seq_start[t.seq];
-        t.count = a.seq_start[t.seq + 1];
-        t.len = a.own_len ? a.own_len[t.seq] : 0;
+        t.start = a.seq_start[seq];
+        t.count = a.seq_start[seq + 1];
+        t.len = a.own_len ? a.own_len[seq] : 0;
     }
     return t;
 }
@@ -290,12 +306,12 @@ struct PaJobs {
     }
 };
 
-__device__ __forceinline__ void tma_load_3d_plain(void *dst, const CUtensorMap *tm, int x, int y, int z,
-                                                  uint64_t *bar) {
+__device__ __forceinline__ void tma_load_3d_plain(uint32_t dst, const CUtensorMap *tm, int x, int y, int z,
+                                                  uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];\n" ::"r"(smem_addr(dst)),
-        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        "[%5];\n" ::"r"(dst),
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 
@@ -516,19 +532,19 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                                 for (int r = 0; r < qb; r++)
 #pragma unroll
                                     for (int c = 0; c < HD / 64; c++)
-                                        tma_load_3d_plain(smem + L::kQ + c * kPaPlane + r * q_rows * 128, &maps.q, 64 * c,
-                                                          j.hk * a.group, j.first + r * a.box_toks, b);
+                                        tma_load_3d_plain(sbase + L::kQ + c * kPaPlane + r * q_rows * 128, &maps.q, 64 * c,
+                                                          j.hk * a.group, j.first + r * a.box_toks, smem_addr(b));
                             } else {
                                 mbar_expect_tx(b, bytes);
                             }
                             const CUtensorMap *m = &maps.kv[full][own][kv];
-                            unsigned char *dst = smem + (kv ? L::kV : L::kK);
+                            uint32_t dst = sbase + (kv ? L::kV : L::kK);
 #pragma unroll 1
                             for (int r = 0; r < copies; r++, dst += kPaBoxRows * 128)
 #pragma unroll
                                 for (int c = 0; c < HD / 64; c++)
                                     tma_load_3d_plain(dst + c * kPaPlane, m, j.hk * HD + 64 * c, key + kPaBoxRows * r,
-                                                      own ? j.seq : 0, b);
+                                                      own ? j.seq : 0, smem_addr(b));
                         }
                     }
                 }
@@ -893,8 +909,8 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
     // row tiles of a sequence that run side by side (a longer one goes round again)
     a.seq_lanes = a.n_seqs == 1 ? tiles_all : std::min(tiles_all, tiles_avg > 1 ? 2 * tiles_avg : 1);
     // Splits of the key axis for `base` items of `tiles` tiles: the fewest rounds of tiles
-    // over the resident CTAs (about 2 us a tile), against writing and reading the states
-    // (4 bytes a picosecond) and the merge's launch.
+    // over the resident CTAs (about 2 us a tile and 2 us an item), against writing and
+    // reading the states (4 bytes a picosecond) and the merge's launch.
     const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 4e6;
     auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
         int best = 1;
@@ -902,7 +918,7 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
         for (int n = 1; n <= std::min(tiles, 128); n++) {
             const int per = div_up(tiles, n);
             if (n > 1 && div_up(tiles, n - 1) == per) continue;  // the same cut with an empty split more
-            const double us = 2.0 * per * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
+            const double us = 2.0 * (per + 1) * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
             if (us < best_us) best = n, best_us = us;
         }
         return best;
@@ -945,6 +961,9 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
         a.seq_splits = a.direct == a.seq_base ? 1 : div_up(tiles, per);
     }
     a.merge = a.direct < a.seq_base || !tiles;
+    auto div = [](int d) { return PaDiv{((1ull << 63) + d - 1) / d, d}; };
+    a.by_rest = div(std::max(1, a.seq_base - a.direct));
+    a.by_heads = div(a.n_kv), a.by_seqs = div(a.n_seqs), a.by_tiles = div(a.row_tiles), a.by_chunk = div(num_sms);
     // Prefix items lean on the tensor cores and sequence items on memory, so they
     // alternate (a CTA of each per SM), unless those of the prefix are much longer:
     // then they come first, as the others even out the end.
