@@ -19,6 +19,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "lc_internal.cuh"
 #include "lc_sm100.cuh"
@@ -26,8 +27,9 @@
 namespace {
 
 constexpr int kLgThreads = 512;
-constexpr int kLgSlice = 8192;  // tokens counted at a time
-constexpr uint32_t kLgListMax = 0x7FFF0000u;  // list positions + kLgThreads stay int32
+constexpr int kLgVecs = 4;
+constexpr int kLgSlice = kLgThreads * 4 * kLgVecs;  // 8192 tokens counted at a time
+constexpr uint32_t kLgListMax = 0x7FFF0000u;  // list positions + 4 kLgThreads stay int32
 constexpr uint32_t kSeen = 0x80000000u;  // of a counter: in the history (low bits: generated count)
 
 struct LgArgs {
@@ -62,17 +64,51 @@ __device__ __forceinline__ void cluster_store(uint64_t *p, uint32_t rank, uint64
 
 __device__ __forceinline__ int clamp_index(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-__global__ void __launch_bounds__(kLgThreads) logits_kernel(const LgArgs a) {
+// One token after the penalties, the bias entry s - 1 (0: none) and the mask bit.
+struct LgRow {
+    float rep, freq, pres;
+    const float *bias;
+    __device__ __forceinline__ float operator()(float v, uint32_t c, uint32_t s) const {
+        if (c) {
+            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            c &= ~kSeen;
+            if (c) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres);
+        }
+        return s ? __fadd_rn(v, bias[s - 1]) : v;
+    }
+};
+
+__global__ void __launch_bounds__(kLgThreads, 3) logits_kernel(const __grid_constant__ LgArgs a) {
     extern __shared__ __align__(16) uint32_t lg_smem[];
     __shared__ long long best_warp[kLgThreads / 32];
     __shared__ uint64_t best_cta[16];
-    uint32_t *cnt = lg_smem;             // [kLgSlice]
+    uint32_t *cnt = lg_smem;              // [kLgSlice]
     uint32_t *slot = lg_smem + kLgSlice;  // [kLgSlice], only with a bias list: 1 + list position
     const uint32_t cl = cluster_size(), rank = cluster_rank();
     const uint32_t row = blockIdx.x / cl;
     const float *x = a.x + (size_t)row * a.ldx;
     float *y = a.y ? a.y + (size_t)row * a.ldy : nullptr;
     const lc_logits_rules &r = a.r;
+    const uint32_t p0 = min(a.n, rank * a.part), p1 = min(a.n, p0 + a.part);
+
+    // A thread's share of a slice: kLgVecs pieces of 4 tokens, kLgThreads * 4 apart,
+    // requested before the lists are counted.
+    float4 v[kLgVecs];
+    auto load = [&](uint32_t s0, uint32_t len) {
+#pragma unroll
+        for (int u = 0; u < kLgVecs; u++) {
+            const uint32_t i = (threadIdx.x + u * kLgThreads) * 4;
+            if (a.vec_x && i + 4 <= len) {
+                v[u] = *reinterpret_cast<const float4 *>(x + s0 + i);
+            } else {
+                v[u].x = i < len ? x[s0 + i] : 0.f;
+                v[u].y = i + 1 < len ? x[s0 + i + 1] : 0.f;
+                v[u].z = i + 2 < len ? x[s0 + i + 2] : 0.f;
+                v[u].w = i + 3 < len ? x[s0 + i + 3] : 0.f;
+            }
+        }
+    };
+    if (p0 < p1) load(p0, min((uint32_t)kLgSlice, p1 - p0));
 
     // the row's lists; indexes from the device are held inside the arrays
     int h0 = 0, h1 = 0, g0 = 0, b0 = 0, b1 = 0;
@@ -85,53 +121,44 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LgArgs a) {
         b0 = clamp_index(r.bias_start[row], 0, (int)r.bias_len);
         b1 = clamp_index(r.bias_start[row + 1], b0, (int)r.bias_len);
     }
-    const float rep = r.repetition ? r.repetition[row] : 1.f;
-    const float freq = r.frequency ? r.frequency[row] : 0.f;
-    const float pres = r.presence ? r.presence[row] : 0.f;
     const uint32_t *mask = nullptr;
     if (r.mask) {
         const int mr = r.mask_row ? r.mask_row[row] : (int)row;
         if (mr >= 0 && (uint32_t)mr < r.n_masks) mask = r.mask + (size_t)mr * r.mask_ld;
     }
-    const bool listed = h1 > h0 || b1 > b0;
+    const LgRow rules = {r.repetition ? r.repetition[row] : 1.f, r.frequency ? r.frequency[row] : 0.f,
+                         r.presence ? r.presence[row] : 0.f, r.bias + b0};
+    const bool listed = h1 > h0 || b1 > b0, biased = b1 > b0;
 
-    const uint32_t p0 = min(a.n, rank * a.part), p1 = min(a.n, p0 + a.part);
+    // best (value order of lc_pack_key: the bits as a signed integer; token)
     int best_ord = INT_MIN;
     uint32_t best_j = 0;
     bool any = false;
-    auto value = [&](float v, uint32_t j, uint32_t c, uint32_t s) {
-        if (c) {
-            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-            c &= ~kSeen;
-            if (c) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres);
-        }
-        if (s) v = __fadd_rn(v, r.bias[b0 + s - 1]);
-        if (mask) {
-            const uint32_t g = a.row_offset + j;
-            if (!(mask[g >> 5] >> (g & 31) & 1)) v = -INFINITY;
-        }
-        // the order of lc_pack_key: value bits as a signed integer
-        const int b = __float_as_int(v), ord = b ^ ((b >> 31) & 0x7FFFFFFF);
-        if (ord >= best_ord) best_ord = ord, best_j = j, any = true;
-        return v;
-    };
     for (uint32_t s0 = p0; s0 < p1; s0 += kLgSlice) {
-        const uint32_t len = min((uint32_t)kLgSlice, p1 - s0);
+        const uint32_t len = min((uint32_t)kLgSlice, p1 - s0), first = a.row_offset + s0;
+        if (s0 != p0) load(s0, len);
         if (listed) {
-            for (uint32_t i = threadIdx.x * 4; i < len; i += kLgThreads * 4) {
+#pragma unroll
+            for (int u = 0; u < kLgVecs; u++) {
+                const uint32_t i = (threadIdx.x + u * kLgThreads) * 4;
                 *reinterpret_cast<uint4 *>(cnt + i) = make_uint4(0, 0, 0, 0);
-                if (b1 > b0) *reinterpret_cast<uint4 *>(slot + i) = make_uint4(0, 0, 0, 0);
+                if (biased) *reinterpret_cast<uint4 *>(slot + i) = make_uint4(0, 0, 0, 0);
             }
             __syncthreads();
-            const uint32_t first = a.row_offset + s0;  // tokens outside [first, first + len) wrap past len
-            for (int i = h0 + (int)threadIdx.x; i < h1; i += kLgThreads) {
-                const uint32_t t = (uint32_t)r.hist[i] - first;
-                if (t < len) {
-                    if (i >= g0)
-                        atomicAdd(cnt + t, 1u);
-                    else
-                        atomicOr(cnt + t, kSeen);
-                }
+            // tokens outside [first, first + len) wrap past len; 4 loads in flight
+            for (int i = h0 + (int)threadIdx.x; i < h1; i += 4 * kLgThreads) {
+                uint32_t t[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    t[u] = i + u * kLgThreads < h1 ? (uint32_t)r.hist[i + u * kLgThreads] - first : ~0u;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (t[u] < len) {
+                        if (i + u * kLgThreads >= g0)
+                            atomicAdd(cnt + t[u], 1u);
+                        else
+                            atomicOr(cnt + t[u], kSeen);
+                    }
             }
             for (int i = b0 + (int)threadIdx.x; i < b1; i += kLgThreads) {
                 const uint32_t t = (uint32_t)r.bias_tok[i] - first;
@@ -139,36 +166,43 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LgArgs a) {
             }
             __syncthreads();
         }
-        for (uint32_t i = threadIdx.x * 4; i < len; i += kLgThreads * 4) {
-            const uint32_t j = s0 + i, have = min(4u, len - i);
-            float v[4];
-            if (a.vec_x && have == 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(x + j);
-                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-            } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = e < (int)have ? x[j + e] : 0.f;
-            }
-            uint4 c = make_uint4(0, 0, 0, 0), s = c;
+        for (int u = 0; u < kLgVecs; u++) {
+            const uint32_t i = (threadIdx.x + u * kLgThreads) * 4, j = s0 + i;
+            if (i >= len) break;
+            float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
             if (listed) {
-                c = *reinterpret_cast<const uint4 *>(cnt + i);
-                if (b1 > b0) s = *reinterpret_cast<const uint4 *>(slot + i);
+                const uint4 c = *reinterpret_cast<const uint4 *>(cnt + i);
+                const uint4 s = biased ? *reinterpret_cast<const uint4 *>(slot + i) : make_uint4(0, 0, 0, 0);
+                if (c.x | c.y | c.z | c.w | s.x | s.y | s.z | s.w) {
+                    e[0] = rules(e[0], c.x, s.x), e[1] = rules(e[1], c.y, s.y);
+                    e[2] = rules(e[2], c.z, s.z), e[3] = rules(e[3], c.w, s.w);
+                }
             }
-            const uint32_t cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+            if (mask) {
+                const uint32_t g = a.row_offset + j;  // 4 bits that may end in the next word, if that exists
+                const uint32_t lo = mask[g >> 5], hi = (g & 31) > 28 && i + 32 - (g & 31) < len ? mask[(g >> 5) + 1] : 0u;
+                const uint32_t bits = __funnelshift_r(lo, hi, g & 31);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (e < (int)have) v[e] = value(v[e], j + e, cc[e], ss[e]);
+                for (int q = 0; q < 4; q++)
+                    if (!(bits >> q & 1)) e[q] = -INFINITY;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int b = __float_as_int(e[q]), ord = b ^ ((b >> 31) & 0x7FFFFFFF);
+                if (ord >= best_ord && i + q < len) best_ord = ord, best_j = j + q, any = true;
+            }
             if (y) {
-                if (a.vec_y && have == 4) {
-                    *reinterpret_cast<float4 *>(y + j) = make_float4(v[0], v[1], v[2], v[3]);
+                if (a.vec_y && i + 4 <= len) {
+                    __stcs(reinterpret_cast<float4 *>(y + j), make_float4(e[0], e[1], e[2], e[3]));
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (e < (int)have) y[j + e] = v[e];
+                    for (int q = 0; q < 4; q++)
+                        if (i + q < len) y[j + q] = e[q];
                 }
             }
         }
-        __syncthreads();  // the counters are read before the next slice clears them
+        if (listed) __syncthreads();  // the counters are read before the next slice clears them
     }
     if (!a.keys) return;  // uniform over the cluster
     // (order, global token) as the signed key of lc_pack_key
@@ -233,10 +267,16 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     a.x = logits, a.y = out, a.ldx = ld, a.ldy = ld_out, a.n = n, a.row_offset = row_offset, a.r = r, a.keys = keys;
     a.vec_x = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     a.vec_y = ((uintptr_t)out & 15) == 0 && ld_out % 4 == 0;
-    // CTAs of a row's cluster: at most 8 (the portable size), each with at least
+    // CTAs of a row's cluster: 8 (the portable size), or 16 where few rows leave SMs
+    // idle (one row of 128256 tokens: a slice a CTA instead of two); each with at least
     // 2048 tokens
-    uint32_t cl = 8;
+    uint32_t cl = m * 16 <= 2u * ctx->num_sms ? 16 : 8;
     while (cl > 1 && n / cl < 2048) cl /= 2;
+    static std::atomic<uint64_t> wide{0};  // devices (below 64) on which the size is allowed already
+    if (cl > 8 && (ctx->device > 63 || !(wide.load() >> ctx->device & 1))) {
+        LC_CUDA(cudaFuncSetAttribute(logits_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        if (ctx->device < 64) wide |= 1ull << ctx->device;
+    }
     a.part = ((n + cl - 1) / cl + 127) / 128 * 128;
     const size_t smem = (size_t)kLgSlice * 4 * (r.bias_len ? 2 : 1);
     if (int s = lc_set_smem_attr((const void *)logits_kernel, smem)) return s;

@@ -9,9 +9,9 @@
 // reduced mod 2 pi there; sincosf then sees |a| <= pi.  The rotation itself is
 // f32 with one rounding to the output type.
 //
-// Bound by the bytes of x and y.  One CTA takes a row (or a share of its heads
-// when there are few rows): the row's table of (cos, sin) is formed once in
-// shared memory for every head, while each thread's first loads are in flight.
+// Bound by the bytes of x and y.  One CTA takes some rows (or a share of one
+// row's heads when there are few): the rows' table of (cos, sin) is formed once
+// in shared memory for every head, while each thread's first loads are in flight.
 #include <math.h>
 
 #include <algorithm>
@@ -22,11 +22,11 @@
 
 namespace {
 
-constexpr int kRpThreads = 128;
-// Items a thread loads before the table is ready.  A 40-head row of 128 in
-// 16-bit types is 320 items, 2.5 a thread.
-constexpr int kRpItems = 3;
-constexpr uint32_t kRpMaxDim = 8192;  // table of 32 KB
+constexpr int kRpThreads = 256;
+// Items a thread has in flight (and loads before the table is ready).  A 40-head
+// row of 128 in 16-bit types is 320 items.
+constexpr int kRpItems = 4;
+constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 
 template <class T>
 struct RpVec;  // 16 bytes of T
@@ -87,7 +87,9 @@ struct RpArgs {
     int n_q, n_heads;         // heads of q, of q and k together
     int head_dim, rope_dim;
     int rot, items;           // rotated items of a head, all items of a head
-    int heads_per_cta;
+    int heads_per_cta, rows_per_cta;
+    uint32_t m;
+    uint64_t inv_items, inv_row;  // ceil(2^63 / d) of items and of a CTA's items in a row: exact quotients below 2^31
     const int32_t *pos;
     const float *freq;
     float scale;
@@ -97,32 +99,36 @@ struct RpArgs {
 // V / 2 pairs of V neighbouring dims.  Items rot.. are V copied dims.
 template <class TI, class TO, bool PAIRS, int V, bool VEC>
 __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
-    extern __shared__ float2 cs[];  // [rope_dim / 2]
-    const size_t row = blockIdx.x;
+    extern __shared__ float2 cs_rows[];  // [rows][rope_dim / 2]
+    const size_t row0 = (size_t)blockIdx.x * a.rows_per_cta;
+    const int rows = (int)min((size_t)a.rows_per_cta, a.m - row0);
     const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.n_heads, h0 + a.heads_per_cta);
-    const int total = (h1 - h0) * a.items, half = a.rope_dim >> 1;
+    const int per_row = (h1 - h0) * a.items, total = rows * per_row, half = a.rope_dim >> 1;
 
-    auto place = [&](int idx, int &t, int &head, int &item) {
-        const int h = idx / a.items;
+    auto place = [&](int idx, int &in, int &t, int &head, int &item) {
+        in = rows == 1 ? 0 : (int)__umul64hi((uint64_t)idx << 1, a.inv_row);
+        idx -= in * per_row;
+        const int h = (int)__umul64hi((uint64_t)idx << 1, a.inv_items);
         item = idx - h * a.items;
         t = h0 + h >= a.n_q;
         head = h0 + h - (t ? a.n_q : 0);
     };
     auto first = [&](int item) { return item < a.rot ? item * V : a.rope_dim + (item - a.rot) * V; };
     auto load = [&](int idx, RpPack<TI, V> &p0, RpPack<TI, V> &p1) {
-        int t, head, item;
-        place(idx, t, head, item);
-        const TI *x = static_cast<const TI *>(t ? a.x[1] : a.x[0]) + row * (t ? a.ldx[1] : a.ldx[0]) +
+        int in, t, head, item;
+        place(idx, in, t, head, item);
+        const TI *x = static_cast<const TI *>(t ? a.x[1] : a.x[0]) + (row0 + in) * (t ? a.ldx[1] : a.ldx[0]) +
                       (size_t)head * a.head_dim + first(item);
         if (item >= a.rot && (t ? a.same[1] : a.same[0])) return;
         p0 = rp_load<TI, V, VEC>(x);
         if (!PAIRS && item < a.rot) p1 = rp_load<TI, V, VEC>(x + half);
     };
     auto finish = [&](int idx, const RpPack<TI, V> &p0, const RpPack<TI, V> &p1) {
-        int t, head, item;
-        place(idx, t, head, item);
-        TO *y = static_cast<TO *>(t ? a.y[1] : a.y[0]) + row * (t ? a.ldy[1] : a.ldy[0]) +
+        int in, t, head, item;
+        place(idx, in, t, head, item);
+        TO *y = static_cast<TO *>(t ? a.y[1] : a.y[0]) + (row0 + in) * (t ? a.ldy[1] : a.ldy[0]) +
                 (size_t)head * a.head_dim + first(item);
+        const float2 *cs = cs_rows + in * half;
         float o0[V], o1[V];
         if (item >= a.rot) {
             if (t ? a.same[1] : a.same[0]) return;
@@ -156,24 +162,25 @@ __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
     for (int j = 0; j < kRpItems; j++)
         if ((int)threadIdx.x + j * kRpThreads < total) load(threadIdx.x + j * kRpThreads, p0[j], p1[j]);
     if (half) {
-        const double pos = (double)a.pos[row];
-        for (int i = threadIdx.x; i < half; i += kRpThreads) {
-            const double t = pos * (double)a.freq[i];
-            const double n = rint(t * 0.15915494309189533577);      // 1 / (2 pi)
-            double r = fma(-n, 6.28318530717958623200, t);           // 2 pi, rounded to a double,
-            r = fma(-n, 2.44929359829470635445e-16, r);              // and what it lacks
+        for (int i = threadIdx.x; i < rows * half; i += kRpThreads) {
+            const int in = i / half;
+            const double t = (double)a.pos[row0 + in] * (double)a.freq[i - in * half];  // exact
+            const double n = t * 0.15915494309189533577;  // turns: 1 / (2 pi), rounded to a double,
+            const double d = fma(t, 0.15915494309189533577, -n) + t * -9.8393383375912435e-18;  // and what that lost
             float sn, cn;
-            sincosf((float)r, &sn, &cn);
-            cs[i] = make_float2(cn * a.scale, sn * a.scale);
+            sincospif((float)(2.0 * ((n - rint(n)) + d)), &sn, &cn);
+            cs_rows[i] = make_float2(cn * a.scale, sn * a.scale);
         }
         __syncthreads();
     }
+    for (int base = threadIdx.x; base < total;) {
 #pragma unroll
-    for (int j = 0; j < kRpItems; j++)
-        if ((int)threadIdx.x + j * kRpThreads < total) finish(threadIdx.x + j * kRpThreads, p0[j], p1[j]);
-    for (int idx = threadIdx.x + kRpItems * kRpThreads; idx < total; idx += kRpThreads) {
-        load(idx, p0[0], p1[0]);
-        finish(idx, p0[0], p1[0]);
+        for (int j = 0; j < kRpItems; j++)
+            if (base + j * kRpThreads < total) finish(base + j * kRpThreads, p0[j], p1[j]);
+        base += kRpItems * kRpThreads;
+#pragma unroll
+        for (int j = 0; j < kRpItems; j++)
+            if (base + j * kRpThreads < total) load(base + j * kRpThreads, p0[j], p1[j]);
     }
 }
 
@@ -200,18 +207,26 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     a.items = a.rot + ((q_copies || k_copies) ? (a.head_dim - a.rope_dim) / v : 0);
     if (a.items == 0) return LC_OK;
     // Few rows: a row's heads go to several CTAs, each with at least one item a
-    // thread; every CTA forms the table again (a 16-row, 40-head block of 128:
-    // 6 CTAs a row instead of 1).
-    const int per_head = a.items;
+    // thread; every CTA forms the table again.  Many rows: a CTA takes as many as
+    // give each thread 8 items, or until the grid is down to 4 CTAs per SM.
+    const int row_items = a.n_heads * a.items;
     int splits = 1;
     if (m < 2u * ctx->num_sms) {
-        const int most = std::max(1, a.n_heads * per_head / kRpThreads);
+        const int most = std::max(1, row_items / kRpThreads);
         splits = std::min<int>(most, std::max(1, 2 * ctx->num_sms / (int)m));
     }
     a.heads_per_cta = (a.n_heads + splits - 1) / splits;
     splits = (a.n_heads + a.heads_per_cta - 1) / a.heads_per_cta;
-    const dim3 grid(m, splits);
-    const size_t smem = (size_t)half * sizeof(float2);
+    a.rows_per_cta = 1;
+    const size_t table = (size_t)half * sizeof(float2);
+    while (splits == 1 && a.rows_per_cta * row_items < 8 * kRpThreads && m / (a.rows_per_cta + 1) >= 4u * ctx->num_sms &&
+           (a.rows_per_cta + 1) * table <= 32 * 1024)
+        a.rows_per_cta++;
+    a.m = m;
+    auto inv = [](uint64_t d) { return ((1ull << 63) + d - 1) / d; };
+    a.inv_items = inv(a.items), a.inv_row = inv((uint64_t)a.heads_per_cta * a.items);
+    const dim3 grid((m + a.rows_per_cta - 1) / a.rows_per_cta, splits);
+    const size_t smem = a.rows_per_cta * table;
     auto go = [&](auto kernel) -> int {
         kernel<<<grid, kRpThreads, smem, ctx->stream>>>(a);
         return lc_after_launch(ctx, "lc_rope");
