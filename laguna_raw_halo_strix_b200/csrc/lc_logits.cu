@@ -11,9 +11,11 @@
 // bits whatever the launch shape.
 //
 // Bound by reading and writing the logits once.  The history and the bias list
-// are scattered: a CTA owns a slice of the vocabulary, counts the row's tokens
+// are scattered: a CTA owns a slice of the vocabulary and counts the row's tokens
 // that fall into it in shared memory (integer adds, and a maximum over list
-// positions for biases: no order changes a result), then streams the slice.
+// positions for biases: no order changes a result), then streams the slice.  In
+// the stream a warp works its touched tokens out one per lane at a time: there are
+// a few dozen in 8192, so most warps meet one, and few lanes two.
 // A row is one cluster of CTAs, so the row's key is reduced over distributed
 // shared memory and the whole call is one launch without a workspace.
 #include <math.h>
@@ -28,8 +30,9 @@ namespace {
 
 constexpr int kLgThreads = 512;
 constexpr int kLgVecs = 4;
+constexpr int kLgHold = 8;  // 4096 tokens of a row's history
 constexpr int kLgSlice = kLgThreads * 4 * kLgVecs;  // 8192 tokens counted at a time
-constexpr uint32_t kLgListMax = 0x7FFF0000u;  // list positions + 4 kLgThreads stay int32
+constexpr uint32_t kLgListMax = 0x7FFF0000u;  // list positions + kLgHold * kLgThreads stay int32
 constexpr uint32_t kSeen = 0x80000000u;  // of a counter: in the history (low bits: generated count)
 
 struct LgArgs {
@@ -78,7 +81,7 @@ struct LgRow {
     }
 };
 
-__global__ void __launch_bounds__(kLgThreads, 3) logits_kernel(const __grid_constant__ LgArgs a) {
+__global__ void __launch_bounds__(kLgThreads, 2) logits_kernel(const __grid_constant__ LgArgs a) {
     extern __shared__ __align__(16) uint32_t lg_smem[];
     __shared__ long long best_warp[kLgThreads / 32];
     __shared__ uint64_t best_cta[16];
@@ -91,24 +94,23 @@ __global__ void __launch_bounds__(kLgThreads, 3) logits_kernel(const __grid_cons
     const lc_logits_rules &r = a.r;
     const uint32_t p0 = min(a.n, rank * a.part), p1 = min(a.n, p0 + a.part);
 
-    // A thread's share of a slice: kLgVecs pieces of 4 tokens, kLgThreads * 4 apart,
-    // requested before the lists are counted.
+    // A thread's share of a slice: kLgVecs pieces of 4 tokens, kLgThreads * 4 apart.
+    // A piece of the next slice is requested where the last one's has been written,
+    // so that it arrives while the lists are counted.
     float4 v[kLgVecs];
-    auto load = [&](uint32_t s0, uint32_t len) {
-#pragma unroll
-        for (int u = 0; u < kLgVecs; u++) {
-            const uint32_t i = (threadIdx.x + u * kLgThreads) * 4;
-            if (a.vec_x && i + 4 <= len) {
-                v[u] = *reinterpret_cast<const float4 *>(x + s0 + i);
-            } else {
-                v[u].x = i < len ? x[s0 + i] : 0.f;
-                v[u].y = i + 1 < len ? x[s0 + i + 1] : 0.f;
-                v[u].z = i + 2 < len ? x[s0 + i + 2] : 0.f;
-                v[u].w = i + 3 < len ? x[s0 + i + 3] : 0.f;
-            }
+    auto load = [&](int u, uint32_t s0) {
+        const uint32_t i = s0 + (threadIdx.x + u * kLgThreads) * 4;
+        if (a.vec_x && i + 4 <= p1) {
+            v[u] = __ldcs(reinterpret_cast<const float4 *>(x + i));
+        } else {
+            v[u].x = i < p1 ? x[i] : 0.f;
+            v[u].y = i + 1 < p1 ? x[i + 1] : 0.f;
+            v[u].z = i + 2 < p1 ? x[i + 2] : 0.f;
+            v[u].w = i + 3 < p1 ? x[i + 3] : 0.f;
         }
     };
-    if (p0 < p1) load(p0, min((uint32_t)kLgSlice, p1 - p0));
+#pragma unroll
+    for (int u = 0; u < kLgVecs; u++) load(u, p0);
 
     // the row's lists; indexes from the device are held inside the arrays
     int h0 = 0, h1 = 0, g0 = 0, b0 = 0, b1 = 0;
@@ -134,35 +136,50 @@ __global__ void __launch_bounds__(kLgThreads, 3) logits_kernel(const __grid_cons
     int best_ord = INT_MIN;
     uint32_t best_j = 0;
     bool any = false;
+    // The first kLgHold tokens of a thread's share of the history, and its first bias
+    // token, stay in registers for every slice (~0: none).
+    uint32_t held[kLgHold], held_bias = ~0u;
+#pragma unroll
+    for (int u = 0; u < kLgHold; u++) {
+        const int i = h0 + (int)threadIdx.x + u * kLgThreads;
+        held[u] = i < h1 ? (uint32_t)r.hist[i] : ~0u;
+    }
+    if (b0 + (int)threadIdx.x < b1) held_bias = (uint32_t)r.bias_tok[b0 + threadIdx.x];
+    if (listed) {
+#pragma unroll
+        for (int u = 0; u < kLgVecs; u++) {
+            const uint32_t i = (threadIdx.x + u * kLgThreads) * 4;
+            *reinterpret_cast<uint4 *>(cnt + i) = make_uint4(0, 0, 0, 0);
+            if (biased) *reinterpret_cast<uint4 *>(slot + i) = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+    }
     for (uint32_t s0 = p0; s0 < p1; s0 += kLgSlice) {
-        const uint32_t len = min((uint32_t)kLgSlice, p1 - s0), first = a.row_offset + s0;
-        if (s0 != p0) load(s0, len);
+        const uint32_t len = min((uint32_t)kLgSlice, p1 - s0);
         if (listed) {
+            // tokens outside [first, first + len) wrap past len
+            const uint32_t first = a.row_offset + s0;
+            auto count = [&](uint32_t token, int i) {
+                const uint32_t t = token - first;
+                if (t >= len) return;
+                if (i >= g0)
+                    atomicAdd(cnt + t, 1u);
+                else
+                    atomicOr(cnt + t, kSeen);
+            };
 #pragma unroll
-            for (int u = 0; u < kLgVecs; u++) {
-                const uint32_t i = (threadIdx.x + u * kLgThreads) * 4;
-                *reinterpret_cast<uint4 *>(cnt + i) = make_uint4(0, 0, 0, 0);
-                if (biased) *reinterpret_cast<uint4 *>(slot + i) = make_uint4(0, 0, 0, 0);
-            }
-            __syncthreads();
-            // tokens outside [first, first + len) wrap past len; 4 loads in flight
-            for (int i = h0 + (int)threadIdx.x; i < h1; i += 4 * kLgThreads) {
-                uint32_t t[4];
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-                    t[u] = i + u * kLgThreads < h1 ? (uint32_t)r.hist[i + u * kLgThreads] - first : ~0u;
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (t[u] < len) {
-                        if (i + u * kLgThreads >= g0)
-                            atomicAdd(cnt + t[u], 1u);
-                        else
-                            atomicOr(cnt + t[u], kSeen);
-                    }
-            }
-            for (int i = b0 + (int)threadIdx.x; i < b1; i += kLgThreads) {
-                const uint32_t t = (uint32_t)r.bias_tok[i] - first;
-                if (t < len) atomicMax(slot + t, (uint32_t)(i - b0) + 1u);
+            for (int u = 0; u < kLgHold; u++) count(held[u], h0 + (int)threadIdx.x + u * kLgThreads);
+#pragma unroll 4
+            for (int i = h0 + (int)threadIdx.x + kLgHold * kLgThreads; i < h1; i += kLgThreads)
+                count((uint32_t)r.hist[i], i);
+            if (biased) {
+                auto enter = [&](uint32_t token, uint32_t place) {
+                    const uint32_t t = token - first;
+                    if (t < len) atomicMax(slot + t, place);
+                };
+                enter(held_bias, threadIdx.x + 1u);
+                for (int i = b0 + (int)threadIdx.x + kLgThreads; i < b1; i += kLgThreads)
+                    enter((uint32_t)r.bias_tok[i], (uint32_t)(i - b0) + 1u);
             }
             __syncthreads();
         }
@@ -171,14 +188,29 @@ __global__ void __launch_bounds__(kLgThreads, 3) logits_kernel(const __grid_cons
             const uint32_t i = (threadIdx.x + u * kLgThreads) * 4, j = s0 + i;
             if (i >= len) break;
             float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-            if (listed) {
-                const uint4 c = *reinterpret_cast<const uint4 *>(cnt + i);
-                const uint4 s = biased ? *reinterpret_cast<const uint4 *>(slot + i) : make_uint4(0, 0, 0, 0);
-                if (c.x | c.y | c.z | c.w | s.x | s.y | s.z | s.w) {
-                    e[0] = rules(e[0], c.x, s.x), e[1] = rules(e[1], c.y, s.y);
-                    e[2] = rules(e[2], c.z, s.z), e[3] = rules(e[3], c.w, s.w);
+            if (listed) {  // what was counted is cleared for the next slice
+                uint4 c = *reinterpret_cast<const uint4 *>(cnt + i), s = make_uint4(0, 0, 0, 0);
+                if (c.x | c.y | c.z | c.w) *reinterpret_cast<uint4 *>(cnt + i) = s;
+                if (biased) {
+                    const uint4 t = *reinterpret_cast<const uint4 *>(slot + i);
+                    if (t.x | t.y | t.z | t.w) *reinterpret_cast<uint4 *>(slot + i) = s;
+                    s = t;
+                }
+                uint32_t left = (c.x | s.x ? 1u : 0u) | (c.y | s.y ? 2u : 0u) | (c.z | s.z ? 4u : 0u) |
+                                (c.w | s.w ? 8u : 0u);
+#pragma unroll 1
+                while (left) {
+                    const uint32_t bit = left & (0u - left);
+                    left ^= bit;
+                    const float x = bit == 1 ? e[0] : bit == 2 ? e[1] : bit == 4 ? e[2] : e[3];
+                    const uint32_t n = bit == 1 ? c.x : bit == 2 ? c.y : bit == 4 ? c.z : c.w;
+                    const uint32_t b = bit == 1 ? s.x : bit == 2 ? s.y : bit == 4 ? s.z : s.w;
+                    const float w = rules(x, n, b);
+                    e[0] = bit == 1 ? w : e[0], e[1] = bit == 2 ? w : e[1];
+                    e[2] = bit == 4 ? w : e[2], e[3] = bit == 8 ? w : e[3];
                 }
             }
+            if (s0 + kLgSlice < p1) load(u, s0 + kLgSlice);
             if (mask) {
                 const uint32_t g = a.row_offset + j;  // 4 bits that may end in the next word, if that exists
                 const uint32_t lo = mask[g >> 5], hi = (g & 31) > 28 && i + 32 - (g & 31) < len ? mask[(g >> 5) + 1] : 0u;
@@ -267,10 +299,10 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     a.x = logits, a.y = out, a.ldx = ld, a.ldy = ld_out, a.n = n, a.row_offset = row_offset, a.r = r, a.keys = keys;
     a.vec_x = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     a.vec_y = ((uintptr_t)out & 15) == 0 && ld_out % 4 == 0;
-    // CTAs of a row's cluster: 8 (the portable size), or 16 where few rows leave SMs
-    // idle (one row of 128256 tokens: a slice a CTA instead of two); each with at least
-    // 2048 tokens
-    uint32_t cl = m * 16 <= 2u * ctx->num_sms ? 16 : 8;
+    // CTAs of a row's cluster: 4, more where few rows leave SMs idle (one row of 128256
+    // tokens is a slice a CTA with 16; 256 rows take 100 us with 4, 110 with 8, 132 with
+    // 16); each with at least 2048 tokens
+    uint32_t cl = m * 16 <= 2u * ctx->num_sms ? 16 : m * 8 <= 2u * ctx->num_sms ? 8 : 4;
     while (cl > 1 && n / cl < 2048) cl /= 2;
     static std::atomic<uint64_t> wide{0};  // devices (below 64) on which the size is allowed already
     if (cl > 8 && (ctx->device > 63 || !(wide.load() >> ctx->device & 1))) {
@@ -278,7 +310,7 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
         if (ctx->device < 64) wide |= 1ull << ctx->device;
     }
     a.part = ((n + cl - 1) / cl + 127) / 128 * 128;
-    const size_t smem = (size_t)kLgSlice * 4 * (r.bias_len ? 2 : 1);
+    const size_t smem = (size_t)kLgSlice * (r.bias_len ? 8 : 4);
     if (int s = lc_set_smem_attr((const void *)logits_kernel, smem)) return s;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(m * cl);

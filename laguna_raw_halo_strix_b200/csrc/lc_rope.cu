@@ -22,10 +22,11 @@
 
 namespace {
 
-constexpr int kRpThreads = 256;
-// Items a thread has in flight (and loads before the table is ready).  A 40-head
-// row of 128 in 16-bit types is 320 items.
-constexpr int kRpItems = 4;
+constexpr int kRpThreads = 128;
+// Items a thread has in flight (and loads before the table is ready): 8192 rows of
+// 40 bf16 heads take 37 us with two in 8 CTAs an SM, 54 us with four in registers
+// for 2 CTAs of 256 threads, 65 us with one in 16.
+constexpr int kRpItems = 2;
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 
 template <class T>
@@ -79,6 +80,15 @@ __device__ __forceinline__ void rp_store(T *p, const float (&y)[N]) {
     }
 }
 
+// Place of entry i in the table: items of 8 or 4 entries (64 or 32 bytes) would
+// meet in the same banks, so their 16-byte pieces are rotated by the item.
+template <int PER>
+__device__ __forceinline__ int rp_slot(int i) {
+    if (PER == 8) return i ^ ((i >> 4 & 3) << 1);
+    if (PER == 4) return i ^ ((i >> 4 & 1) << 1);
+    return i;
+}
+
 struct RpArgs {
     const void *x[2];   // q, k
     void *y[2];
@@ -98,7 +108,7 @@ struct RpArgs {
 // PAIRS false: an item is V dims at i and the V at i + rope_dim / 2; true: the
 // V / 2 pairs of V neighbouring dims.  Items rot.. are V copied dims.
 template <class TI, class TO, bool PAIRS, int V, bool VEC>
-__global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
+__global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
     extern __shared__ float2 cs_rows[];  // [rows][rope_dim / 2]
     const size_t row0 = (size_t)blockIdx.x * a.rows_per_cta;
     const int rows = (int)min((size_t)a.rows_per_cta, a.m - row0);
@@ -138,7 +148,7 @@ __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
         } else if constexpr (PAIRS) {
 #pragma unroll
             for (int i = 0; i + 1 < V; i += 2) {
-                const float2 c = cs[(item * V + i) >> 1];
+                const float2 c = cs[rp_slot<V / 2>((item * V + i) >> 1)];
                 const float u = rp_f32(p0.v[i]), w = rp_f32(p0.v[i + 1]);
                 o0[i] = u * c.x - w * c.y;
                 o0[i + 1] = w * c.x + u * c.y;
@@ -147,7 +157,7 @@ __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float2 c = cs[item * V + i];
+                const float2 c = cs[rp_slot<V>(item * V + i)];
                 const float u = rp_f32(p0.v[i]), w = rp_f32(p1.v[i]);
                 o0[i] = u * c.x - w * c.y;
                 o1[i] = w * c.x + u * c.y;
@@ -169,7 +179,7 @@ __global__ void __launch_bounds__(kRpThreads) rope_kernel(const RpArgs a) {
             const double d = fma(t, 0.15915494309189533577, -n) + t * -9.8393383375912435e-18;  // and what that lost
             float sn, cn;
             sincospif((float)(2.0 * ((n - rint(n)) + d)), &sn, &cn);
-            cs_rows[i] = make_float2(cn * a.scale, sn * a.scale);
+            cs_rows[in * half + rp_slot<PAIRS ? V / 2 : V>(i - in * half)] = make_float2(cn * a.scale, sn * a.scale);
         }
         __syncthreads();
     }
@@ -208,7 +218,7 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     if (a.items == 0) return LC_OK;
     // Few rows: a row's heads go to several CTAs, each with at least one item a
     // thread; every CTA forms the table again.  Many rows: a CTA takes as many as
-    // give each thread 8 items, or until the grid is down to 4 CTAs per SM.
+    // give each thread 4 items, or until the grid is down to 4 CTAs per SM.
     const int row_items = a.n_heads * a.items;
     int splits = 1;
     if (m < 2u * ctx->num_sms) {
@@ -219,7 +229,7 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     splits = (a.n_heads + a.heads_per_cta - 1) / a.heads_per_cta;
     a.rows_per_cta = 1;
     const size_t table = (size_t)half * sizeof(float2);
-    while (splits == 1 && a.rows_per_cta * row_items < 8 * kRpThreads && m / (a.rows_per_cta + 1) >= 4u * ctx->num_sms &&
+    while (splits == 1 && a.rows_per_cta * row_items < 4 * kRpThreads && m / (a.rows_per_cta + 1) >= 4u * ctx->num_sms &&
            (a.rows_per_cta + 1) * table <= 32 * 1024)
         a.rows_per_cta++;
     a.m = m;
