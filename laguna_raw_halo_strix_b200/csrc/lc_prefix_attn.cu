@@ -10,16 +10,19 @@
 //
 // A work item is up to 128 query rows of one KV head (whole tokens) against a
 // range of the virtual key axis [prefix | own rows of its sequence].  Per tile
-// of 128 keys
+// of 64 keys
 //   S = Q K^T   tcgen05, Q and K K-major in shared memory, S in TMEM 0..127
-//   P           softmax warps, one thread a row, written over S as 16-bit pairs
-//               (and a second plane of what the rounding lost, for f32 outputs)
+//   P           softmax warps, one thread a row and half tile, written over S as
+//               16-bit pairs (for f32 outputs with one or two planes more of what
+//               the rounding lost)
 //   O += P V    tcgen05, P from TMEM, V read MN-major as it lies in memory
-// Q, K and V come by TMA.  Roles: warps 0-7 softmax, 8 loads, 9 MMA.  S and P
-// share their TMEM columns, so within a CTA a tile's products and its softmax
-// alternate; two CTAs share an SM (256 TMEM columns and 98 KB each) and fill
-// each other's gaps.  CTAs stay for several items: the next item's Q and K are
-// loaded while the last one's weights, values and results are worked on.
+// Q, K and V come by TMA.  Roles: warps 0-7 softmax, 8 loads of Q and K and the
+// hand-out of work, 9 loads of V, 10 issues S, 11 issues O.  K, V and S have two
+// stages: the next tile's scores are formed while the softmax warps work on this
+// one's, so that these, the longest link, do not wait (with one stage of 128 keys
+// a tile's products and softmax alternated: 3850 cycles per 128 keys).  Two CTAs share an
+// SM (256 TMEM columns and 100 KB each).  CTAs stay for several items: the next
+// one's Q and K are loaded while the last one's values and results are worked on.
 #include <float.h>
 #include <math.h>
 
@@ -32,20 +35,21 @@
 
 namespace {
 
-constexpr int kPaRows = 128, kPaKeys = 128;
-constexpr int kPaLoadWarp = 8, kPaMmaWarp = 9;  // 0..7 softmax
-constexpr int kPaThreads = 320;
-constexpr int kPaBoxRows = 32;             // key rows of one TMA copy
-constexpr uint32_t kPaPlane = 128 * 128;   // 128 rows x 64 16-bit elements (one swizzle span)
+constexpr int kPaRows = 128, kPaKeys = 64;
+constexpr int kPaLoadWarp = 8, kPaValueWarp = 9, kPaScoreWarp = 10, kPaMmaWarp = 11;  // 0..7 softmax
+constexpr int kPaThreads = 384;
+constexpr int kPaHalf = kPaKeys / 2;           // keys of a softmax warp, and of the smaller TMA copy
+constexpr uint32_t kPaPlane = kPaRows * 128;   // 128 rows of Q x 64 16-bit elements (one swizzle span)
+constexpr uint32_t kPaKvPlane = kPaKeys * 128;  // the same of K or V
 constexpr uint32_t kPaColS = 0, kPaColO = 128, kPaTmemCols = 256;
 constexpr uint32_t kPaMaxLen = 0x3FFFF000u;  // prefix_len + own_cap: ranges of the key axis stay int32
 
-// Shared memory: Q, K, V tiles of HD / 64 planes each, then the barriers.
+// Shared memory: Q, then two stages of K and of V, in HD / 64 planes each; barriers.
 template <int HD>
 struct PaSmem {
-    static constexpr uint32_t kTile = HD / 64 * kPaPlane;
-    static constexpr uint32_t kQ = 0, kK = kTile, kV = 2 * kTile, kBar = 3 * kTile;
-    static constexpr uint32_t kSched = kBar + 80, kJobs = kSched + 48, kRed = kJobs + 128;  // kRed: maxima [2][kPaRows], sums [2][kPaRows]
+    static constexpr uint32_t kTile = HD / 64 * kPaKvPlane;
+    static constexpr uint32_t kQ = 0, kK = HD / 64 * kPaPlane, kV = kK + 2 * kTile, kBar = kV + 2 * kTile;
+    static constexpr uint32_t kSched = kBar + 128, kJobs = kSched + 48, kRed = kJobs + 128;  // kRed: maxima [2][kPaRows], sums [2][kPaRows]
     static constexpr uint32_t kBytes = kRed + 4 * kPaRows * 4 + 1024;  // + slack to 1024-align the base
 };
 
@@ -93,7 +97,7 @@ struct PaArgs {
     unsigned *status;
 };
 
-// K/V copies: [a whole tile or kPaBoxRows of its rows][prefix or own][K or V], as
+// K/V copies: [half a tile or a whole one][prefix or own][K or V], as
 // [sequence][row][element] (one sequence for the prefix); Q as [token][head][element].
 struct PaMaps {
     CUtensorMap kv[2][2][2], q;
@@ -283,7 +287,7 @@ struct PaSched {
 };
 
 // Jobs in shared memory, from the load thread to the other warps: two slots, each
-// filled once and released by the 8 softmax warps and the MMA warp.
+// filled once and released by the softmax warps and those of V and the products.
 struct PaJobs {
     PaJob *slot;
     uint64_t *bar;  // full[2], empty[2]
@@ -295,8 +299,9 @@ struct PaJobs {
         mbar_arrive(bar + (k & 1));
         k++;
     }
-    __device__ __forceinline__ const PaJob &get(PaWait &wait) {
+    __device__ __forceinline__ const PaJob &get(PaWait &wait) {  // a whole warp: its lanes agree on wait.ok
         wait(bar + (k & 1), (k >> 1) & 1);
+        wait.ok = __all_sync(0xffffffffu, wait.ok);
         return slot[k & 1];
     }
     __device__ __forceinline__ void release(int lane) {
@@ -409,14 +414,16 @@ template <>
 __device__ __forceinline__ uint32_t pa_pack<__half>(float a, float b, float &la, float &lb) {
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    la = a - f.x, lb = b - f.y;
+    const float2 d = fadd2(make_float2(a, b), make_float2(-f.x, -f.y));
+    la = d.x, lb = d.y;
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 template <>
 __device__ __forceinline__ uint32_t pa_pack<__nv_bfloat16>(float a, float b, float &la, float &lb) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     const float2 f = __bfloat1622float2(h);
-    la = a - f.x, lb = b - f.y;
+    const float2 d = fadd2(make_float2(a, b), make_float2(-f.x, -f.y));
+    la = d.x, lb = d.y;
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
@@ -448,15 +455,20 @@ template <class T, class TO, int HD>
 __global__ void __launch_bounds__(kPaThreads, 2)
     prefix_attn_kernel(const __grid_constant__ PaMaps maps, const __grid_constant__ PaArgs a) {
     using L = PaSmem<HD>;
-    constexpr bool kTwoPlanes = std::is_same<TO, float>::value;  // P as hi + lo
+    // Planes of P: 1, or for f32 outputs as many as hold 22 bits or more
+    constexpr int kPlanes = !std::is_same<TO, float>::value ? 1 : std::is_same<T, __half>::value ? 2 : 3;
+    // TMEM columns of S: two stages of 64; a warp's planes of 16 columns overwrite its
+    // own 32 scores, and the third, where there is one, takes the second stage's place
+    constexpr int kStages = kPlanes < 3 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *k_full = bar, *v_full = bar + 1, *s_full = bar + 2, *p_ready = bar + 3, *pv_done = bar + 4;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 9);
+    // two of each, for the tiles of either parity
+    uint64_t *k_full = bar, *v_full = bar + 2, *s_full = bar + 4, *p_ready = bar + 6, *pv_done = bar + 8;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 14);
     const uint32_t sbase = smem_addr(smem);
     PaSched sched{smem + L::kSched};
-    PaJobs jobs{reinterpret_cast<PaJob *>(smem + L::kJobs), bar + 5};
+    PaJobs jobs{reinterpret_cast<PaJob *>(smem + L::kJobs), bar + 10};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     PaItem next;
@@ -466,15 +478,15 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     }
     griddep_launch_dependents();  // the merge kernel may be scheduled once the last items run
     if (threadIdx.x == 0) {
-        mbar_init(k_full, 1);
-        mbar_init(v_full, 1);
-        mbar_init(s_full, 1);
-        mbar_init(p_ready, 8);
-        mbar_init(pv_done, 1);
         mbar_init(sched.bar(), 1);
         for (int k = 0; k < 2; k++) {
+            mbar_init(k_full + k, 1);
+            mbar_init(v_full + k, 1);
+            mbar_init(s_full + k, 1);
+            mbar_init(p_ready + k, 8);
+            mbar_init(pv_done + k, 1);
             mbar_init(jobs.bar + k, 1);
-            mbar_init(jobs.bar + 2 + k, 9);
+            mbar_init(jobs.bar + 2 + k, 11);
         }
         mbar_init_fence();
     }
@@ -489,10 +501,20 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     tc_fence_after();
     const uint32_t tbase = *tslot;
     PaWait wait{a.status};
-    uint32_t it = 0;  // tiles so far: every barrier completes once per tile
+    // Tile `it` counts on through the CTA's jobs; its stage is it & 1, and each barrier
+    // of that stage completes once for it: the phase (it >> 1) & 1.
+    uint32_t it = 0;
+    auto tile_done = [&](uint64_t *b, uint32_t t) { wait(b + (t & 1), (t >> 1) & 1); };
+    auto load_rows = [&](uint32_t slot, const PaJob &j, int key, int nk, bool own, int kv, uint64_t *b, uint32_t more) {
+        const bool full = nk > kPaHalf;
+        mbar_expect_tx(b, (full ? kPaKeys : kPaHalf) * HD * 2 + more);
+#pragma unroll
+        for (int c = 0; c < HD / 64; c++)
+            tma_load_3d_plain(sbase + slot + c * kPaKvPlane, &maps.kv[full][own][kv], j.hk * HD + 64 * c, key,
+                              own ? j.seq : 0, smem_addr(b));
+    };
 
-    if (warp == kPaLoadWarp) {  // ---- loads
-        // (kept short: the thread has about 1500 cycles a tile beside its waits)
+    if (warp == kPaLoadWarp) {  // ---- work, Q and K
         if (lane == 0) {
             while (true) {
                 pa_item_finish(a, next);
@@ -509,43 +531,31 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     jobs.put(wait, j);
 #pragma unroll 1
                     for (int i = 0; i < j.n && wait.ok; i++, it++) {
-                        // The next item is asked for two tiles before this one's end (not sooner: an
-                        // item taken early would wait behind this one while other CTAs run dry).
-                        if (!asked && i >= j.n - 2 && at + next.t_step >= next.count) sched.ask(), asked = true;
+                        // The next item is asked for four tiles before this one's end (not sooner:
+                        // an item taken early would wait behind this one while other CTAs run dry).
+                        if (!asked && i >= j.n - 4 && at + next.t_step >= next.count) sched.ask(), asked = true;
                         int key, nk;
                         bool own;
                         j.tile(i, key, nk, own);
-                        const bool full = nk == kPaKeys;
-                        const int copies = full ? 1 : (nk + kPaBoxRows - 1) / kPaBoxRows;
-                        const uint32_t bytes = (full ? kPaKeys : copies * kPaBoxRows) * HD * 2;
-#pragma unroll 1
-                        for (int kv = 0; kv < 2; kv++) {
-                            // the slot is free once the products that read it are done (Q: those
-                            // of the last job's last scores)
-                            if (it) wait(kv ? pv_done : s_full, (it - 1) & 1);
+                        // K's stage is free once the scores of two tiles ago are formed, Q's place
+                        // once the last job's all are
+                        if (it >= 2) tile_done(s_full, it - 2);
+                        uint32_t q_bytes = 0;
+                        if (i == 0) {
+                            if (it) tile_done(s_full, it - 1);
                             if (!wait.ok) break;
-                            uint64_t *b = kv ? v_full : k_full;
-                            if (i == 0 && kv == 0) {
-                                const int qb = (j.count + a.box_toks - 1) / a.box_toks, q_rows = a.box_toks * a.group;
-                                mbar_expect_tx(b, bytes + (uint32_t)(qb * q_rows * HD * 2));
+                            const int qb = (j.count + a.box_toks - 1) / a.box_toks, q_rows = a.box_toks * a.group;
+                            q_bytes = qb * q_rows * HD * 2;
 #pragma unroll 1
-                                for (int r = 0; r < qb; r++)
-#pragma unroll
-                                    for (int c = 0; c < HD / 64; c++)
-                                        tma_load_3d_plain(sbase + L::kQ + c * kPaPlane + r * q_rows * 128, &maps.q, 64 * c,
-                                                          j.hk * a.group, j.first + r * a.box_toks, smem_addr(b));
-                            } else {
-                                mbar_expect_tx(b, bytes);
-                            }
-                            const CUtensorMap *m = &maps.kv[full][own][kv];
-                            uint32_t dst = sbase + (kv ? L::kV : L::kK);
-#pragma unroll 1
-                            for (int r = 0; r < copies; r++, dst += kPaBoxRows * 128)
+                            for (int r = 0; r < qb; r++)
 #pragma unroll
                                 for (int c = 0; c < HD / 64; c++)
-                                    tma_load_3d_plain(dst + c * kPaPlane, m, j.hk * HD + 64 * c, key + kPaBoxRows * r,
-                                                      own ? j.seq : 0, smem_addr(b));
+                                    tma_load_3d_plain(sbase + L::kQ + c * kPaPlane + r * q_rows * 128, &maps.q, 64 * c,
+                                                      j.hk * a.group, j.first + r * a.box_toks,
+                                                      smem_addr(k_full + (it & 1)));
                         }
+                        if (!wait.ok) break;
+                        load_rows(L::kK + (it & 1) * L::kTile, j, key, nk, own, 0, k_full + (it & 1), q_bytes);
                     }
                 }
                 if (!asked) sched.ask();
@@ -556,85 +566,124 @@ __global__ void __launch_bounds__(kPaThreads, 2)
             PaJob last = {};
             last.n = -1;
             jobs.put(wait, last);
-            if (!wait.ok) {  // copies of this CTA still in flight
-                mbar_wait(k_full, it & 1);
-                mbar_wait(v_full, it ? (it - 1) & 1 : 0);
-            }
+            if (!wait.ok)  // copies of this CTA still in flight
+                for (uint32_t t = it > 2 ? it - 2 : 0; t <= it; t++) mbar_wait(k_full + (t & 1), (t >> 1) & 1);
         }
-    } else if (warp == kPaMmaWarp) {  // ---- products
+    } else if (warp == kPaValueWarp) {  // ---- V
 #pragma unroll 1
         while (wait.ok) {
             const PaJob &j = jobs.get(wait);
             const int n = wait.ok ? j.n : -1;
             if (n < 0) break;
-            {
+            if (lane == 0) {
 #pragma unroll 1
-                for (int i = 0; i < n; i++, it++) {
+                for (int i = 0; i < n && wait.ok; i++) {
+                    const uint32_t t = it + i;
                     int key, nk;
                     bool own;
                     j.tile(i, key, nk, own);
-                    wait(k_full, it & 1);
-                    if (!wait.ok) break;
-                    __syncwarp();
-                    tc_fence_after();
-                    // unrolled: a product runs 64 cycles, and a loop around one takes 88 to issue it
-                    if (lane == 0) {
-                        const uint64_t qd = umma_desc_sw128(sbase + L::kQ), kd = umma_desc_sw128(sbase + L::kK);
-#pragma unroll
-                        for (int s = 0; s < HD / 16; s++) {
-                            const uint64_t o = ((s >> 2) * kPaPlane + (s & 3) * 32) >> 4;
-                            umma_f16_ss(tbase + kPaColS, qd + o, kd + o, pa_idesc<T>(kPaKeys, false), s ? 1u : 0u);
-                        }
-                        umma_commit(s_full);
-                    }
-                    __syncwarp();
-                    wait(v_full, it & 1);
-                    // keys of the tile's last 16-key step that do not exist: their P is 0,
-                    // and 0 times whatever lies there must not be NaN
-                    const int steps = (nk + 15) >> 4, gone = steps * 16 - nk;
-                    if (gone && wait.ok) {
+                    if (t >= 2) tile_done(pv_done, t - 2);
+                    if (wait.ok) load_rows(L::kV + (t & 1) * L::kTile, j, key, nk, own, 1, v_full + (t & 1), 0);
+                }
+            }
+            it += n;
+            wait.ok = __all_sync(0xffffffffu, wait.ok);
+            if (wait.ok) jobs.release(lane);
+        }
+        if (lane == 0 && !wait.ok)
+            for (uint32_t t = it > 2 ? it - 2 : 0; t <= it; t++) mbar_wait(v_full + (t & 1), (t >> 1) & 1);
+    } else if (warp == kPaScoreWarp) {  // ---- scores
 #pragma unroll 1
-                        for (int e = lane; e < gone * (HD / 8); e += 32) {
-                            const int row = nk + e / (HD / 8), ch = e % (HD / 8);
-                            *reinterpret_cast<uint4 *>(smem + L::kV + (ch >> 3) * kPaPlane + row * 128 +
-                                                       (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    wait(p_ready, it & 1);
-                    if (!wait.ok) break;
-                    __syncwarp();
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint64_t vd = pa_desc_mn(sbase + L::kV, HD > 64 ? kPaPlane : 1024u);
-                        auto step = [&](int s) {
-                            const uint32_t p = tbase + kPaColS + (s >> 2) * 64 + (s & 3) * 8;
-                            const uint64_t v = vd + ((s * 2048) >> 4);
-                            umma_f16_ts(tbase + kPaColO, p, v, pa_idesc<T>(HD, true), (i | s) ? 1u : 0u);
-                            if constexpr (kTwoPlanes)
-                                umma_f16_ts(tbase + kPaColO, p + 32, v, pa_idesc<T>(HD, true), 1u);
-                        };
-                        if (steps == 8) {
-#pragma unroll
-                            for (int s = 0; s < 8; s++) step(s);
-                        } else {
+        while (wait.ok) {
+            const PaJob &j = jobs.get(wait);
+            const int n = wait.ok ? j.n : -1;
+            if (n < 0) break;
 #pragma unroll 1
-                            for (int s = 0; s < steps; s++) step(s);
-                        }
-                        umma_commit(pv_done);
+            for (int i = 0; i < n && wait.ok; i++, it++) {
+                // S's stage is free once the products with the weights that took its place are done
+                if (it >= kStages) tile_done(pv_done, it - kStages);
+                tile_done(k_full, it);
+                wait.ok = __all_sync(0xffffffffu, wait.ok);
+                tc_fence_after();
+                // unrolled: a product runs 50 cycles, and a loop around one takes 88 to issue it
+                if (lane == 0 && wait.ok) {
+                    const uint64_t qd = umma_desc_sw128(sbase + L::kQ);
+                    const uint64_t kd = umma_desc_sw128(sbase + L::kK + (it & 1) * L::kTile);
+                    const uint32_t d = tbase + kPaColS + (it & (kStages - 1)) * kPaKeys;
+#pragma unroll
+                    for (int s = 0; s < HD / 16; s++)
+                        umma_f16_ss(d, qd + (((s >> 2) * kPaPlane + (s & 3) * 32) >> 4),
+                                    kd + (((s >> 2) * kPaKvPlane + (s & 3) * 32) >> 4), pa_idesc<T>(kPaKeys, false),
+                                    s ? 1u : 0u);
+                    umma_commit(s_full + (it & 1));
+                }
+                __syncwarp();
+            }
+            if (wait.ok) jobs.release(lane);
+        }
+        if (!wait.ok)  // products still under way
+            for (uint32_t t = it > 2 ? it - 2 : 0; t < it; t++) mbar_wait(s_full + (t & 1), (t >> 1) & 1);
+    } else if (warp == kPaMmaWarp) {  // ---- values
+#pragma unroll 1
+        while (wait.ok) {
+            const PaJob &j = jobs.get(wait);
+            const int n = wait.ok ? j.n : -1;
+            if (n < 0) break;
+#pragma unroll 1
+            for (int i = 0; i < n && wait.ok; i++, it++) {
+                int key, nk;
+                bool own;
+                j.tile(i, key, nk, own);
+                tile_done(v_full, it);
+                // keys of the tile's last 16-key step that do not exist: their P is 0,
+                // and 0 times whatever lies there must not be NaN
+                const uint32_t v_at = L::kV + (it & 1) * L::kTile;
+                const int steps = (nk + 15) >> 4, gone = steps * 16 - nk;
+                if (gone && wait.ok) {
+#pragma unroll 1
+                    for (int e = lane; e < gone * (HD / 8); e += 32) {
+                        const int row = nk + e / (HD / 8), ch = e % (HD / 8);
+                        *reinterpret_cast<uint4 *>(smem + v_at + (ch >> 3) * kPaKvPlane + row * 128 + (ch & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
                     }
+                    fence_proxy_async_smem();
                     __syncwarp();
                 }
+                tile_done(p_ready, it);
+                wait.ok = __all_sync(0xffffffffu, wait.ok);
+                if (!wait.ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t vd = pa_desc_mn(sbase + v_at, HD > 64 ? kPaKvPlane : 1024u);
+                    const uint32_t ps = tbase + kPaColS + (it & (kStages - 1)) * kPaKeys;
+                    auto step = [&](int s) {
+                        const uint32_t p = ps + (s >> 1) * 32 + (s & 1) * 8;
+                        const uint64_t v = vd + ((s * 2048) >> 4);
+                        constexpr uint32_t id = pa_idesc<T>(HD, true);
+                        umma_f16_ts(tbase + kPaColO, p, v, id, (i | s) ? 1u : 0u);
+                        if constexpr (kPlanes > 1) umma_f16_ts(tbase + kPaColO, p + 16, v, id, 1u);
+                        if constexpr (kPlanes > 2)
+                            umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 64 + 8 * s, v, id, 1u);
+                    };
+                    if (steps == 4) {
+#pragma unroll
+                        for (int s = 0; s < 4; s++) step(s);
+                    } else {
+#pragma unroll 1
+                        for (int s = 0; s < steps; s++) step(s);
+                    }
+                    umma_commit(pv_done + (it & 1));
+                }
+                __syncwarp();
             }
             jobs.release(lane);
         }
-        if (!wait.ok && it) mbar_wait(pv_done, (it - 1) & 1);
+        if (!wait.ok)  // products still under way
+            for (uint32_t t = it > 2 ? it - 2 : 0; t < it; t++) mbar_wait(pv_done + (t & 1), (t >> 1) & 1);
     } else {  // ---- softmax
-        // Row = TMEM lane; the two warps of a lane quarter take 64 keys of a tile, and half
-        // of O's columns, each (64 scores in registers; one warp per quarter and 128 keys
-        // left the chain of a tile 1.6x as long).  Thread pairs meet at a barrier of their
-        // two warps to agree on a row's maximum.
+        // Row = TMEM lane; the two warps of a lane quarter take half of a tile's keys, and of
+        // O's columns, each.  Thread pairs meet at a barrier of their two warps to agree
+        // on a row's maximum.
         const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
         const uint32_t ts = tbase + lanes + kPaColS, to = tbase + lanes + kPaColO + half * (HD / 2);
@@ -655,34 +704,31 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     int key, nk;
                     bool own;
                     j.tile(i, key, nk, own);
-                    wait(s_full, it & 1);
+                    tile_done(s_full, it);
                     __syncwarp();
                     if (busy) {
+                        const uint32_t st = ts + (it & (kStages - 1)) * kPaKeys + kPaHalf * half;
                         tc_fence_after();
                         // keys [0, lim) of this half are visible to the row
                         int lim = nk;
                         if (own && a.causal)
                             lim = min(max(j.pos0 + j.first + pa_token(a, row) + 1 - key, 0), nk);
-                        lim -= 64 * half;
-                        float s0[32], s1[32];
-                        tmem_ld32(ts + 64 * half, s0);
-                        tmem_ld32(ts + 64 * half + 32, s1);
+                        lim -= kPaHalf * half;
+                        float x[kPaHalf];
+                        tmem_ld32(st, x);
                         tmem_ld_wait();
-                        tmem_regs_ready(s0);
-                        tmem_regs_ready(s1);
-                        const bool part = __any_sync(0xffffffffu, lim < 64);
+                        tmem_regs_ready(x);
+                        const bool part = __any_sync(0xffffffffu, lim < kPaHalf);
                         if (part) {
 #pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                if (e >= lim) s0[e] = -INFINITY;
-                                if (32 + e >= lim) s1[e] = -INFINITY;
-                            }
+                            for (int e = 0; e < kPaHalf; e++)
+                                if (e >= lim) x[e] = -INFINITY;
                         }
-                        float t0 = s0[0], t1 = s0[1], t2 = s1[0], t3 = s1[1];
+                        float t0 = x[0], t1 = x[1], t2 = x[2], t3 = x[3];
 #pragma unroll
-                        for (int e = 2; e < 32; e += 2) {
-                            t0 = fmaxf(t0, s0[e]), t1 = fmaxf(t1, s0[e + 1]);
-                            t2 = fmaxf(t2, s1[e]), t3 = fmaxf(t3, s1[e + 1]);
+                        for (int e = 4; e < kPaHalf; e += 4) {
+                            t0 = fmaxf(t0, x[e]), t1 = fmaxf(t1, x[e + 1]);
+                            t2 = fmaxf(t2, x[e + 2]), t3 = fmaxf(t3, x[e + 3]);
                         }
                         const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2;
                         // The reference maximum moves, and O is rescaled, only when a score is
@@ -693,7 +739,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             const float m_new = fmaxf(m_ref, fmaxf(top, *other));
                             const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
                             if (i) {
-                                wait(pv_done, (it - 1) & 1);
+                                tile_done(pv_done, it - 1);
                                 __syncwarp();
                                 tc_fence_after();
 #pragma unroll 1
@@ -713,39 +759,33 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
                         const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
                         // P as pairs over the first half of the warp's own scores, what the rounding
-                        // lost over the second
-                        auto weights = [&](const float (&x)[32], int c, auto by_polynomial) {
-                            uint32_t hi[16];
-                            [[maybe_unused]] uint32_t lo[16];
+                        // lost over the second, and what that lost in the other stage
+                        auto weights = [&](auto by_polynomial) {
+                            uint32_t p[3][16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
                                 const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
-                                const float2 p = decltype(by_polynomial)::value && e % 4 == 3
-                                                     ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(t)
-                                                     : make_float2(exp2_fast(t.x), exp2_fast(t.y));
-                                l = fadd2(l, p);
-                                float r0, r1;
-                                hi[e] = pa_pack<T>(p.x, p.y, r0, r1);
-                                if constexpr (kTwoPlanes) {
-                                    float u0, u1;
-                                    lo[e] = pa_pack<T>(r0, r1, u0, u1);
-                                }
+                                float2 w = decltype(by_polynomial)::value && e % 4 == 3
+                                               ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(t)
+                                               : make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                                l = fadd2(l, w);
+#pragma unroll
+                                for (int k = 0; k < kPlanes; k++) p[k][e] = pa_pack<T>(w.x, w.y, w.x, w.y);
                             }
-                            tmem_st16(ts + 64 * half + 16 * c, hi);
-                            if constexpr (kTwoPlanes) tmem_st16(ts + 64 * half + 32 + 16 * c, lo);
+                            tmem_st16(st, p[0]);
+                            if constexpr (kPlanes > 1) tmem_st16(st + 16, p[1]);
+                            if constexpr (kPlanes > 2) tmem_st16(ts + 64 + 16 * half, p[2]);
                         };
-                        if (kTwoPlanes || part) {
-                            if (nk > 64 * half) weights(s0, 0, std::false_type());  // the products stop at nk
-                            if (nk > 64 * half + 32) weights(s1, 1, std::false_type());
+                        if (kPlanes > 1 || part) {
+                            if (nk > kPaHalf * half) weights(std::false_type());  // the products stop at nk
                         } else {
-                            weights(s0, 0, std::true_type());
-                            weights(s1, 1, std::true_type());
+                            weights(std::true_type());
                         }
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
                     }
-                    if (lane == 0) mbar_arrive(p_ready);
+                    if (lane == 0) mbar_arrive(p_ready + (it & 1));
                 }
                 if (busy) {
                     mine[2 * kPaRows] = l.x + l.y;
@@ -754,7 +794,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     const bool real = row < j.count * a.group;
                     const int tok = j.first + pa_token(a, row), gq = j.first * a.group + row;
                     if (n) {
-                        wait(pv_done, (it - 1) & 1);
+                        tile_done(pv_done, it - 1);
                         __syncwarp();
                         tc_fence_after();
                     }
@@ -909,16 +949,16 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
     // row tiles of a sequence that run side by side (a longer one goes round again)
     a.seq_lanes = a.n_seqs == 1 ? tiles_all : std::min(tiles_all, tiles_avg > 1 ? 2 * tiles_avg : 1);
     // Splits of the key axis for `base` items of `tiles` tiles: the fewest rounds of tiles
-    // over the resident CTAs (about 2 us a tile and 2 us an item), against writing and
+    // over the resident CTAs (about 1 us a tile and 2 us an item), against writing and
     // reading the states (4 bytes a picosecond) and the merge's launch.
     const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 4e6;
     auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
         int best = 1;
         double best_us = 1e30;
-        for (int n = 1; n <= std::min(tiles, 128); n++) {
+        for (int n = 1; n <= std::min(tiles, 256); n++) {
             const int per = div_up(tiles, n);
             if (n > 1 && div_up(tiles, n - 1) == per) continue;  // the same cut with an empty split more
-            const double us = 2.0 * (per + 1) * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
+            const double us = (per + 2.0) * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
             if (us < best_us) best = n, best_us = us;
         }
         return best;
@@ -943,10 +983,10 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
         int per;
         const int64_t real = (int64_t)a.n_kv * tiles_all;  // about so many items have rows
         if (!joint) {
-            // Own parts differ in length: items of at most 4 tiles keep one long sequence from
+            // Own parts differ in length: items of at most 8 tiles keep one long sequence from
             // being the launch's tail, unless there are many sequences to even out.
             per = div_up(tiles, splits_for(a.seq_base, tiles, true));
-            if (a.seq_base < 16 * slots) per = std::min(per, 4);
+            if (a.seq_base < 16 * slots) per = std::min(per, 8);
         } else if (real < slots) {
             per = div_up(tiles, splits_for(real, tiles, false));
             if (per == tiles) a.direct = a.seq_base;
@@ -1082,7 +1122,7 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     }
     PaMaps maps = {};
     for (int full = 0; full < 2; full++) {
-        const uint32_t box = full ? kPaKeys : kPaBoxRows;
+        const uint32_t box = full ? kPaKeys : kPaHalf;
         if (a.prefix_len) {
             const uint64_t dims[3] = {wk, kv->prefix_len, 1}, ld[2] = {ldp, ldp};
             if (int s = pa_map(&maps.kv[full][0][0], kv->k_prefix, dtype, dims, ld, box, 1)) return s;
