@@ -385,28 +385,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// 2^x of two numbers on the FMA pipes, which the special function unit (16 results
-// a cycle and SM, the limit of a tile's weights) leaves idle: x = n + f with n
-// the nearest integer, read off the low mantissa bits after adding 1.5 * 2^23;
-// 2^f by a polynomial of degree N (least squares of the relative error over
-// [-1/2, 1/2]: off by 7.5e-5 for N = 3, 2.6e-6 for N = 4, against half a step of
-// 2e-3 for bf16 and 2.4e-4 for f16 weights); n added to the exponent.  Below
-// -126 the result stays at 2^-126.
-template <int N>
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    constexpr float c[2][5] = {{0.99992806f, 0.69326097f, 0.24261113f, 0.05517167f, 0.f},
-                               {0.99999928f, 0.69312179f, 0.24024744f, 0.05591786f, 0.0095701f}};
-    constexpr float kMagic = 12582912.f;
-    const float2 m = make_float2(kMagic, kMagic), mm = make_float2(-kMagic, -kMagic);
-    x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
-    const float2 r = fadd2(x, m), n = fadd2(r, mm), f = ffma2(n, make_float2(-1.f, -1.f), x);
-    float2 p = make_float2(c[N - 3][N], c[N - 3][N]);
-#pragma unroll
-    for (int i = N - 1; i >= 0; i--) p = ffma2(p, f, make_float2(c[N - 3][i], c[N - 3][i]));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
-}
-
 // (a, b) as a pair of T, and what that lost.
 template <class T>
 __device__ __forceinline__ uint32_t pa_pack(float a, float b, float &la, float &lb);
@@ -718,8 +696,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         tmem_ld32(st, x);
                         tmem_ld_wait();
                         tmem_regs_ready(x);
-                        const bool part = __any_sync(0xffffffffu, lim < kPaHalf);
-                        if (part) {
+                        if (__any_sync(0xffffffffu, lim < kPaHalf)) {
 #pragma unroll
                             for (int e = 0; e < kPaHalf; e++)
                                 if (e >= lim) x[e] = -INFINITY;
@@ -760,14 +737,12 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         const float2 sc = make_float2(a.scale_log2, a.scale_log2), ng = make_float2(neg, neg);
                         // P as pairs over the first half of the warp's own scores, what the rounding
                         // lost over the second, and what that lost in the other stage
-                        auto weights = [&](auto by_polynomial) {
-                            uint32_t p[3][16];
+                        if (nk > kPaHalf * half) {  // the products stop at nk
+                            uint32_t p[kPlanes][16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
                                 const float2 t = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sc, ng);
-                                float2 w = decltype(by_polynomial)::value && e % 4 == 3
-                                               ? exp2_poly<std::is_same<T, __half>::value ? 4 : 3>(t)
-                                               : make_float2(exp2_fast(t.x), exp2_fast(t.y));
+                                float2 w = make_float2(exp2_fast(t.x), exp2_fast(t.y));
                                 l = fadd2(l, w);
 #pragma unroll
                                 for (int k = 0; k < kPlanes; k++) p[k][e] = pa_pack<T>(w.x, w.y, w.x, w.y);
@@ -775,11 +750,6 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             tmem_st16(st, p[0]);
                             if constexpr (kPlanes > 1) tmem_st16(st + 16, p[1]);
                             if constexpr (kPlanes > 2) tmem_st16(ts + 64 + 16 * half, p[2]);
-                        };
-                        if (kPlanes > 1 || part) {
-                            if (nk > kPaHalf * half) weights(std::false_type());  // the products stop at nk
-                        } else {
-                            weights(std::true_type());
                         }
                         tmem_st_wait();
                         tc_fence_before();
@@ -950,8 +920,8 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
     a.seq_lanes = a.n_seqs == 1 ? tiles_all : std::min(tiles_all, tiles_avg > 1 ? 2 * tiles_avg : 1);
     // Splits of the key axis for `base` items of `tiles` tiles: the fewest rounds of tiles
     // over the resident CTAs (about 1 us a tile and 2 us an item), against writing and
-    // reading the states (4 bytes a picosecond) and the merge's launch.
-    const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 4e6;
+    // reading the states (8 bytes a picosecond) and the merge's launch.
+    const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 8e6;
     auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
         int best = 1;
         double best_us = 1e30;
