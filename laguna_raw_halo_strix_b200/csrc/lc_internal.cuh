@@ -32,6 +32,7 @@ struct lc_ctx {
     size_t scratch_bytes[8] = {};
     // Blocks that lc_scratch_kept replaced, freed by lc_destroy.
     std::vector<void *> kept;
+    size_t kept_bytes = 0;
     // Device word that kernels set (atomicOr of LC_DEV_*) when a bounded wait
     // gives up; read and cleared by lc_device_status().  Allocated at init.
     unsigned *dev_status = nullptr;

@@ -42,6 +42,7 @@ constexpr int kPaHalf = kPaKeys / 2;           // keys of a softmax warp, and of
 constexpr uint32_t kPaPlane = kPaRows * 128;   // 128 rows of Q x 64 16-bit elements (one swizzle span)
 constexpr uint32_t kPaKvPlane = kPaKeys * 128;  // the same of K or V
 constexpr uint32_t kPaColS = 0, kPaColO = 128, kPaTmemCols = 256;
+constexpr int64_t kPaMaxItems = 1 << 22;
 constexpr uint32_t kPaMaxLen = 0x3FFFF000u;  // prefix_len + own_cap: ranges of the key axis stay int32
 
 // Shared memory: Q, then two stages of K and of V, in HD / 64 planes each; barriers.
@@ -454,7 +455,6 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         next = pa_item_begin(a, blockIdx.x);
         prefetch_tensormap(&maps.q);
     }
-    griddep_launch_dependents();  // the merge kernel may be scheduled once the last items run
     if (threadIdx.x == 0) {
         mbar_init(sched.bar(), 1);
         for (int k = 0; k < 2; k++) {
@@ -541,6 +541,9 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                 if (w < 0) break;
                 next = pa_item_begin(a, w);
             }
+            // Nothing is left to take over: the merge kernel may be scheduled once every CTA is
+            // here (not from the start: its waiting CTAs kept SMs from this kernel's)
+            griddep_launch_dependents();
             PaJob last = {};
             last.n = -1;
             jobs.put(wait, last);
@@ -1081,7 +1084,8 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     a.status = ctx->dev_status;
     pa_plan(a, ctx->num_sms, (int)head_dim);
     const int64_t items = a.prefix_items + a.direct + (int64_t)(a.seq_base - a.direct) * a.seq_splits;
-    LC_REQUIRE(items <= 0x7FFFFFFF, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
+    // (a CTA that skips empty items must not keep its other warps waiting past their bound)
+    LC_REQUIRE(items <= kPaMaxItems, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
     if (a.merge) {
         a.row_blocks = div_up((int64_t)rows * a.group, 32);
         const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;

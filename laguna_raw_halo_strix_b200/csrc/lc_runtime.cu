@@ -85,7 +85,7 @@ extern "C" int lc_init(int device, lc_ctx **out) {
 
 extern "C" int lc_ctx_scratch_bytes(lc_ctx *ctx, size_t *bytes) {
     LC_REQUIRE(ctx && bytes, LC_ERR_INVALID, "lc_ctx_scratch_bytes: null argument");
-    size_t t = 0;
+    size_t t = ctx->kept_bytes;
     for (int i = 0; i < LC_SCRATCH_COUNT; i++) t += ctx->scratch_bytes[i];
     *bytes = t;
     return LC_OK;
@@ -248,7 +248,10 @@ int lc_scratch_kept(lc_ctx *ctx, int slot, size_t bytes, void **out) {
             cudaGetLastError();
             return lc_fail(LC_ERR_OOM, "scratch: cudaMalloc(%zu): %s", want, cudaGetErrorString(e));
         }
-        if (ctx->scratch[slot]) ctx->kept.push_back(ctx->scratch[slot]);
+        if (ctx->scratch[slot]) {
+            ctx->kept.push_back(ctx->scratch[slot]);
+            ctx->kept_bytes += ctx->scratch_bytes[slot];
+        }
         ctx->scratch[slot] = p;
         ctx->scratch_bytes[slot] = want;
     }
