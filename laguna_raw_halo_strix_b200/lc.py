@@ -223,14 +223,15 @@ class LogitsRules(C.Structure):
     def __init__(self, hist=None, hist_start=None, gen_start=None, repetition=None, frequency=None, presence=None,
                  bias_tok=None, bias=None, bias_start=None, mask=None, mask_row=None, hist_len=None, bias_len=None,
                  mask_ld=None, n_masks=None):
-        def size(t, given):
-            return given if given is not None else 0 if t is None else t.numel()
-
+        if hist_len is None:
+            hist_len = 0 if hist is None else hist.numel()
+        if bias_len is None:
+            bias_len = 0 if bias_tok is None else bias_tok.numel()
         if mask is not None and (mask_ld is None or n_masks is None):
             n_masks, mask_ld = mask.shape[0], mask.stride(0)
-        super().__init__(ptr(hist), ptr(hist_start), ptr(gen_start), size(hist, hist_len), ptr(repetition),
-                         ptr(frequency), ptr(presence), ptr(bias_tok), ptr(bias), ptr(bias_start),
-                         size(bias_tok, bias_len), ptr(mask), ptr(mask_row), mask_ld or 0, n_masks or 0)
+        super().__init__(ptr(hist), ptr(hist_start), ptr(gen_start), hist_len, ptr(repetition), ptr(frequency),
+                         ptr(presence), ptr(bias_tok), ptr(bias), ptr(bias_start), bias_len, ptr(mask), ptr(mask_row),
+                         mask_ld or 0, n_masks or 0)
         self.held = (hist, hist_start, gen_start, repetition, frequency, presence, bias_tok, bias, bias_start, mask,
                      mask_row)
 
@@ -285,9 +286,10 @@ def ptr(t) -> int:
     """Device pointer of a torch tensor / int / None."""
     if t is None:
         return 0
-    if isinstance(t, int):
+    try:
+        return t.data_ptr()
+    except AttributeError:
         return t
-    return t.data_ptr()
 
 
 def pack_key(value: float, index: int) -> int:
@@ -332,13 +334,14 @@ class Context:
         own stream).  A torch stream whose handle is 0 (torch's default stream) maps
         to cudaStreamLegacy, so the work really runs on that stream: a NULL handle
         would select the context's own stream instead."""
-        if stream is None:
-            raw = None
-        elif hasattr(stream, "cuda_stream"):
-            raw = stream.cuda_stream or 0x1  # cudaStreamLegacy
+        raw = getattr(stream, "cuda_stream", None)
+        if raw is not None:
+            raw = raw or 0x1  # cudaStreamLegacy
         else:
             raw = stream or None
-        check(self.L.lc_set_stream(self.h, raw), "lc_set_stream")
+        status = self.L.lc_set_stream(self.h, raw)
+        if status:
+            check(status, "lc_set_stream")
 
     def synchronize(self) -> None:
         check(self.L.lc_synchronize(self.h), "lc_synchronize")
@@ -402,9 +405,10 @@ class Context:
     def rope(self, dtype, out_dtype, layout, q, q_out, n_q_heads, k, k_out, n_kv_heads, pos, freq, m, head_dim,
              rope_dim, scale=1.0, ldq=0, ldq_out=0, ldk=0, ldk_out=0):
         """lc_rope: q and k (either may be None with 0 heads) rotated at pos[row]; strides in elements, 0 = packed."""
-        check(self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k), ldk,
-                             ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale),
-              "lc_rope")
+        status = self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k),
+                                ldk, ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale)
+        if status:
+            check(status, "lc_rope")
 
     def activation(self, gate, up, h, n):
         check(self.L.lc_activation(self.h, ptr(gate), ptr(up), ptr(h), n), "lc_activation")
@@ -429,16 +433,20 @@ class Context:
     def prefix_attn(self, dtype, out_dtype, q, kv, out, rows, n_q_heads, n_kv_heads, head_dim, scale, causal=1, ldq=0,
                     ldo=0):
         """lc_prefix_attn with a PrefixKV; strides in elements, 0 = packed."""
-        check(self.L.lc_prefix_attn(self.h, dtype, out_dtype, ptr(q), ldq, C.byref(kv), ptr(out), ldo, rows, n_q_heads,
-                                    n_kv_heads, head_dim, scale, causal), "lc_prefix_attn")
+        status = self.L.lc_prefix_attn(self.h, dtype, out_dtype, ptr(q), ldq, C.byref(kv), ptr(out), ldo, rows,
+                                       n_q_heads, n_kv_heads, head_dim, scale, causal)
+        if status:
+            check(status, "lc_prefix_attn")
 
     def argmax_rows(self, logits, m, n, row_offset, keys):
         check(self.L.lc_argmax_rows(self.h, ptr(logits), m, n, row_offset, ptr(keys)), "lc_argmax_rows")
 
     def logits_process(self, logits, rules, out, keys, m, n, row_offset=0, ld=0, ld_out=0):
         """lc_logits_process with a LogitsRules; out (or keys) may be None; strides in floats, 0 = n."""
-        check(self.L.lc_logits_process(self.h, ptr(logits), ld, ptr(out), ld_out, m, n, row_offset, C.byref(rules),
-                                       ptr(keys)), "lc_logits_process")
+        status = self.L.lc_logits_process(self.h, ptr(logits), ld, ptr(out), ld_out, m, n, row_offset, C.byref(rules),
+                                          ptr(keys))
+        if status:
+            check(status, "lc_logits_process")
 
     def check_bounded_wait(self, spins: int = 1024) -> None:
         check(self.L.lc_check_bounded_wait(self.h, spins), "lc_check_bounded_wait")
