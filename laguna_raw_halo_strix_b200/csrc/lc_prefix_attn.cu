@@ -81,10 +81,9 @@ struct PaArgs {
     // sequences, the rest rows of one sequence over [seq_from, end) of the
     // virtual axis
     int prefix_items, row_tiles, prefix_keys;
-    int chunk, chunk_pairs;  // prefix and sequence items alternate in chunks, chunk_pairs times
     int prefix_splits, seq_splits, seq_keys, seq_from, seq_lanes;
     int seq_base;  // n_kv * n_seqs * seq_lanes
-    PaDiv by_chunk, by_rest, by_heads, by_seqs, by_tiles;  // chunk, seq_base - direct, n_kv, n_seqs, row_tiles
+    PaDiv by_rest, by_heads, by_seqs, by_tiles;  // seq_base - direct, n_kv, n_seqs, row_tiles
     // The first `direct` sequence items run over the whole axis and write out (their
     // rows' first state says so: l = -1); merge: the others leave states
     int direct, merge;
@@ -134,18 +133,8 @@ struct PaItem {
 // at, so that they can be under way while the last item's copies are waited for.
 __device__ __forceinline__ PaItem pa_item_begin(const PaArgs &a, int i) {
     PaItem t;
-    // prefix and sequence items in turn, a chunk of each, while there are both
-    bool prefix;
-    if (i < 2 * a.chunk_pairs * a.chunk) {
-        int in = i;
-        const int q = a.by_chunk(in);
-        prefix = !(q & 1);
-        i = (q >> 1) * a.chunk + in;
-    } else {
-        i -= a.chunk_pairs * a.chunk;
-        prefix = i < a.prefix_items;
-        if (!prefix) i -= a.prefix_items - a.chunk_pairs * a.chunk;
-    }
+    const bool prefix = i < a.prefix_items;
+    if (!prefix) i -= a.prefix_items;
     // sequence items: the direct ones, then the splits of the rest
     t.direct = !prefix && i < a.direct;
     int sp = 0;
@@ -976,14 +965,7 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
     a.merge = a.direct < a.seq_base || !tiles;
     auto div = [](int d) { return PaDiv{((1ull << 63) + d - 1) / d, d}; };
     a.by_rest = div(std::max(1, a.seq_base - a.direct));
-    a.by_heads = div(a.n_kv), a.by_seqs = div(a.n_seqs), a.by_tiles = div(a.row_tiles), a.by_chunk = div(num_sms);
-    // Prefix items lean on the tensor cores and sequence items on memory, so they
-    // alternate (a CTA of each per SM), unless those of the prefix are much longer:
-    // then they come first, as the others even out the end.
-    a.chunk = num_sms;
-    a.chunk_pairs = a.prefix_keys > 2 * a.seq_keys
-                        ? 0
-                        : (int)std::min<int64_t>(a.prefix_items, (int64_t)a.seq_base * a.seq_splits) / a.chunk;
+    a.by_heads = div(a.n_kv), a.by_seqs = div(a.n_seqs), a.by_tiles = div(a.row_tiles);
 }
 
 template <class T, class TO, int HD>
