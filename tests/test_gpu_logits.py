@@ -204,3 +204,95 @@ def test_two_streams_and_graph_replay(ctx, dev):
     del graph
     for c in ctxs:
         c.close()
+
+
+@pytest.mark.parametrize("m,n,hist,bias,masks", [(450, 7, 5, 2, 3), (700, 1500, 60, 10, 2), (460, 4097, 0, 20, 460),
+                                                 (450, 9001, 30, 150, 1), (300, 20000, 100, 0, 0), (130, 50021, 300, 40, 2),
+                                                 (20, 128256, 2000, 200, 3), (450, 8192, 3000, 5, 0)])
+def test_many_rows(ctx, dev, m, n, hist, bias, masks):
+    """More rows than the device takes at a time: lists of each row ahead of its logits, and in the last two
+    sizes more tokens in one place than are kept."""
+    rng = np.random.default_rng(m + n)
+    x = (4 * rng.standard_normal((m, n))).astype(np.float32)
+    check(ctx, dev, x, make(rng, m, n, hist, bias, masks))
+
+
+@pytest.mark.parametrize("n,ld,shift,offset", [(4099, 4100, 0, 0), (4101, 4103, 3, 16032), (6000, 6000, 0, 33)])
+@pytest.mark.parametrize("in_place,keys,out", [(True, True, True), (False, False, True), (False, True, False)])
+def test_many_rows_strides_and_shards(ctx, dev, n, ld, shift, offset, in_place, keys, out):
+    rng = np.random.default_rng(n + offset)
+    x = (4 * rng.standard_normal((500, n))).astype(np.float32)
+    d = make(rng, 500, n, 40, 10, 7, offset=offset, vocab=offset + 2 * n)
+    check(ctx, dev, x, d, offset=offset, ld=ld, shift=shift, in_place=in_place, keys=keys, out=out)
+
+
+def test_many_rows_of_a_long_vocabulary(ctx, dev):
+    """A CTA with more slices than groups of tokens kept for them."""
+    import torch
+
+    m, n = 444, 140000
+    rng = np.random.default_rng(8)
+    x = torch.randn(m, n, device=dev)
+    d = make(rng, m, n, 300, 30, 2)
+    out, keys = torch.empty_like(x), torch.empty(m, dtype=torch.int64, device=dev)
+    ctx.logits_process(x, to_gpu(d, dev), out, keys, m, n)
+    torch.cuda.synchronize()
+    for r in (0, 1, 200, 443):
+        one = {k: v[r:r + 1] for k, v in d.items() if k in ("gen_start", "repetition", "frequency", "presence", "mask_row")}
+        one |= {k: d[k] for k in ("hist", "bias_tok", "bias", "mask")}
+        one |= {k: d[k][r:r + 2] for k in ("hist_start", "bias_start")}
+        ref, _, best = logits_ref.process(x[r:r + 1].cpu().numpy(), **one)
+        assert np.array_equal(out[r].cpu().numpy().view(np.uint32), ref[0].view(np.uint32))
+        assert lc.key_index(int(keys[r])) == best[0]
+
+
+def test_many_rows_special_values(ctx, dev):
+    """Rows of the order's lowest value, of -inf and of NaN among ordinary ones."""
+    import torch
+
+    m, n = 450, 5000
+    x = torch.zeros(m, n, device=dev)
+    x[1] = -float("inf")
+    x[2].view(torch.int32)[:] = -1
+    x[3, 17] = float("nan")
+    x[449, 3] = 1.0
+    out, keys = torch.empty_like(x), torch.empty(m, dtype=torch.int64, device=dev)
+    ctx.logits_process(x, lc.LogitsRules(), out, keys, m, n)
+    torch.cuda.synchronize()
+    assert torch.equal(out.view(torch.int32), x.view(torch.int32))
+    at = [lc.key_index(int(k)) for k in keys.cpu()]
+    assert at[1] == n - 1 and at[2] == n - 1 and at[3] == 17 and at[449] == 3 and at[4] == n - 1
+
+
+def test_captured_calls_of_many_rows_on_two_streams(ctx, dev):
+    """Replays side by side, and a list that grew between them."""
+    import torch
+
+    rng = np.random.default_rng(9)
+    m, n = 460, 9000
+    x = (4 * rng.standard_normal((m, n))).astype(np.float32)
+    d = make(rng, m, n, 60, 10, 2)
+    d["hist_start"][m] -= 7
+    xd, rules = torch.from_numpy(x).to(dev), to_gpu(d, dev)
+    streams, ctxs = [torch.cuda.Stream(), torch.cuda.Stream()], [lc.Context(0), lc.Context(0)]
+    outs = [torch.empty_like(xd) for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for c, s, o in zip(ctxs, streams, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            c.set_stream(s)
+            c.logits_process(xd, rules, o, None, m, n)
+        graphs.append(g)
+    for grow in (0, 7):
+        d["hist_start"][m] += grow
+        rules.held[1].copy_(torch.from_numpy(d["hist_start"]))
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        ref, _, _ = logits_ref.process(x, **d)
+        for o in outs:
+            assert np.array_equal(o.cpu().numpy().view(np.uint32), ref.view(np.uint32))
