@@ -265,7 +265,8 @@ typedef struct {
  * 0..rows (values outside are held inside); rows of no sequence stay as they
  * are in out.  Lengths and starts are read on the device, so a captured call
  * can be replayed as sequences grow up to own_cap.  head_dim 64 or 128, scale
- * positive, at most 128 query heads to a KV head, ldq / ldo elements between rows (0: packed), 16-byte aligned rows.
+ * positive, at most 128 query heads to a KV head, ldq / ldo elements between
+ * rows (0: packed), 16-byte aligned rows.
  * Partial states live in the context's scratch: graphs captured on one context
  * are not replayed at the same time, and capture needs a call of the same size
  * before it.  The reference attends one sequence at a time
