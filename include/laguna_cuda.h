@@ -258,7 +258,9 @@ typedef struct {
  * and its sequence's own rows, the query heads of a group sharing a KV head.  A
  * sequence of c query rows holds its last c own positions: with causal, row t
  * of it sees own rows 0 .. own_len - c + t (none where that is negative),
- * without, all own_len.  A row that sees no key gets 0.  The prefix's products
+ * without, all own_len.  A row that sees no key gets 0.  Own rows behind own_len
+ * may hold anything; a row of v that only some rows of its sequence see has to
+ * be finite, for the others multiply it by 0.  The prefix's products
  * are formed once for the batch.  q, k, v are of type dtype (LC_F16 or LC_BF16),
  * out of that type or LC_F32; softmax and sums in f32, weights rounded to dtype
  * (to twice its digits for LC_F32 outputs).  seq_start is non-decreasing within

@@ -50,7 +50,8 @@ template <int HD>
 struct PaSmem {
     static constexpr uint32_t kTile = HD / 64 * kPaKvPlane;
     static constexpr uint32_t kQ = 0, kK = HD / 64 * kPaPlane, kV = kK + 2 * kTile, kBar = kV + 2 * kTile;
-    static constexpr uint32_t kSched = kBar + 128, kJobs = kSched + 48, kRed = kJobs + 128;  // kRed: maxima [2][kPaRows], sums [2][kPaRows]
+    // kRed: maxima [2][kPaRows], sums [2][kPaRows]
+    static constexpr uint32_t kSched = kBar + 128, kJobs = kSched + 48, kRed = kJobs + 128;
     static constexpr uint32_t kBytes = kRed + 4 * kPaRows * 4 + 1024;  // + slack to 1024-align the base
 };
 
@@ -536,8 +537,10 @@ __global__ void __launch_bounds__(kPaThreads, 2)
             PaJob last = {};
             last.n = -1;
             jobs.put(wait, last);
-            if (!wait.ok)  // copies of this CTA still in flight
+            if (!wait.ok) {  // copies of this CTA still in flight, and the last answer
                 for (uint32_t t = it > 2 ? it - 2 : 0; t <= it; t++) mbar_wait(k_full + (t & 1), (t >> 1) & 1);
+                mbar_wait(sched.bar(), (sched.got - 1) & 1);
+            }
         }
     } else if (warp == kPaValueWarp) {  // ---- V
 #pragma unroll 1
@@ -830,6 +833,8 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
     const size_t at = (size_t)hk * a.row_blocks + blk;
     const float2 *ml = a.ml_part + at * 32 + lane;
     const float4 *op = reinterpret_cast<const float4 *>(a.o_part + at * (32 * HD)) + piece * 64 + lane;
+    // rows written already (without direct items not worth a round trip of its own)
+    if (a.direct && ml[0].y < 0.f) return;
     // a batch's (m, l) and pieces in one round trip; the sums move to its maximum
     float M = -INFINITY, sum = 0.f, o[8] = {};
 #pragma unroll 1
@@ -843,7 +848,7 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
             x[u][0] = op[s * stride * (8 * HD)];
             x[u][1] = op[s * stride * (8 * HD) + 32];
         }
-        if (s0 == 0 && (st[0].y < 0.f || tok < first || tok >= last)) return;  // written already, or of no sequence
+        if (tok < first || tok >= last) return;  // of no sequence
         float top = M;
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
@@ -973,8 +978,7 @@ int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const PaMaps &maps) {
     auto kernel = prefix_attn_kernel<T, TO, HD>;
     if (items) {
         if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
-        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(
-            maps, a);
+        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(maps, a);
     }
     if (a.merge) {
         cudaLaunchConfig_t cfg = {};
