@@ -429,6 +429,11 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     // TMEM columns of S: two stages of 64; a warp's planes of 16 columns overwrite its
     // own 32 scores, and the third, where there is one, takes the second stage's place
     constexpr int kStages = kPlanes < 3 ? 2 : 1;
+    // Tiles whose products are summed in TMEM.  The tensor cores' f32 sums drop what lies
+    // below the last bit, 1.7e-8 of O a product, so for f32 outputs O is added to a sum in
+    // memory after that many (998 rows of 8 heads on 5884 + 431 bf16 keys: 9e-7 off and
+    // 238 us; with 25 tiles in one sum 5.3e-6 and 212 us)
+    constexpr int kRun = kPlanes > 1 ? 4 : 1 << 30;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBar);
@@ -633,7 +638,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                         const uint32_t p = ps + (s >> 1) * 32 + (s & 1) * 8;
                         const uint64_t v = vd + ((s * 2048) >> 4);
                         constexpr uint32_t id = pa_idesc<T>(HD, true);
-                        umma_f16_ts(tbase + kPaColO, p, v, id, (i | s) ? 1u : 0u);
+                        umma_f16_ts(tbase + kPaColO, p, v, id, (i % kRun | s) ? 1u : 0u);
                         if constexpr (kPlanes > 1) umma_f16_ts(tbase + kPaColO, p + 16, v, id, 1u);
                         if constexpr (kPlanes > 2)
                             umma_f16_ts(tbase + kPaColO, tbase + kPaColS + 64 + 8 * s, v, id, 1u);
@@ -672,6 +677,27 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                 const bool busy = 32 * quarter < j.count * a.group;
                 float m_ref = -INFINITY;
                 float2 l = make_float2(0.f, 0.f);
+                // O so far, in the place of the row's state, with the maximum m_run
+                float m_run = -INFINITY;
+                bool run = false;
+                auto state_at = [&]() {  // the row's half of its state: 4 columns are 128 floats on
+                    const int gq = j.first * a.group + row;
+                    const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks + (gq >> 5);
+                    return a.o_part + blk * (32 * HD) + (gq & 31) * 4 + half * (HD * 16);
+                };
+                auto out_at = [&]() {  // the row's half of its result
+                    const int gq = j.first * a.group + row, tok = j.first + pa_token(a, row);
+                    return static_cast<TO *>(a.out) + (size_t)tok * a.ldo +
+                           (size_t)(j.hk * a.group + gq - tok * a.group) * HD + half * (HD / 2);
+                };
+                auto add_run = [&](const float *p, float (&o)[16]) {  // 16 columns of it to those of TMEM
+                    const float f = m_run == m_ref ? 1.f : exp2_fast(m_run - m_ref);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 b = *reinterpret_cast<const float4 *>(p + e * 32);
+                        o[e] += b.x * f, o[e + 1] += b.y * f, o[e + 2] += b.z * f, o[e + 3] += b.w * f;
+                    }
+                };
 #pragma unroll 1
                 for (int i = 0; i < n; i++, it++) {
                     int key, nk;
@@ -682,6 +708,28 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     if (busy) {
                         const uint32_t st = ts + (it & (kStages - 1)) * kPaKeys + kPaHalf * half;
                         tc_fence_after();
+                        if (kPlanes > 1 && i && i % kRun == 0) {
+                            tile_done(pv_done, it - 1);
+                            __syncwarp();
+                            tc_fence_after();
+                            const bool real = row < j.count * a.group;
+                            float *part = state_at();
+#pragma unroll 1
+                            for (int c = 0; c < HD / 2; c += 16, part += 16 * 32) {
+                                float o[16];
+                                tmem_ld16(to + c, o);
+                                tmem_ld_wait();
+                                tmem_regs_ready(o);
+                                if (real) {
+                                    if (run) add_run(part, o);
+#pragma unroll
+                                    for (int e = 0; e < 16; e += 4)
+                                        pa_store4(part + e * 32, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                                }
+                                __syncwarp();
+                            }
+                            m_run = m_ref, run = true;
+                        }
                         // keys [0, lim) of this half are visible to the row
                         int lim = nk;
                         if (own && a.causal)
@@ -710,7 +758,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             pa_meet(quarter);
                             const float m_new = fmaxf(m_ref, fmaxf(top, *other));
                             const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
-                            if (i) {
+                            if (i % kRun) {
                                 tile_done(pv_done, it - 1);
                                 __syncwarp();
                                 tc_fence_after();
@@ -757,26 +805,26 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                     pa_meet(quarter);
                     const float sum = l.x + l.y + other[2 * kPaRows];
                     const bool real = row < j.count * a.group;
-                    const int tok = j.first + pa_token(a, row), gq = j.first * a.group + row;
                     if (n) {
                         tile_done(pv_done, it - 1);
                         __syncwarp();
                         tc_fence_after();
                     }
-                    const size_t blk = (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks;
+                    float2 *ml = a.ml_part + (size_t)(j.split * a.n_kv + j.hk) * a.row_blocks * 32 + j.first * a.group + row;
                     if (j.direct) {
-                        if (real && half == 0 && a.merge) a.ml_part[blk * 32 + gq] = make_float2(0.f, -1.f);
+                        if (real && half == 0 && a.merge) *ml = make_float2(0.f, -1.f);
                         const bool none = n == 0 || sum == 0.f;  // no visible key: 0
                         const float f = none ? 0.f : 1.f / sum;
-                        TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo +
-                                  (size_t)(j.hk * a.group + gq - tok * a.group) * HD + half * (HD / 2);
+                        const float *part = kPlanes > 1 && run ? state_at() : nullptr;
+                        TO *out = out_at();
 #pragma unroll 1
-                        for (int c = 0; c < HD / 2; c += 16, out += 16) {
+                        for (int c = 0; c < HD / 2; c += 16, out += 16, part += 16 * 32) {
                             float o[16];
                             tmem_ld16(to + c, o);  // without a tile whatever is there, and not used
                             tmem_ld_wait();
                             tmem_regs_ready(o);
                             if (real) {
+                                if (kPlanes > 1 && run) add_run(part, o);
 #pragma unroll
                                 for (int e = 0; e < 16; e++) o[e] = none ? 0.f : o[e] * f;
                                 pa_store16(out, o);
@@ -784,17 +832,18 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             __syncwarp();
                         }
                     } else {
-                        if (real && half == 0) a.ml_part[blk * 32 + gq] = make_float2(m_ref, sum);
-                        float *part = a.o_part + (blk + (gq >> 5)) * (32 * HD) + (gq & 31) * 4 + half * (HD * 16);
+                        if (real && half == 0) *ml = make_float2(m_ref, sum);
+                        float *part = state_at();
 #pragma unroll 1
-                        for (int c = 0; c < HD / 2 && n; c += 32, part += 32 * 32) {
-                            float o[32];
-                            tmem_ld32(to + c, o);
+                        for (int c = 0; c < HD / 2 && n; c += 16, part += 16 * 32) {
+                            float o[16];
+                            tmem_ld16(to + c, o);
                             tmem_ld_wait();
                             tmem_regs_ready(o);
                             if (real) {
+                                if (kPlanes > 1 && run) add_run(part, o);
 #pragma unroll
-                                for (int e = 0; e < 32; e += 4)
+                                for (int e = 0; e < 16; e += 4)
                                     pa_store4(part + e * 32, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
                             }
                             __syncwarp();
@@ -1072,7 +1121,7 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     const int64_t items = a.prefix_items + a.direct + (int64_t)(a.seq_base - a.direct) * a.seq_splits;
     // (a CTA that skips empty items must not keep its other warps waiting past their bound)
     LC_REQUIRE(items <= kPaMaxItems, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
-    if (a.merge) {
+    if (a.merge || out_dtype == LC_F32) {  // (items that write out sum long rows there too)
         a.row_blocks = div_up((int64_t)rows * a.group, 32);
         const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;
         void *scr = nullptr;

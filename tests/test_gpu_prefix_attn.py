@@ -310,3 +310,34 @@ def test_repeats_bit_for_bit(ctx, dev):
         b.run(ctx)
     torch.cuda.synchronize()
     assert torch.equal(first, b.out)
+
+
+@pytest.mark.parametrize("src", ["bf16", "f16"])
+@pytest.mark.parametrize("n_q,n_kv,hd,counts,lens,prefix,cap", [
+    (8, 2, 64, [343, 262, 393], [396, 262, 393], 5884, 431),     # states of many tiles
+    (32, 8, 128, [343, 262, 393, 500], [396, 262, 393, 500], 1500, 512),  # rows written out by whole items
+])
+def test_long_sums_keep_their_digits(ctx, dev, src, n_q, n_kv, hd, counts, lens, prefix, cap):
+    """f32 outputs: the tensor cores drop what lies below a sum's last bit, 2^-24 of it on the average, and at
+    most 48 products (4 tiles of 64 keys, 16 at a time, in 3 planes) are summed there; scores, exponentials and
+    planes of the weights add up to 4 times 2^-22.  All of the result's norm."""
+    import torch
+
+    b = Batch(dev, src, "f32", n_q, n_kv, hd, prefix, cap, counts, lens, seed=4)
+    b.run(ctx)
+    torch.cuda.synchronize()
+    at, err, norm = 0, 0.0, 0.0
+    for i, (c, length) in enumerate(zip(counts, lens)):
+        k = torch.cat([b.kp[:prefix], b.ko[i, :length]]).double().view(-1, n_kv, hd)
+        v = torch.cat([b.vp[:prefix], b.vo[i, :length]]).double().view(-1, n_kv, hd)
+        hidden = torch.ones(c, length, dtype=torch.bool, device=dev).triu(length - c + 1)
+        hidden = torch.cat([torch.zeros(c, prefix, dtype=torch.bool, device=dev), hidden], 1)
+        for h in range(n_kv):
+            group = n_q // n_kv
+            q = b.q[at:at + c].double().view(c, n_kv, group, hd)[:, h]
+            s = torch.einsum("rgd,kd->grk", q, k[:, h]) * b.scale
+            o = torch.einsum("grk,kd->rgd", s.masked_fill(hidden, -math.inf).softmax(-1), v[:, h])
+            got = b.out[at:at + c].double().view(c, n_kv, group, hd)[:, h]
+            err, norm = err + float((got - o).square().sum()), norm + float(o.square().sum())
+        at += c
+    assert math.sqrt(err / norm) <= 48 * 2.0 ** -24 + 4 * 2.0 ** -22
