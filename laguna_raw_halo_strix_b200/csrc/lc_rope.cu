@@ -6,7 +6,7 @@
 // the remaining dims are copied.  The angle of a far position needs more than
 // 24 bits (pos 1e6 at freq 1 is 0.06 rad off in f32): the product of two
 // numbers of at most 31 and 24 bits is exact to 2^-53 in a double, and is
-// reduced mod 2 pi there; sincosf then sees |a| <= pi.  The rotation itself is
+// reduced mod 2 pi there; sincospif then sees |a| <= pi.  The rotation itself is
 // f32 with one rounding to the output type.
 //
 // Bound by the bytes of x and y.  One CTA takes some rows (or a share of one
@@ -24,8 +24,7 @@ namespace {
 
 constexpr int kRpThreads = 128;
 // Items a thread has in flight (and loads before the table is ready): 8192 rows of
-// 40 bf16 heads take 37 us with two in 8 CTAs an SM, 54 us with four in registers
-// for 2 CTAs of 256 threads, 65 us with one in 16.
+// 40 bf16 heads take 36 us with two in 8 CTAs an SM, 41 us with three in 6.
 constexpr int kRpItems = 2;
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 
@@ -96,10 +95,9 @@ struct RpArgs {
     int same[2];              // y is x: dims past rope_dim stay as they are
     int n_q, n_heads;         // heads of q, of q and k together
     int head_dim, rope_dim;
-    int rot, items;           // rotated items of a head, all items of a head
+    int rot, items, lanes;    // rotated items of a head, all items of a head, those side by side in a CTA
     int heads_per_cta, rows_per_cta;
     uint32_t m;
-    uint64_t inv_items, inv_row;  // ceil(2^63 / d) of items and of a CTA's items in a row: exact quotients below 2^31
     const int32_t *pos;
     const float *freq;
     float scale;
@@ -112,39 +110,38 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
     extern __shared__ float2 cs_rows[];  // [rows][rope_dim / 2]
     const size_t row0 = (size_t)blockIdx.x * a.rows_per_cta;
     const int rows = (int)min((size_t)a.rows_per_cta, a.m - row0);
-    const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.n_heads, h0 + a.heads_per_cta);
-    const int per_row = (h1 - h0) * a.items, total = rows * per_row, half = a.rope_dim >> 1;
-
-    auto place = [&](int idx, int &in, int &t, int &head, int &item) {
-        in = rows == 1 ? 0 : (int)__umul64hi((uint64_t)idx << 1, a.inv_row);
-        idx -= in * per_row;
-        const int h = (int)__umul64hi((uint64_t)idx << 1, a.inv_items);
-        item = idx - h * a.items;
-        t = h0 + h >= a.n_q;
-        head = h0 + h - (t ? a.n_q : 0);
+    const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.n_heads, h0 + a.heads_per_cta) - h0;
+    const int half = a.rope_dim >> 1;
+    // A thread keeps its item (one of `lanes` side by side) and goes over (row, head)
+    // pairs `sides` apart, rows first in steps of whole rows and rest heads.
+    const int lanes = a.lanes, sides = kRpThreads / lanes, side = threadIdx.x / lanes;
+    const int step_rows = sides / nh, step_heads = sides - step_rows * nh;
+    auto step = [&](int &in, int &h) {
+        in += step_rows, h += step_heads;
+        if (h >= nh) h -= nh, in++;
     };
-    auto first = [&](int item) { return item < a.rot ? item * V : a.rope_dim + (item - a.rot) * V; };
-    auto load = [&](int idx, RpPack<TI, V> &p0, RpPack<TI, V> &p1) {
-        int in, t, head, item;
-        place(idx, in, t, head, item);
-        const TI *x = static_cast<const TI *>(t ? a.x[1] : a.x[0]) + (row0 + in) * (t ? a.ldx[1] : a.ldx[0]) +
-                      (size_t)head * a.head_dim + first(item);
-        if (item >= a.rot && (t ? a.same[1] : a.same[0])) return;
-        p0 = rp_load<TI, V, VEC>(x);
-        if (!PAIRS && item < a.rot) p1 = rp_load<TI, V, VEC>(x + half);
+    int item = threadIdx.x - side * lanes;
+    int in_head;  // the item's first dim (a row's heads are below 2^30 elements)
+    auto take_item = [&]() { in_head = item < a.rot ? item * V : a.rope_dim + (item - a.rot) * V; };
+    auto load = [&](int in, int h, RpPack<TI, V> &p0, RpPack<TI, V> &p1) {
+        const bool k = h0 + h >= a.n_q;
+        const TI *from = static_cast<const TI *>(k ? a.x[1] : a.x[0]) + (row0 + in) * (k ? a.ldx[1] : a.ldx[0]) +
+                         ((h0 + h - (k ? a.n_q : 0)) * a.head_dim + in_head);
+        if (item >= a.rot && (k ? a.same[1] : a.same[0])) return;
+        p0 = rp_load<TI, V, VEC>(from);
+        if (!PAIRS && item < a.rot) p1 = rp_load<TI, V, VEC>(from + half);
     };
-    auto finish = [&](int idx, const RpPack<TI, V> &p0, const RpPack<TI, V> &p1) {
-        int in, t, head, item;
-        place(idx, in, t, head, item);
-        TO *y = static_cast<TO *>(t ? a.y[1] : a.y[0]) + (row0 + in) * (t ? a.ldy[1] : a.ldy[0]) +
-                (size_t)head * a.head_dim + first(item);
+    auto finish = [&](int in, int h, const RpPack<TI, V> &p0, const RpPack<TI, V> &p1) {
+        const bool k = h0 + h >= a.n_q;
+        TO *to = static_cast<TO *>(k ? a.y[1] : a.y[0]) + (row0 + in) * (k ? a.ldy[1] : a.ldy[0]) +
+                 ((h0 + h - (k ? a.n_q : 0)) * a.head_dim + in_head);
         const float2 *cs = cs_rows + in * half;
         float o0[V], o1[V];
         if (item >= a.rot) {
-            if (t ? a.same[1] : a.same[0]) return;
+            if (k ? a.same[1] : a.same[0]) return;
 #pragma unroll
             for (int i = 0; i < V; i++) o0[i] = rp_f32(p0.v[i]);
-            rp_store<TO, V, VEC>(y, o0);
+            rp_store<TO, V, VEC>(to, o0);
         } else if constexpr (PAIRS) {
 #pragma unroll
             for (int i = 0; i + 1 < V; i += 2) {
@@ -153,7 +150,7 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
                 o0[i] = u * c.x - w * c.y;
                 o0[i + 1] = w * c.x + u * c.y;
             }
-            rp_store<TO, V, VEC>(y, o0);
+            rp_store<TO, V, VEC>(to, o0);
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -162,15 +159,20 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
                 o0[i] = u * c.x - w * c.y;
                 o1[i] = w * c.x + u * c.y;
             }
-            rp_store<TO, V, VEC>(y, o0);
-            rp_store<TO, V, VEC>(y + half, o1);
+            rp_store<TO, V, VEC>(to, o0);
+            rp_store<TO, V, VEC>(to + half, o1);
         }
     };
 
     RpPack<TI, V> p0[kRpItems], p1[kRpItems];
+    const int in0 = side < sides ? side / nh : rows, first_h = side - side / nh * nh;
+    int in = in0, h = first_h;  // of the next load
+    take_item();
 #pragma unroll
-    for (int j = 0; j < kRpItems; j++)
-        if ((int)threadIdx.x + j * kRpThreads < total) load(threadIdx.x + j * kRpThreads, p0[j], p1[j]);
+    for (int j = 0; j < kRpItems; j++) {
+        if (in < rows) load(in, h, p0[j], p1[j]);
+        step(in, h);
+    }
     if (half) {
         for (int i = threadIdx.x; i < rows * half; i += kRpThreads) {
             const int in = i / half;
@@ -183,14 +185,28 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
         }
         __syncthreads();
     }
-    for (int base = threadIdx.x; base < total;) {
+    while (true) {
+        for (int fin = in0, fh = first_h; fin < rows;) {
 #pragma unroll
-        for (int j = 0; j < kRpItems; j++)
-            if (base + j * kRpThreads < total) finish(base + j * kRpThreads, p0[j], p1[j]);
-        base += kRpItems * kRpThreads;
+            for (int j = 0; j < kRpItems; j++) {
+                if (fin < rows) finish(fin, fh, p0[j], p1[j]);
+                step(fin, fh);
+            }
 #pragma unroll
-        for (int j = 0; j < kRpItems; j++)
-            if (base + j * kRpThreads < total) load(base + j * kRpThreads, p0[j], p1[j]);
+            for (int j = 0; j < kRpItems; j++) {
+                if (in < rows) load(in, h, p0[j], p1[j]);
+                step(in, h);
+            }
+        }
+        item += lanes;  // heads of more items than threads
+        if (item >= a.items) break;
+        take_item();
+        in = in0, h = first_h;
+#pragma unroll
+        for (int j = 0; j < kRpItems; j++) {
+            if (in < rows) load(in, h, p0[j], p1[j]);
+            step(in, h);
+        }
     }
 }
 
@@ -233,8 +249,7 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
            (a.rows_per_cta + 1) * table <= 32 * 1024)
         a.rows_per_cta++;
     a.m = m;
-    auto inv = [](uint64_t d) { return ((1ull << 63) + d - 1) / d; };
-    a.inv_items = inv(a.items), a.inv_row = inv((uint64_t)a.heads_per_cta * a.items);
+    a.lanes = std::min(a.items, kRpThreads);
     const dim3 grid((m + a.rows_per_cta - 1) / a.rows_per_cta, splits);
     const size_t smem = a.rows_per_cta * table;
     auto go = [&](auto kernel) -> int {
