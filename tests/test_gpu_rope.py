@@ -174,3 +174,42 @@ def test_offsets_past_32_bits(ctx, dev):
     torch.cuda.synchronize()
     ref, mag = reference(x, pos.cpu().numpy(), freq.cpu().numpy(), 1, hd, hd, False, 1.0)
     within(rows, ref, mag, "bf16")
+
+
+@pytest.mark.parametrize("m,n_q,n_kv,hd,rd", [(5, 1, 1, 1022, 1022), (700, 3, 1, 600, 598), (2, 2, 1, 8192, 8192),
+                                              (1500, 1, 0, 4, 2), (650, 5, 0, 254, 10), (3, 300, 7, 6, 4)])
+@pytest.mark.parametrize("src,dst", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_items_and_threads_that_do_not_divide(ctx, dev, m, n_q, n_kv, hd, rd, src, dst, pairs):
+    """Heads of more pieces than a CTA has threads, and few pieces with threads left over."""
+    test_against_64_bits(ctx, dev, m, n_q, n_kv, hd, rd, src, dst, pairs)
+
+
+def test_first_call_of_a_process_captured():
+    """Neither lc_rope nor lc_logits_process needs a call before its capture."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from laguna_raw_halo_strix_b200 import lc
+d = torch.device("cuda", 0)
+x = torch.randn(2, 128, device=d); y = torch.zeros_like(x); l = torch.randn(3, 5000, device=d)
+big = torch.randn(500, 5000, device=d)
+pos = torch.arange(2, dtype=torch.int32, device=d); freq = torch.from_numpy(lc.rope_freq(64)).to(d)
+keys, all_keys = torch.zeros(3, dtype=torch.int64, device=d), torch.zeros(500, dtype=torch.int64, device=d)
+s = torch.cuda.Stream(); ctx = lc.Context(0); ctx.set_stream(s); g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=s):
+    ctx.rope(lc.F32, lc.F32, lc.ROPE_HALF, x, y, 2, None, None, 0, pos, freq, 2, 64, 64)
+    ctx.logits_process(l, lc.LogitsRules(), None, keys, 3, 5000)
+    ctx.logits_process(big, lc.LogitsRules(), None, all_keys, 500, 5000)
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(y[0], x[0]) and not torch.equal(y[1], x[1])
+assert [lc.key_index(int(k)) for k in keys] == l.argmax(1).tolist()
+assert [lc.key_index(int(k)) for k in all_keys] == big.argmax(1).tolist()
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
