@@ -950,7 +950,7 @@ int pa_map(CUtensorMap *tm, const void *p, int dtype, const uint64_t (&dims)[3],
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How the work is cut into items.
-void pa_plan(PaArgs &a, int num_sms, int hd) {
+void pa_plan(PaArgs &a, int num_sms, int hd, int planes) {
     const int slots = 2 * num_sms;  // CTAs resident at once
     const int64_t R = (int64_t)a.rows * a.group;
     // Tokens of a row tile: as many as fit 128 rows in whole copies of Q, which hold
@@ -968,8 +968,11 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
     // row tiles of a sequence that run side by side (a longer one goes round again)
     a.seq_lanes = a.n_seqs == 1 ? tiles_all : std::min(tiles_all, tiles_avg > 1 ? 2 * tiles_avg : 1);
     // Splits of the key axis for `base` items of `tiles` tiles: the fewest rounds of tiles
-    // over the resident CTAs (about 1 us a tile and 2 us an item), against writing and
-    // reading the states (8 bytes a picosecond) and the merge's launch.
+    // over the resident CTAs (about 1 us a tile, 0.6 more for a further plane, and 2 us an
+    // item), against writing and reading the states (8 bytes a picosecond), the merge's
+    // launch and its round trips, 8 states each (one row of 4 heads on 10581 keys: 25 us
+    // without that last part, 14 with).
+    const double tile_us = 1.0 + 0.6 * (planes - 1);
     const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 8e6;
     auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
         int best = 1;
@@ -977,7 +980,8 @@ void pa_plan(PaArgs &a, int num_sms, int hd) {
         for (int n = 1; n <= std::min(tiles, 256); n++) {
             const int per = div_up(tiles, n);
             if (n > 1 && div_up(tiles, n - 1) == per) continue;  // the same cut with an empty split more
-            const double us = (per + 2.0) * div_up(base * n, slots) + (n > 1 || merged_anyway ? n * state_us + 4 : 0);
+            const double us = (per * tile_us + 2) * div_up(base * n, slots) +
+                              (n > 1 || merged_anyway ? n * (state_us + 0.09) + 4 : 0);
             if (us < best_us) best = n, best_us = us;
         }
         return best;
@@ -1125,7 +1129,7 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
     a.scale_log2 = scale_log2;
     a.causal = causal != 0;
     a.status = ctx->dev_status;
-    pa_plan(a, ctx->num_sms, (int)head_dim);
+    pa_plan(a, ctx->num_sms, (int)head_dim, out_dtype != LC_F32 ? 1 : dtype == LC_F16 ? 2 : 3);
     const int64_t items = a.prefix_items + a.direct + (int64_t)(a.seq_base - a.direct) * a.seq_splits;
     // (a CTA that skips empty items must not keep its other warps waiting past their bound)
     LC_REQUIRE(items <= kPaMaxItems, LC_ERR_UNSUPPORTED, "lc_prefix_attn: %lld work items", (long long)items);
