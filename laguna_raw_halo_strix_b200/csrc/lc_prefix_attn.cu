@@ -88,6 +88,7 @@ struct PaArgs {
     // The first `direct` sequence items run over the whole axis and write out (their
     // rows' first state says so: l = -1); merge: the others leave states
     int direct, merge;
+    int merge_ways;  // warps that share the states of 32 rows and 8 dims: 1 or 4
     // partial states of row r = token * group + head within the group: O
     // unnormalised as [split][KV head][r / 32][HD / 4][r % 32][4] (32 rows' 16-byte
     // pieces side by side: the lanes of a warp hold neighbouring rows), and (m in
@@ -867,14 +868,17 @@ __global__ void __launch_bounds__(kPaThreads, 2)
 
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits that saw a
 // key, 0 if none did.  One warp per 32 rows of a KV head and 8 dims, a lane per
-// row: the states' pieces are read 512 bytes at a time, 8 splits in flight.
+// row: the states' pieces are read 512 bytes at a time, 8 splits in flight; or the four
+// warps of a block, a share of the splits each.
 // Rows outside [seq_start[0], seq_start[n_seqs]) belong to no sequence and stay
 // as they are.
 template <class TO, int HD>
 __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_constant__ PaArgs a) {
     constexpr int kPer = HD / 8, kBatch = 8;  // warps of a block of rows; splits in flight
     griddep_wait();  // the partial states
-    const int w = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    __shared__ float shares[3][10][32];
+    const int ways = a.merge_ways, way = threadIdx.x / 32 & (ways - 1);
+    const int w = (blockIdx.x * 4 + (threadIdx.x >> 5)) / ways, lane = threadIdx.x & 31;
     const int piece = w % kPer, blk = w / kPer % a.row_blocks, hk = w / kPer / a.row_blocks;
     const int gq = blk * 32 + lane, tok = gq / a.group;
     if (hk >= a.n_kv || gq >= a.rows * a.group) return;
@@ -888,8 +892,9 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
     if (a.direct && ml[0].y < 0.f) return;
     // a batch's (m, l) and pieces in one round trip; the sums move to its maximum
     float M = -INFINITY, sum = 0.f, o[8] = {};
+    const int share = (splits + ways - 1) / ways, end = min(splits, (way + 1) * share);
 #pragma unroll 1
-    for (int s0 = 0; s0 < splits; s0 += kBatch) {
+    for (int s0 = way * share; s0 < end; s0 += kBatch) {
         float2 st[kBatch];
         float4 x[kBatch][2];
 #pragma unroll
@@ -903,7 +908,7 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
         float top = M;
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
-            if (s0 + u >= splits) st[u].y = 0.f;
+            if (s0 + u >= end) st[u].y = 0.f;
             if (st[u].y != 0.f) top = fmaxf(top, st[u].x);
         }
         if (top > M) {
@@ -922,7 +927,31 @@ __global__ void __launch_bounds__(128) prefix_attn_merge_kernel(const __grid_con
                 o[4] += x[u][1].x * f, o[5] += x[u][1].y * f, o[6] += x[u][1].z * f, o[7] += x[u][1].w * f;
             }
     }
-    if (splits == 0 && (tok < first || tok >= last)) return;
+    if (tok < first || tok >= last) return;
+    if (ways > 1) {
+        if (way) {
+            float *to = &shares[way - 1][0][lane];
+            to[0] = M, to[32] = sum;
+#pragma unroll
+            for (int e = 0; e < 8; e++) to[(2 + e) * 32] = o[e];
+        }
+        __syncthreads();
+        if (way) return;
+        float top = M;
+        for (int k = 0; k < ways - 1; k++) top = fmaxf(top, shares[k][0][lane]);
+        const float f = sum != 0.f ? exp2f(M - top) : 0.f;
+        sum *= f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] *= f;
+        for (int k = 0; k < ways - 1; k++) {
+            const float *from = &shares[k][0][lane];
+            if (from[32] == 0.f) continue;
+            const float g = exp2f(from[0] - top);
+            sum += from[32] * g;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] += from[(2 + e) * 32] * g;
+        }
+    }
     const float f = sum != 0.f ? 1.f / sum : 0.f;
     TO *out = static_cast<TO *>(a.out) + (size_t)tok * a.ldo + (size_t)(hk * a.group + gq - tok * a.group) * HD +
               8 * piece;
@@ -974,6 +1003,11 @@ void pa_plan(PaArgs &a, int num_sms, int hd, int planes) {
     // without that last part, 14 with).
     const double tile_us = 1.0 + 0.6 * (planes - 1);
     const double state_us = 2.0 * a.n_kv * div_up(R, 32) * 32 * (hd * 4 + 8) / 8e6;
+    // Few rows leave warps to share their states (4 x 2 rows on 16487 keys: 15.8 us in one
+    // warp, 11.0 in four); more rows fill the merge's warps by themselves (64 sequences of 32
+    // heads on 8192: 47.7 us, with four 48.7).
+    const bool shared_merge = a.n_kv * div_up(R, 32) * (hd / 8) <= 2 * slots;
+    const double split_us = state_us + (shared_merge ? 0.03 : 0.09);
     auto splits_for = [&](int64_t base, int tiles, bool merged_anyway) {
         int best = 1;
         double best_us = 1e30;
@@ -981,7 +1015,7 @@ void pa_plan(PaArgs &a, int num_sms, int hd, int planes) {
             const int per = div_up(tiles, n);
             if (n > 1 && div_up(tiles, n - 1) == per) continue;  // the same cut with an empty split more
             const double us = (per * tile_us + 2) * div_up(base * n, slots) +
-                              (n > 1 || merged_anyway ? n * (state_us + 0.09) + 4 : 0);
+                              (n > 1 || merged_anyway ? n * split_us + 4 : 0);
             if (us < best_us) best = n, best_us = us;
         }
         return best;
@@ -1028,6 +1062,7 @@ void pa_plan(PaArgs &a, int num_sms, int hd, int planes) {
         a.seq_splits = a.direct == a.seq_base ? 1 : div_up(tiles, per);
     }
     a.merge = a.direct < a.seq_base || !tiles;
+    a.merge_ways = shared_merge && a.prefix_splits + a.seq_splits > 8 ? 4 : 1;
     auto div = [](int d) { return PaDiv{((1ull << 63) + d - 1) / d, d}; };
     a.by_rest = div(std::max(1, a.seq_base - a.direct));
     a.by_heads = div(a.n_kv), a.by_seqs = div(a.n_seqs), a.by_tiles = div(a.row_tiles);
@@ -1042,7 +1077,7 @@ int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const PaMaps &maps) {
     }
     if (a.merge) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(div_up((int64_t)a.n_kv * a.row_blocks * (HD / 8), 4));
+        cfg.gridDim = dim3(div_up((int64_t)a.n_kv * a.row_blocks * (HD / 8) * a.merge_ways, 4));
         cfg.blockDim = dim3(128);
         cfg.stream = ctx->stream;
         cudaLaunchAttribute attr[1];

@@ -341,3 +341,14 @@ def test_long_sums_keep_their_digits(ctx, dev, src, n_q, n_kv, hd, counts, lens,
             err, norm = err + float((got - o).square().sum()), norm + float(o.square().sum())
         at += c
     assert math.sqrt(err / norm) <= 48 * 2.0 ** -24 + 4 * 2.0 ** -22
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+@pytest.mark.parametrize("n_q,n_kv,hd,prefix,cap,counts,lens", [
+    (4, 1, 64, 10581, 206, [1], [200]), (2, 2, 128, 13851, 7, [1, 0, 1], [7, 3, 1]), (1, 1, 64, 0, 9000, [3], [8999]),
+    (6, 2, 128, 700, 0, [1, 2], [0, 0])])
+def test_few_rows_on_many_keys(ctx, dev, src, dst, n_q, n_kv, hd, prefix, cap, counts, lens):
+    """Many states of a few rows, merged by several warps together; rows of no sequence among them."""
+    b = Batch(dev, src, dst, n_q, n_kv, hd, prefix, cap, counts, lens, seed=6, extra=3)
+    b.run(ctx)
+    b.check()
