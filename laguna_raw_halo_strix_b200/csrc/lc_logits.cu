@@ -626,7 +626,10 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     // Few rows, a slice a CTA and all at a time, as many CTAs a row as that allows but
     // at least 4096 tokens each (one row of 128256: 7.9 us against 11.5 in the other
     // kernel, 37 of 50021: 9.1 against 12.8; with clusters that wait for others to end
-    // 15.0; 16 rows of 32000 with 2048 each 7.4 us, with 4096 7.2).
+    // 15.0; 16 rows of 32000 with 2048 each 7.4 us, with 4096 7.2).  Rows of one slice
+    // with a history above an eighth of it too, which all of the CTA's threads count then
+    // (512 rows of 4495 with 2000 tokens: 20 against 37; with 50 tokens on 3000, 41 against 24).
+    const bool long_lists = r.hist_len > (uint64_t)m * n / 8;
     uint32_t cl = 1, clusters = 1;
     bool few = false;
     if ((n + 15) / 16 <= kLgRowSlice) {
@@ -635,7 +638,8 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
         for (; (n + cl - 1) / cl <= kLgRowSlice; cl--) {
             int at_a_time = 0;
             if (int s = lg_resident(ctx, 1, cl, &at_a_time)) return s;
-            if ((few = m <= (uint32_t)at_a_time) || cl == 1) break;
+            few = m <= (uint32_t)at_a_time || (cl == 1 && long_lists);
+            if (few || cl == 1) break;
         }
     }
     // Many: the CTAs of a cluster with which they end first.  Clusters of c take

@@ -208,10 +208,11 @@ def test_two_streams_and_graph_replay(ctx, dev):
 
 @pytest.mark.parametrize("m,n,hist,bias,masks", [(450, 7, 5, 2, 3), (700, 1500, 60, 10, 2), (460, 4097, 0, 20, 460),
                                                  (450, 9001, 30, 150, 1), (300, 20000, 100, 0, 0), (130, 50021, 300, 40, 2),
-                                                 (20, 128256, 2000, 200, 3), (450, 8192, 3000, 5, 0)])
+                                                 (20, 128256, 2000, 200, 3), (450, 8192, 3000, 5, 0),
+                                                 (600, 1849, 2000, 3, 2)])
 def test_many_rows(ctx, dev, m, n, hist, bias, masks):
-    """More rows than the device takes at a time: lists of each row ahead of its logits, and in the last two
-    sizes more tokens in one place than are kept."""
+    """More rows than the device takes at a time: lists of each row ahead of its logits, and in some
+    sizes more tokens in one place than are kept, or a history longer than the vocabulary."""
     rng = np.random.default_rng(m + n)
     x = (4 * rng.standard_normal((m, n))).astype(np.float32)
     check(ctx, dev, x, make(rng, m, n, hist, bias, masks))
