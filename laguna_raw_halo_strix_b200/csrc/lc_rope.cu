@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kRpThreads = 128;
 // Items a thread has in flight (and loads before the table is ready): 8192 rows of
-// 40 bf16 heads take 36 us with two in 8 CTAs an SM, 41 us with three in 6.
+// 40 bf16 heads take 36 us with two in 8 CTAs an SM, 41 us with three in 6; more of
+// narrower ones gained nothing.
 constexpr int kRpItems = 2;
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 
@@ -104,8 +105,10 @@ struct RpArgs {
 };
 
 // PAIRS false: an item is V dims at i and the V at i + rope_dim / 2; true: the
-// V / 2 pairs of V neighbouring dims.  Items rot.. are V copied dims.
-template <class TI, class TO, bool PAIRS, int V, bool VEC>
+// V / 2 pairs of V neighbouring dims.  With COPIES, items rot.. are 2 V copied dims, V
+// for the last where as many are left (a kernel of its own, for the copies' code costs
+// rows that are all rotated a quarter of their speed).
+template <class TI, class TO, bool PAIRS, int V, bool VEC, bool COPIES>
 __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
     extern __shared__ float2 cs_rows[];  // [rows][rope_dim / 2]
     const size_t row0 = (size_t)blockIdx.x * a.rows_per_cta;
@@ -122,14 +125,18 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
     };
     int item = threadIdx.x - side * lanes;
     int in_head;  // the item's first dim (a row's heads are below 2^30 elements)
-    auto take_item = [&]() { in_head = item < a.rot ? item * V : a.rope_dim + (item - a.rot) * V; };
+    auto take_item = [&]() { in_head = !COPIES || item < a.rot ? item * V : a.rope_dim + (item - a.rot) * (2 * V); };
     auto load = [&](int in, int h, RpPack<TI, V> &p0, RpPack<TI, V> &p1) {
         const bool k = h0 + h >= a.n_q;
         const TI *from = static_cast<const TI *>(k ? a.x[1] : a.x[0]) + (row0 + in) * (k ? a.ldx[1] : a.ldx[0]) +
                          ((h0 + h - (k ? a.n_q : 0)) * a.head_dim + in_head);
-        if (item >= a.rot && (k ? a.same[1] : a.same[0])) return;
+        if (COPIES && item >= a.rot && (k ? a.same[1] : a.same[0])) return;
         p0 = rp_load<TI, V, VEC>(from);
-        if (!PAIRS && item < a.rot) p1 = rp_load<TI, V, VEC>(from + half);
+        if (COPIES && item >= a.rot) {
+            if (in_head + V < a.head_dim) p1 = rp_load<TI, V, VEC>(from + V);
+        } else if (!PAIRS) {
+            p1 = rp_load<TI, V, VEC>(from + half);
+        }
     };
     auto finish = [&](int in, int h, const RpPack<TI, V> &p0, const RpPack<TI, V> &p1) {
         const bool k = h0 + h >= a.n_q;
@@ -137,11 +144,12 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
                  ((h0 + h - (k ? a.n_q : 0)) * a.head_dim + in_head);
         const float2 *cs = cs_rows + in * half;
         float o0[V], o1[V];
-        if (item >= a.rot) {
+        if (COPIES && item >= a.rot) {
             if (k ? a.same[1] : a.same[0]) return;
 #pragma unroll
-            for (int i = 0; i < V; i++) o0[i] = rp_f32(p0.v[i]);
+            for (int i = 0; i < V; i++) o0[i] = rp_f32(p0.v[i]), o1[i] = rp_f32(p1.v[i]);
             rp_store<TO, V, VEC>(to, o0);
+            if (in_head + V < a.head_dim) rp_store<TO, V, VEC>(to + V, o1);
         } else if constexpr (PAIRS) {
 #pragma unroll
             for (int i = 0; i + 1 < V; i += 2) {
@@ -217,20 +225,26 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     constexpr int V = RpVec<TI>::kN;
     RpArgs a = base;
     const int half = a.rope_dim / 2;
-    // 16-byte input vectors (and the same element count out) where every row,
-    // head and half starts on a multiple of them; single elements otherwise
-    bool vec = a.head_dim % V == 0 && (pairs ? a.rope_dim : half) % V == 0;
-    for (int t = 0; t < 2; t++)
-        if (t ? a.n_heads > a.n_q : a.n_q > 0) {
-            const uintptr_t need_y = V * sizeof(TO) > 16 ? 16 : V * sizeof(TO);
-            vec = vec && (uintptr_t)a.x[t] % 16 == 0 && a.ldx[t] % V == 0 && (uintptr_t)a.y[t] % need_y == 0 &&
-                  a.ldy[t] % V == 0;
-        }
-    const int v = vec ? V : pairs ? 2 : 1;
+    // Vectors of 16 or 8 bytes in, or of two elements, where every row, head and half starts on
+    // a multiple of them (and the same element count out); single elements otherwise
+    // (8192 rows of 8 + 8 bf16 heads of 80 with 20 dims rotated: 25 us in twos, 60 when
+    // they went singly)
+    auto fits = [&](int n) {
+        bool yes = a.head_dim % n == 0 && (pairs ? a.rope_dim : half) % n == 0;
+        for (int t = 0; t < 2; t++)
+            if (t ? a.n_heads > a.n_q : a.n_q > 0) {
+                const uintptr_t need_y = std::min<uintptr_t>(n * sizeof(TO), 16);
+                yes = yes && (uintptr_t)a.x[t] % (n * sizeof(TI)) == 0 && a.ldx[t] % n == 0 &&
+                      (uintptr_t)a.y[t] % need_y == 0 && a.ldy[t] % n == 0;
+            }
+        return yes;
+    };
+    const bool vec = fits(V), halves = fits(V / 2), twos = fits(2);
+    const int v = vec ? V : halves ? V / 2 : twos || pairs ? 2 : 1;
     const bool q_copies = a.n_q > 0 && !a.same[0], k_copies = a.n_heads > a.n_q && !a.same[1];
     // (head_dim and rope_dim are even, so the copied dims divide by 2 as well)
     a.rot = pairs ? a.rope_dim / v : half / v;
-    a.items = a.rot + ((q_copies || k_copies) ? (a.head_dim - a.rope_dim) / v : 0);
+    a.items = a.rot + ((q_copies || k_copies) ? (a.head_dim - a.rope_dim + 2 * v - 1) / (2 * v) : 0);
     if (a.items == 0) return LC_OK;
     // Few rows: a row's heads go to several CTAs, each with at least one item a
     // thread; every CTA forms the table again.  Many rows: a CTA takes as many as
@@ -245,8 +259,8 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     splits = (a.n_heads + a.heads_per_cta - 1) / a.heads_per_cta;
     a.rows_per_cta = 1;
     const size_t table = (size_t)half * sizeof(float2);
-    while (splits == 1 && a.rows_per_cta * row_items < 4 * kRpThreads && m / (a.rows_per_cta + 1) >= 4u * ctx->num_sms &&
-           (a.rows_per_cta + 1) * table <= 32 * 1024)
+    while (splits == 1 && a.rows_per_cta * row_items < 4 * kRpThreads &&
+           m / (a.rows_per_cta + 1) >= 4u * ctx->num_sms && (a.rows_per_cta + 1) * table <= 32 * 1024)
         a.rows_per_cta++;
     a.m = m;
     a.lanes = std::min(a.items, kRpThreads);
@@ -256,8 +270,18 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
         kernel<<<grid, kRpThreads, smem, ctx->stream>>>(a);
         return lc_after_launch(ctx, "lc_rope");
     };
-    if (pairs) return vec ? go(rope_kernel<TI, TO, true, V, true>) : go(rope_kernel<TI, TO, true, 2, false>);
-    return vec ? go(rope_kernel<TI, TO, false, V, true>) : go(rope_kernel<TI, TO, false, 1, false>);
+    auto width = [&](auto pair, auto copies) {
+        constexpr bool P = decltype(pair)::value, C = decltype(copies)::value;
+        if (vec) return go(rope_kernel<TI, TO, P, V, true, C>);
+        if (halves) return go(rope_kernel<TI, TO, P, V / 2, true, C>);
+        if constexpr (V / 2 > 2)
+            if (twos) return go(rope_kernel<TI, TO, P, 2, true, C>);
+        return go(rope_kernel<TI, TO, P, P ? 2 : 1, false, C>);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (a.items > a.rot) return pairs ? width(Yes(), Yes()) : width(No(), Yes());
+    return pairs ? width(Yes(), No()) : width(No(), No());
 }
 
 template <class TI>
