@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(kLgAll, 3) logits_kernel(const __grid_constant
     const uint32_t lane = tid & 31;
     const bool stream = tid < kLgThreads, lists = r.hist_len || r.bias_len;
     uint32_t row = blockIdx.x / a.cl;  // the cluster's rows: `clusters` apart
+    griddep_wait();  // the kernel before this one, whose end the launch need not wait for
     if (a.keys) cluster_arrive();      // that all its CTAs run, before the first store to another one
 
     // A stream thread's share of a slice: kLgVecs pieces of 4 tokens, kLgThreads * 4
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(kLgRowThreads, 2) logits_row_kernel(const __gr
     const uint32_t p0 = min(a.n, rank * a.part), len = min(a.n - p0, a.part);
     const int tid = threadIdx.x;
     const uint32_t lane = tid & 31, warp_at = (tid & ~31) * 4;
+    griddep_wait();  // the kernel before this one, whose end the launch need not wait for
     if (a.keys) cluster_arrive();  // that all its CTAs run, before the first store to another one
 
     constexpr int kStep = kLgRowThreads * 4;
@@ -543,18 +545,20 @@ __global__ void __launch_bounds__(kLgRowThreads, 2) logits_row_kernel(const __gr
     }
 }
 
-// What a launch of clusters of `cl` CTAs says (attr: its one attribute).
+// What a launch of clusters of `cl` CTAs says (attr: its two attributes).
 cudaLaunchConfig_t lg_config(int threads, size_t smem, uint32_t cl, cudaLaunchAttribute *attr) {
-    attr->id = cudaLaunchAttributeClusterDimension;
-    attr->val.clusterDim.x = cl;
-    attr->val.clusterDim.y = 1;
-    attr->val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cl;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cl);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cfg;
 }
 
@@ -571,8 +575,9 @@ int lg_resident(lc_ctx *ctx, int kernel, uint32_t cl, int *clusters) {
     const size_t smem = kernel ? kLgRowSlice * 8 : kLgSlice * 14 + kLgMine * 4;
     LC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (int s = lc_set_smem_attr(f, smem)) return s;
-    cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = lg_config(kernel ? kLgRowThreads : kLgAll, smem, cl, &attr);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = lg_config(kernel ? kLgRowThreads : kLgAll, smem, cl, attr);
+    cfg.numAttrs = 1;
     LC_CUDA(cudaOccupancyMaxActiveClusters(clusters, f, &cfg));
     if (at) at->store(1 + *clusters);
     return LC_OK;
@@ -665,8 +670,8 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     const size_t smem = !lists ? 0
                         : few  ? kLgRowSlice * (r.bias_len ? 8 : 4)
                                : kLgSlice * (r.bias_len ? 14 : 10) + kLgMine * 4;
-    cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = lg_config(few ? kLgRowThreads : kLgAll, smem, cl, &attr);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = lg_config(few ? kLgRowThreads : kLgAll, smem, cl, attr);
     cfg.gridDim = dim3(a.clusters * cl);
     cfg.stream = ctx->stream;
     LC_CUDA(cudaLaunchKernelEx(&cfg, few ? logits_row_kernel : logits_kernel, (const LgArgs)a));

@@ -20,7 +20,8 @@
 // hand-out of work, 9 loads of V, 10 issues S, 11 issues O.  K, V and S have two
 // stages: the next tile's scores are formed while the softmax warps work on this
 // one's, so that these, the longest link, do not wait (with one stage of 128 keys
-// a tile's products and softmax alternated: 3850 cycles per 128 keys).  Two CTAs share an
+// a tile's products and softmax alternated: 3850 cycles per 128 keys, now 3340; 900 to
+// 1040 TFLOP/s on a long prefix).  Two CTAs share an
 // SM (256 TMEM columns and 100 KB each).  CTAs stay for several items: the next
 // one's Q and K are loaded while the last one's values and results are worked on.
 #include <float.h>
@@ -448,10 +449,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     PaItem next;
-    if (threadIdx.x == 32 * kPaLoadWarp) {
-        next = pa_item_begin(a, blockIdx.x);
-        prefetch_tensormap(&maps.q);
-    }
+    if (threadIdx.x == 32 * kPaLoadWarp) prefetch_tensormap(&maps.q);
     if (threadIdx.x == 0) {
         mbar_init(sched.bar(), 1);
         for (int k = 0; k < 2; k++) {
@@ -465,6 +463,8 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         }
         mbar_init_fence();
     }
+    griddep_wait();  // the kernel before this one, whose end the launch and the lines above need not wait for
+    if (threadIdx.x == 32 * kPaLoadWarp) next = pa_item_begin(a, blockIdx.x);
     if (warp == kPaMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
                      "r"(kPaTmemCols)
@@ -1071,20 +1071,24 @@ void pa_plan(PaArgs &a, int num_sms, int hd, int planes) {
 template <class T, class TO, int HD>
 int pa_launch(lc_ctx *ctx, const PaArgs &a, int items, const PaMaps &maps) {
     auto kernel = prefix_attn_kernel<T, TO, HD>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = ctx->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     if (items) {
         if (int s = lc_set_smem_attr((const void *)kernel, PaSmem<HD>::kBytes)) return s;
-        kernel<<<items, kPaThreads, PaSmem<HD>::kBytes, ctx->stream>>>(maps, a);
+        cfg.gridDim = dim3(items);
+        cfg.blockDim = dim3(kPaThreads);
+        cfg.dynamicSmemBytes = PaSmem<HD>::kBytes;
+        LC_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, a));
     }
     if (a.merge) {
-        cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(div_up((int64_t)a.n_kv * a.row_blocks * (HD / 8) * a.merge_ways, 4));
         cfg.blockDim = dim3(128);
-        cfg.stream = ctx->stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = items ? 1 : 0;
+        cfg.dynamicSmemBytes = 0;
         LC_CUDA(cudaLaunchKernelEx(&cfg, prefix_attn_merge_kernel<TO, HD>, a));
     }
     return lc_after_launch(ctx, "lc_prefix_attn");

@@ -19,13 +19,14 @@
 #include <cuda_bf16.h>
 
 #include "lc_internal.cuh"
+#include "lc_sm100.cuh"
 
 namespace {
 
 constexpr int kRpThreads = 128;
 // Items a thread has in flight (and loads before the table is ready): 8192 rows of
-// 40 bf16 heads take 36 us with two in 8 CTAs an SM, 41 us with three in 6; more of
-// narrower ones gained nothing.
+// 40 bf16 heads take 34 us with two in 8 CTAs an SM (4.9 TB/s), 5 us more with three in
+// 6; more of narrower ones gained nothing.
 constexpr int kRpItems = 2;
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
         }
     };
 
+    griddep_wait();  // the kernel before this one, whose end the launch need not wait for
     RpPack<TI, V> p0[kRpItems], p1[kRpItems];
     const int in0 = side < sides ? side / nh : rows, first_h = side - side / nh * nh;
     int in = in0, h = first_h;  // of the next load
@@ -267,7 +269,17 @@ int rope_launch(lc_ctx *ctx, const RpArgs &base, uint32_t m, bool pairs) {
     const dim3 grid((m + a.rows_per_cta - 1) / a.rows_per_cta, splits);
     const size_t smem = a.rows_per_cta * table;
     auto go = [&](auto kernel) -> int {
-        kernel<<<grid, kRpThreads, smem, ctx->stream>>>(a);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kRpThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = ctx->stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        LC_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
         return lc_after_launch(ctx, "lc_rope");
     };
     auto width = [&](auto pair, auto copies) {

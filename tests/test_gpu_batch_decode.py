@@ -158,3 +158,72 @@ def test_beside_other_kernels(ctx, dev):
     for c in ctxs:
         c.device_status()
         c.close()
+
+
+def test_captured_among_copies_and_forks(ctx, dev):
+    """A graph in which the operators follow memsets, copies, events of another stream and each other, each with
+    inputs that the node before it writes late; replays see new inputs."""
+    import torch
+
+    g = torch.Generator(dev).manual_seed(1)
+    rows, prefix, cap = 6, 700, 40
+    f16 = torch.float16
+    src = torch.randn(rows, WQ + WK, generator=g, device=dev)
+    q, k = torch.empty(rows, WQ, device=dev), torch.empty(rows, WK, device=dev)
+    q16, k16 = torch.empty(rows, WQ, device=dev, dtype=f16), torch.empty(rows, WK, device=dev, dtype=f16)
+    kp, vp = (torch.randn(prefix, WK, generator=g, device=dev).to(f16) for _ in range(2))
+    ko = torch.zeros(rows, cap, WK, device=dev, dtype=f16)
+    vo = torch.randn(rows, cap, WK, generator=g, device=dev).to(f16)
+    pos = torch.arange(rows, device=dev, dtype=torch.int32) + prefix
+    freq = torch.from_numpy(lc.rope_freq(HD)).to(dev)
+    own_len = torch.ones(rows, device=dev, dtype=torch.int32)
+    seq_start = torch.arange(rows + 1, device=dev, dtype=torch.int32)
+    kv = lc.PrefixKV(kp, vp, prefix, ko, vo, cap, own_len, seq_start, rows)
+    out, logits = torch.empty(rows, WQ, device=dev), torch.empty(rows, 9000, device=dev)
+    head = torch.randn(WQ, 9000, generator=g, device=dev) / 16
+    keys, side_keys = (torch.empty(rows, device=dev, dtype=torch.int64) for _ in range(2))
+    pen = torch.full((rows,), 1.3, device=dev)
+    rules = lc.LogitsRules(hist=torch.arange(600, device=dev, dtype=torch.int32),
+                           hist_start=torch.arange(rows + 1, device=dev, dtype=torch.int32) * 100, repetition=pen)
+    main, side, other = torch.cuda.Stream(), torch.cuda.Stream(), lc.Context(0)
+
+    def step():
+        mine = torch.cuda.current_stream()
+        ctx.set_stream(mine), other.set_stream(side)
+        q.copy_(src[:, :WQ])  # copies, then rope on what they wrote
+        k.copy_(src[:, WQ:])
+        ctx.rope(lc.F32, lc.F16, lc.ROPE_HALF, q, q16, N_Q, k, k16, N_KV, pos, freq, rows, HD, HD)
+        ko[:, 0].copy_(k16)
+        side.wait_stream(mine)
+        with torch.cuda.stream(side):
+            logits.zero_()
+            other.logits_process(logits, rules, None, side_keys, rows, 9000)
+            pen.mul_(1.0)
+        mine.wait_stream(side)
+        ctx.prefix_attn(lc.F16, lc.F32, q16, kv, out, rows, N_Q, N_KV, HD, HD ** -0.5)
+        ctx.prefix_attn(lc.F16, lc.F32, q16, kv, out, rows, N_Q, N_KV, HD, HD ** -0.5)
+        torch.mm(out, head, out=logits)
+        ctx.logits_process(logits, rules, logits, keys, rows, 9000)
+        ctx.rope(lc.F32, lc.F32, lc.ROPE_HALF, out, out, N_Q, None, None, 0, pos, freq, rows, HD, HD)
+        return [t.clone() for t in (q16, out, logits, keys, side_keys)]
+
+    try:
+        with torch.cuda.stream(main):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            captured = step()
+        for seed in range(4):
+            src.copy_(torch.randn(src.shape, generator=torch.Generator(dev).manual_seed(seed), device=dev))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in captured]
+            with torch.cuda.stream(main):
+                want = step()
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    finally:
+        ctx.set_stream(None)
