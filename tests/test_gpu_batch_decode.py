@@ -160,7 +160,7 @@ def test_beside_other_kernels(ctx, dev):
         c.close()
 
 
-def test_captured_among_copies_and_forks(ctx, dev):
+def test_captured_among_copies_and_forks(dev):
     """A graph in which the operators follow memsets, copies, events of another stream and each other, each with
     inputs that the node before it writes late; replays see new inputs."""
     import torch
@@ -185,7 +185,7 @@ def test_captured_among_copies_and_forks(ctx, dev):
     pen = torch.full((rows,), 1.3, device=dev)
     rules = lc.LogitsRules(hist=torch.arange(600, device=dev, dtype=torch.int32),
                            hist_start=torch.arange(rows + 1, device=dev, dtype=torch.int32) * 100, repetition=pen)
-    main, side, other = torch.cuda.Stream(), torch.cuda.Stream(), lc.Context(0)
+    main, side, ctx, other = torch.cuda.Stream(), torch.cuda.Stream(), lc.Context(0), lc.Context(0)
 
     def step():
         mine = torch.cuda.current_stream()
@@ -207,23 +207,20 @@ def test_captured_among_copies_and_forks(ctx, dev):
         ctx.rope(lc.F32, lc.F32, lc.ROPE_HALF, out, out, N_Q, None, None, 0, pos, freq, rows, HD, HD)
         return [t.clone() for t in (q16, out, logits, keys, side_keys)]
 
-    try:
-        with torch.cuda.stream(main):
-            step()
+    with torch.cuda.stream(main):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        captured = step()
+    for seed in range(4):
+        src.copy_(torch.randn(src.shape, generator=torch.Generator(dev).manual_seed(seed), device=dev))
         torch.cuda.synchronize()
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=main):
-            captured = step()
-        for seed in range(4):
-            src.copy_(torch.randn(src.shape, generator=torch.Generator(dev).manual_seed(seed), device=dev))
-            torch.cuda.synchronize()
-            graph.replay()
-            torch.cuda.synchronize()
-            got = [t.clone() for t in captured]
-            with torch.cuda.stream(main):
-                want = step()
-            torch.cuda.synchronize()
-            for a, b in zip(got, want):
-                assert torch.equal(a, b)
-    finally:
-        ctx.set_stream(None)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        with torch.cuda.stream(main):
+            want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
