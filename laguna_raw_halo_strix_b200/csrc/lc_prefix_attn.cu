@@ -463,7 +463,9 @@ __global__ void __launch_bounds__(kPaThreads, 2)
         }
         mbar_init_fence();
     }
-    griddep_wait();  // the kernel before this one, whose end the launch and the lines above need not wait for
+    // The kernel before this one, whose end the launch and the lines above need not wait for.
+    // Its CTAs may still have to allocate their TMEM: nothing is held of that before.
+    griddep_wait();
     if (threadIdx.x == 32 * kPaLoadWarp) next = pa_item_begin(a, blockIdx.x);
     if (warp == kPaMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tslot)),
