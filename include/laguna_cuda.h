@@ -263,7 +263,8 @@ typedef struct {
  * be finite, for the others multiply it by 0.  The prefix's products
  * are formed once for the batch.  q, k, v are of type dtype (LC_F16 or LC_BF16),
  * out of that type or LC_F32; softmax and sums in f32, weights rounded to dtype
- * (to twice its digits for LC_F32 outputs).  seq_start is non-decreasing within
+ * (LC_F32 outputs: to 22 bits or more), f16 ones to 2^-32 of the row's largest
+ * where that is more.  seq_start is non-decreasing within
  * 0..rows (values outside are held inside); rows of no sequence stay as they
  * are in out.  Lengths and starts are read on the device, so a captured call
  * can be replayed as sequences grow up to own_cap.  head_dim 64 or 128, scale

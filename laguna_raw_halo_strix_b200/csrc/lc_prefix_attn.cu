@@ -427,8 +427,15 @@ template <class T, class TO, int HD>
 __global__ void __launch_bounds__(kPaThreads, 2)
     prefix_attn_kernel(const __grid_constant__ PaMaps maps, const __grid_constant__ PaArgs a) {
     using L = PaSmem<HD>;
-    // Planes of P: 1, or for f32 outputs as many as hold 22 bits or more
+    // Planes of P: 1, or for f32 outputs as many as hold 22 bits or more (of f16 weights
+    // above 2^-16 of the row's largest; below, 2^-32 of that one)
     constexpr int kPlanes = !std::is_same<TO, float>::value ? 1 : std::is_same<T, __half>::value ? 2 : 3;
+    // The reference of a row's weights lies 2^kShift below its maximum.  The planes of f16
+    // weights end at its subnormals' spacing, 2^-24: with weights about 2^7 (below 2^15,
+    // see where the reference moves) that is 2^-31 of the largest (f32 outputs of 300 rows
+    // with a first key 14 nats above 5299 others: 2.5e-6 off, 1.8e-5 with weights about 1;
+    // no difference in time).  bf16 has the exponents of f32.
+    constexpr float kShift = std::is_same<T, __half>::value ? 7.f : 0.f;
     // TMEM columns of S: two stages of 64; a warp's planes of 16 columns overwrite its
     // own 32 scores, and the third, where there is one, takes the second stage's place
     constexpr int kStages = kPlanes < 3 ? 2 : 1;
@@ -755,12 +762,13 @@ __global__ void __launch_bounds__(kPaThreads, 2)
                             t2 = fmaxf(t2, x[e + 2]), t3 = fmaxf(t3, x[e + 3]);
                         }
                         const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2;
-                        // The reference maximum moves, and O is rescaled, only when a score is
-                        // more than 2^8 above it: weights up to 256 are as exact, and fit f16
-                        if (pa_meet_any(quarter, i == 0 || top > m_ref + 8.f)) {
+                        // The reference moves, and O is rescaled, only when a score is more than
+                        // 2^8 above the last maximum: weights up to 2^(8 + kShift) are as exact,
+                        // and fit f16
+                        if (pa_meet_any(quarter, i == 0 || top > m_ref + (8.f + kShift))) {
                             *mine = top;
                             pa_meet(quarter);
-                            const float m_new = fmaxf(m_ref, fmaxf(top, *other));
+                            const float m_new = fmaxf(m_ref, fmaxf(top, *other) - kShift);
                             const float f = m_new == m_ref ? 1.f : exp2_fast(m_ref - m_new);
                             if (i % kRun) {
                                 tile_done(pv_done, it - 1);

@@ -352,3 +352,62 @@ def test_few_rows_on_many_keys(ctx, dev, src, dst, n_q, n_kv, hd, prefix, cap, c
     b = Batch(dev, src, dst, n_q, n_kv, hd, prefix, cap, counts, lens, seed=6, extra=3)
     b.run(ctx)
     b.check()
+
+
+@pytest.mark.parametrize("dst", ["f16", "f32"])
+@pytest.mark.parametrize("hd,prefix,cap,counts,peak,second", [
+    (64, 16384, 20, [1], 17.0, 0.0),          # few rows, many states
+    (128, 4096, 100, [1, 1, 1], 12.0, 5.5),   # a later key of 2^7.9 times the first one's weight
+    (64, 32768, 5, [1] * 40, 12.0, 0.0),
+    (64, 0, 9000, [3], 15.0, 5.5),
+    (128, 5000, 300, [300], 14.0, 0.0),       # whole row tiles
+])
+def test_a_dominant_first_key_keeps_the_others(ctx, dev, dst, hd, prefix, cap, counts, peak, second):
+    """f16 keys, the first of them `peak` nats above the rest and with values of 0: the result is what the many small
+    weights add up to.  Weights lie at 2^7 or more where the row's largest is, so that a subnormal one (spacing 2^-24) is
+    off by at most 2^-25 of that scale, 2^-32 of the largest weight; else as above.  `second`: nats by which the last
+    prefix (or own) key exceeds the first."""
+    import torch
+
+    n_q, n_kv = 4, 2
+    lens = [cap] * len(counts)
+    b = Batch(dev, "f16", dst, n_q, n_kv, hd, prefix, cap, counts, lens, seed=prefix + cap, garbage=False)
+    b.q.view(-1, n_q, hd)[:, :, 0] = 8.0
+    for x in (b.kp, b.ko):
+        x.view(-1, n_kv, hd)[:, :, 0] = 0.0
+    for x in (b.vp, b.vo):
+        x.copy_((1 + 0.5 * x.float()).half())
+    k, v = (b.kp, b.vp) if prefix else (b.ko[0], b.vo[0])
+    step = math.sqrt(hd) / 8
+    k.view(-1, n_kv, hd)[0, :, 0] = peak * step
+    v[0] = 0.0
+    if second:
+        k.view(-1, n_kv, hd)[len(k) - sum(counts) - 1, :, 0] = (peak + second) * step
+        v[len(k) - sum(counts) - 1] = 0.0
+    b.run(ctx)
+    torch.cuda.synchronize()
+    at = 0
+    for i, c in enumerate(counts):
+        n = prefix + cap
+        key, reach = torch.arange(n, device=dev), torch.arange(c, device=dev) + cap - c
+        seen = (key < prefix) | (key - prefix <= reach[:, None])
+        for h in range(n_kv):
+            kk = torch.cat([b.kp[:prefix], b.ko[i]]).double().view(n, n_kv, hd)[:, h]
+            vv = torch.cat([b.vp[:prefix], b.vo[i]]).double().view(n, n_kv, hd)[:, h]
+            q = b.q[at:at + c].double().view(c, n_q, hd)[:, 2 * h:2 * h + 2]
+            s = torch.einsum("rgd,kd->grk", q, kk) * b.scale
+            mag = torch.einsum("rgd,kd->grk", q.abs(), kk.abs()) * b.scale
+            s = s.masked_fill(~seen, -math.inf)
+            w = (s - s.amax(-1, keepdim=True)).exp()
+            total = w.sum(-1, keepdim=True)
+            o, a = (w @ vv) / total, (w @ vv.abs()) / total
+            flat = (seen.double() @ vv.abs()) / total
+            err_s = ((hd + 2) * 2.0 ** -24 * mag * seen).amax(-1, keepdim=True)
+            tol = a * (2 * (err_s * 1.01 + 2.0 ** -22 + (math.sqrt(n) + 64) * 2.0 ** -24) +
+                       (2.0 ** -22 if dst == "f32" else 2.0 ** -11)) + flat * 2.0 ** -32
+            fo = torch.finfo(tt(dst))
+            tol = tol * 1.001 + o.abs() * fo.eps / 2 + fo.smallest_normal * fo.eps
+            got = b.out[at:at + c].double().view(c, n_q, hd)[:, 2 * h:2 * h + 2].transpose(0, 1)
+            err = (got - o).abs()
+            assert (err <= tol).all(), (i, h, float((err / o.abs()).max()), float((tol / o.abs()).max()))
+        at += c
