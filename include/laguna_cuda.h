@@ -284,8 +284,8 @@ int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void *q, uint64_
  *   y1 = scale (x1 cos a - x2 sin a),  y2 = scale (x2 cos a + x1 sin a);
  * dims from rope_dim on are copied (rope_dim 0 copies and converts whole rows).
  * LC_ROPE_HALF pairs dim i with i + rope_dim / 2, LC_ROPE_PAIRS dim 2i with
- * 2i + 1.  The angle is exact for every int32 position; -pos with 1 / scale
- * undoes pos.  x is of type dtype and y of out_dtype (LC_F32, LC_F16 or LC_BF16
+ * 2i + 1.  The angle is exact (to 2^-49) for every int32 position; -pos with
+ * 1 / scale undoes pos.  x is of type dtype and y of out_dtype (LC_F32, LC_F16 or LC_BF16
  * each; f32 arithmetic, one rounding), so k can go straight into a 16-bit cache.
  * ld*: elements between rows (0: rows follow each other; q and k may be columns
  * of one buffer).  An output may be its own input (same type and stride); any

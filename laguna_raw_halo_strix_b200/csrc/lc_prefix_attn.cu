@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     prefix_attn_kernel(const __grid_constant__ PaMaps maps, const __grid_constant__ PaArgs a) {
     using L = PaSmem<HD>;
     // Planes of P: 1, or for f32 outputs as many as hold 22 bits or more (of f16 weights
-    // above 2^-16 of the row's largest; below, 2^-32 of that one)
+    // above 2^-10 of the row's largest; below, to 2^-32 of that one)
     constexpr int kPlanes = !std::is_same<TO, float>::value ? 1 : std::is_same<T, __half>::value ? 2 : 3;
     // The reference of a row's weights lies 2^kShift below its maximum.  The planes of f16
     // weights end at its subnormals' spacing, 2^-24: with weights about 2^7 (below 2^15,

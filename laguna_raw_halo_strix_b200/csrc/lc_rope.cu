@@ -4,10 +4,11 @@
 // Pair i of a head (rope_dim / 2 pairs) is turned by a = pos * freq[i]:
 //   y1 = s (x1 cos a - x2 sin a),  y2 = s (x2 cos a + x1 sin a),
 // the remaining dims are copied.  The angle of a far position needs more than
-// 24 bits (pos 1e6 at freq 1 is 0.06 rad off in f32): the product of two
-// numbers of at most 31 and 24 bits is exact to 2^-53 in a double, and is
-// reduced mod 2 pi there; sincospif then sees |a| <= pi.  The rotation itself is
-// f32 with one rounding to the output type.
+// 24 bits (pos 1e6 at freq 1 is 0.06 rad off in f32).  The product of two numbers of
+// at most 31 and 24 bits has 55: it is held as a double and what that lost, and
+// reduced mod 2 pi in 64 bits.  sincospif sees it as an f32, |a| <= pi, and a
+// correction of first order makes up for that rounding (up to 9.4e-8 rad, half its
+// square is 2^-47).  The rotation itself is f32 with one rounding to the output type.
 //
 // Bound by the bytes of x and y.  One CTA takes some rows (or a share of one
 // row's heads when there are few): the rows' table of (cos, sin) is formed once
@@ -29,6 +30,7 @@ constexpr int kRpThreads = 128;
 // 6; more of narrower ones gained nothing.
 constexpr int kRpItems = 2;
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
+constexpr double kRpTurn = 0.15915494309189533577, kRpTurnLost = -9.8393383375912435e-18;  // 1 / (2 pi), its rounding
 
 template <class T>
 struct RpVec;  // 16 bytes of T
@@ -186,12 +188,16 @@ __global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
     if (half) {
         for (int i = threadIdx.x; i < rows * half; i += kRpThreads) {
             const int in = i / half;
-            const double t = (double)a.pos[row0 + in] * (double)a.freq[i - in * half];  // exact
-            const double n = t * 0.15915494309189533577;  // turns: 1 / (2 pi), rounded to a double,
-            const double d = fma(t, 0.15915494309189533577, -n) + t * -9.8393383375912435e-18;  // and what that lost
+            const double p = (double)a.pos[row0 + in], f = (double)a.freq[i - in * half];
+            const double t = p * f, lost = fma(p, f, -t);
+            const double n = t * kRpTurn;  // turns
+            const double d = fma(t, kRpTurn, -n) + fma(lost, kRpTurn, t * kRpTurnLost);
+            const double r = 2.0 * ((n - rint(n)) + d);  // in units of pi
+            const float rf = (float)r, e = (float)(r - (double)rf) * 3.14159265f;
             float sn, cn;
-            sincospif((float)(2.0 * ((n - rint(n)) + d)), &sn, &cn);
-            cs_rows[in * half + rp_slot<PAIRS ? V / 2 : V>(i - in * half)] = make_float2(cn * a.scale, sn * a.scale);
+            sincospif(rf, &sn, &cn);
+            cs_rows[in * half + rp_slot<PAIRS ? V / 2 : V>(i - in * half)] =
+                make_float2(fmaf(-sn, e, cn) * a.scale, fmaf(cn, e, sn) * a.scale);
         }
         __syncthreads();
     }

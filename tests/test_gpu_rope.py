@@ -213,3 +213,51 @@ assert [lc.key_index(int(k)) for k in all_keys] == big.argmax(1).tolist()
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+PI = 3141592653589793238462643383279502884197169399375105820974944592307816406286208999
+
+
+def turned_past(pos, freq):
+    """(how far the exact angle pos * freq is past the nearest multiple of pi, whether that is an odd one)."""
+    from fractions import Fraction
+
+    pi = Fraction(PI, 10 ** 81)
+    a = Fraction(int(pos)) * Fraction(float(freq))
+    k = round(a / pi)
+    return float(a - k * pi), k % 2
+
+
+@pytest.mark.parametrize("far", [131072, 2 ** 31 - 1])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_angles_next_to_multiples_of_pi(ctx, dev, far, pairs):
+    """Where the sine is small its value shows the angle's absolute error.  x = (1, 0) gives (cos a, sin a): the sine
+    within 2 ulp of the function (2^-22), its correction and the angle's rounding (2^-23 each) of the value, and
+    2^-50 for the reduction in 64 bits."""
+    import torch
+
+    rng = np.random.default_rng(far)
+    f = rng.uniform(0.25, 1.0, 400000).astype(np.float32)
+    p = rng.integers(far // 2, far, f.size)
+    p *= rng.choice([-1, 1], f.size)
+    turns = p.astype(np.longdouble) * f.astype(np.longdouble) / (np.longdouble(PI // 10 ** 63) / np.longdouble(10) ** 18)
+    near = np.argsort(np.abs(turns - np.rint(turns)))[:64]
+    f, p = f[near], p[near]
+    half = near.size
+    x = torch.zeros(half, 2 * half, device=dev)
+    (x[:, 0::2] if pairs else x[:, :half]).fill_(1.0)
+    y = torch.empty_like(x)
+    ctx.rope(lc.F32, lc.F32, int(pairs), x, y, 1, None, None, 0, torch.from_numpy(p.astype(np.int32)).to(dev),
+             torch.from_numpy(f).to(dev), half, 2 * half, 2 * half)
+    torch.cuda.synchronize()
+    got = y.cpu().numpy().astype(np.float64)
+    cos, sin = (got[:, 0::2], got[:, 1::2]) if pairs else (got[:, :half], got[:, half:])
+    odd_ones = 0
+    for i in range(half):  # row i's pair i
+        past, odd = turned_past(p[i], f[i])
+        assert abs(past) < 1e-3
+        want = -np.sin(past) if odd else np.sin(past)
+        assert abs(sin[i, i] - want) <= abs(want) * 2.0 ** -21 + 2.0 ** -50, (i, sin[i, i], want, odd)
+        assert abs(cos[i, i] - (-np.cos(past) if odd else np.cos(past))) <= 2.0 ** -22
+        odd_ones += odd
+    assert 0 < odd_ones < half
