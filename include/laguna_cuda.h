@@ -97,7 +97,7 @@ int lc_set_sync(lc_ctx *ctx, int sync);
  * copies gave up (the launch's outputs are then invalid), else LC_OK.  Kernels
  * never hang on such a wait; this call is how the host learns of it. */
 int lc_device_status(lc_ctx *ctx);
-/* Device memory (bytes) the context holds in its grow-only scratch slots;
+/* Device memory (bytes) the context holds in its scratch (which only grows);
  * 0 until a call needs scratch.  No counterpart in the reference, whose
  * buffers are all created up front (ForwardBuffers::new, src/dflash.rs:259-285). */
 int lc_ctx_scratch_bytes(lc_ctx *ctx, size_t *bytes);
@@ -270,9 +270,12 @@ typedef struct {
  * can be replayed as sequences grow up to own_cap.  head_dim 64 or 128, scale
  * positive, at most 128 query heads to a KV head, ldq / ldo elements between
  * rows (0: packed), 16-byte aligned rows.
- * Partial states live in the context's scratch: graphs captured on one context
- * are not replayed at the same time, and capture needs a call of the same size
- * before it.  The reference attends one sequence at a time
+ * Partial states live in scratch of the context, a block for each stream that
+ * calls it and one for each captured graph (which holds it until it is
+ * destroyed, and no longer than the context): calls on several streams, and
+ * replays of several graphs, may run at the same time; one graph not beside
+ * itself.  A context's first call is not captured (LC_ERR_UNSUPPORTED where it
+ * needs scratch).  The reference attends one sequence at a time
  * (kernels/mha_attn.comp:31-72). */
 int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void *q, uint64_t ldq, const lc_prefix_kv *kv,
                    void *out, uint64_t ldo, uint32_t rows, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim,

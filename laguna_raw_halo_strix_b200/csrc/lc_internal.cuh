@@ -6,10 +6,28 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
 #include <functional>
+#include <memory>
 #include <vector>
 
 #include "laguna_cuda.h"
+
+// Scratch of calls that may run at the same time (lc_scratch_here): a block for each
+// stream, and one for each stream of each capture, which the captured graph holds until
+// it is destroyed.  Shared with those graphs, which may outlive the context; all
+// memory is freed by lc_destroy.
+struct LcStreamScratch {
+    struct Block {
+        void *p;
+        size_t bytes;
+        cudaStream_t stream;
+        std::atomic<unsigned long long> capture;  // its id; 0: of a stream, or of no graph any more (set by
+    };                                            // the thread that destroys the graph)
+    std::vector<std::unique_ptr<Block>> eager, captured;
+    bool called = false;  // a call has been made outside captures, or needed no block
+    size_t bytes = 0;
+};
 
 // Context: one device, one stream, one grow-only scratch arena.
 struct lc_ctx {
@@ -30,9 +48,7 @@ struct lc_ctx {
     // Grow-only scratch slots (see LC_SCRATCH_*).
     void *scratch[8] = {};
     size_t scratch_bytes[8] = {};
-    // Blocks that lc_scratch_kept replaced, freed by lc_destroy.
-    std::vector<void *> kept;
-    size_t kept_bytes = 0;
+    std::shared_ptr<LcStreamScratch> stream_scratch = std::make_shared<LcStreamScratch>();
     // Device word that kernels set (atomicOr of LC_DEV_*) when a bounded wait
     // gives up; read and cleared by lc_device_status().  Allocated at init.
     unsigned *dev_status = nullptr;
@@ -66,8 +82,7 @@ enum {
     LC_SCRATCH_FIXUP = 4,
     LC_SCRATCH_FFN = 5,
     LC_SCRATCH_HOSTIO = 6,
-    LC_SCRATCH_PREFIX = 7,  // lc_scratch_kept
-    LC_SCRATCH_COUNT = 8
+    LC_SCRATCH_COUNT = 7
 };
 // Grow-only scratch slot of at least `bytes` (256-byte aligned).  Returns
 // nullptr and sets the error on failure.  Waits for the stream before
@@ -75,12 +90,13 @@ enum {
 void *lc_scratch(lc_ctx *ctx, int slot, size_t bytes);
 // Same, and a newly allocated slot is zero-filled (on the context's stream).
 void *lc_scratch_zeroed(lc_ctx *ctx, int slot, size_t bytes);
-// Scratch slot that a captured graph may go on using after the slot has grown:
-// a replaced block stays allocated until lc_destroy, and each block is at least
-// twice the last, so all of them together hold less than twice the largest.
-// Growing during a stream capture is LC_ERR_UNSUPPORTED (allocate by a call of
-// the same size before).
-int lc_scratch_kept(lc_ctx *ctx, int slot, size_t bytes, void **out);
+// At least `bytes` of scratch that only this stream's calls, or this capture's on this
+// stream, use: calls on several streams and captured graphs may run at the same time.
+// A stream's block that has become too small stays allocated until lc_destroy, for work
+// on it may be under way, and each is at least twice the last.  A captured block
+// lives as long as the graph and goes to a later capture then.  The first call of a
+// context in a capture is LC_ERR_UNSUPPORTED.
+int lc_scratch_here(lc_ctx *ctx, size_t bytes, void **out);
 // Resolve ctx->static_pack with ctx->device current (lc_proj.cu; called by lc_init).
 int lc_static_pack_resolve(lc_ctx *ctx);
 // Make ctx->device current on this thread.

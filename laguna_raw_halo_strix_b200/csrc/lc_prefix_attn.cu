@@ -1186,7 +1186,7 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
         a.row_blocks = div_up((int64_t)rows * a.group, 32);
         const size_t states = (size_t)(a.prefix_splits + a.seq_splits) * a.n_kv * a.row_blocks * 32;
         void *scr = nullptr;
-        if (int s = lc_scratch_kept(ctx, LC_SCRATCH_PREFIX, states * (head_dim * 4 + 8) + 256, &scr)) return s;
+        if (int s = lc_scratch_here(ctx, states * (head_dim * 4 + 8) + 256, &scr)) return s;
         a.ml_part = (float2 *)scr;
         a.o_part = (float *)((char *)scr + ((states * 8 + 255) & ~(size_t)255));
     }
@@ -1208,6 +1208,8 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
         const uint64_t dims[3] = {head_dim, n_q_heads, rows}, ld[2] = {head_dim, ldq};
         if (int s = pa_map(&maps.q, q, dtype, dims, ld, a.group, a.box_toks)) return s;
     }
-    return dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, maps)
-                           : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, maps);
+    const int status = dtype == LC_F16 ? pa_types<__half>(ctx, out_dtype, head_dim, a, (int)items, maps)
+                                       : pa_types<__nv_bfloat16>(ctx, out_dtype, head_dim, a, (int)items, maps);
+    if (status == LC_OK) ctx->stream_scratch->called = true;
+    return status;
 }

@@ -4,6 +4,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <exception>
 #include <map>
 #include <mutex>
 
@@ -85,7 +86,7 @@ extern "C" int lc_init(int device, lc_ctx **out) {
 
 extern "C" int lc_ctx_scratch_bytes(lc_ctx *ctx, size_t *bytes) {
     LC_REQUIRE(ctx && bytes, LC_ERR_INVALID, "lc_ctx_scratch_bytes: null argument");
-    size_t t = ctx->kept_bytes;
+    size_t t = ctx->stream_scratch->bytes;
     for (int i = 0; i < LC_SCRATCH_COUNT; i++) t += ctx->scratch_bytes[i];
     *bytes = t;
     return LC_OK;
@@ -112,7 +113,8 @@ extern "C" int lc_destroy(lc_ctx *ctx) {
     if (ctx->stream && ctx->stream != ctx->own_stream) cudaStreamSynchronize(ctx->stream);
     for (int i = 0; i < LC_SCRATCH_COUNT; i++)
         if (ctx->scratch[i]) cudaFree(ctx->scratch[i]);
-    for (void *p : ctx->kept) cudaFree(p);
+    for (auto *blocks : {&ctx->stream_scratch->eager, &ctx->stream_scratch->captured})
+        for (auto &b : *blocks) cudaFree(b->p);
     if (ctx->dev_status) cudaFree(ctx->dev_status);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     delete ctx;
@@ -233,30 +235,101 @@ void *lc_scratch_zeroed(lc_ctx *ctx, int slot, size_t bytes) {
     return p;
 }
 
-int lc_scratch_kept(lc_ctx *ctx, int slot, size_t bytes, void **out) {
-    if (bytes > ctx->scratch_bytes[slot]) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        LC_CUDA(cudaStreamIsCapturing(ctx->stream, &st));
-        LC_REQUIRE(st == cudaStreamCaptureStatusNone, LC_ERR_UNSUPPORTED,
-                   "scratch: %zu bytes needed during a stream capture, %zu held; make a call of this size before it",
-                   bytes, ctx->scratch_bytes[slot]);
-        size_t want = (std::max(bytes, 2 * ctx->scratch_bytes[slot]) + 255) & ~(size_t)255;
-        if (want < ((size_t)1 << 20)) want = (size_t)1 << 20;
-        void *p = nullptr;
-        cudaError_t e = cudaMalloc(&p, want);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return lc_fail(LC_ERR_OOM, "scratch: cudaMalloc(%zu): %s", want, cudaGetErrorString(e));
-        }
-        if (ctx->scratch[slot]) {
-            ctx->kept.push_back(ctx->scratch[slot]);
-            ctx->kept_bytes += ctx->scratch_bytes[slot];
-        }
-        ctx->scratch[slot] = p;
-        ctx->scratch_bytes[slot] = want;
+namespace {
+
+using Block = LcStreamScratch::Block;
+
+// A new block in `blocks`, allocated although this thread, or another stream, may be capturing.
+int new_block(LcStreamScratch &s, std::vector<std::unique_ptr<Block>> &blocks, size_t bytes, size_t want, Block **out) {
+    blocks.reserve(blocks.size() + 1);
+    auto b = std::make_unique<Block>();
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    LC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    b->bytes = want;
+    cudaError_t e = cudaMalloc(&b->p, want);
+    if (e != cudaSuccess && want > bytes) {
+        cudaGetLastError();
+        b->bytes = bytes;
+        e = cudaMalloc(&b->p, bytes);
     }
-    *out = ctx->scratch[slot];
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return lc_fail(LC_ERR_OOM, "scratch: cudaMalloc(%zu): %s", bytes, cudaGetErrorString(e));
+    }
+    s.bytes += b->bytes;
+    *out = b.get();
+    blocks.push_back(std::move(b));
     return LC_OK;
+}
+
+struct Held {  // a graph's hold on a block
+    std::shared_ptr<LcStreamScratch> scratch;  // keeps the block's entry
+    Block *block;
+};
+
+void CUDART_CB release_held(void *p) {
+    Held *h = static_cast<Held *>(p);
+    h->block->capture = 0;
+    delete h;
+}
+
+int scratch_here(lc_ctx *ctx, size_t bytes, void **out) {
+    bytes = (bytes + 255) & ~(size_t)255;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    LC_CUDA(cudaStreamGetCaptureInfo(ctx->stream, &st, &id, &graph));
+    LC_REQUIRE(st != cudaStreamCaptureStatusInvalidated, LC_ERR_CUDA, "scratch: the stream's capture has failed");
+    LcStreamScratch &s = *ctx->stream_scratch;
+    Block *b = nullptr;
+    if (st == cudaStreamCaptureStatusNone) {
+        size_t largest = 0;
+        for (auto &e : s.eager)
+            if (e->stream == ctx->stream && e->bytes > largest) largest = e->bytes, b = e.get();
+        if (largest < bytes) {
+            const size_t want = std::max(std::max(bytes, 2 * largest), (size_t)1 << 20);
+            if (int status = new_block(s, s.eager, bytes, want, &b)) return status;
+            b->stream = ctx->stream;
+        }
+    } else {
+        LC_REQUIRE(s.called, LC_ERR_UNSUPPORTED,
+                   "scratch: the first call of a context during a stream capture; make a call before it");
+        Block *idle = nullptr;
+        for (auto &e : s.captured) {
+            if (e->bytes < bytes) continue;
+            if (e->capture == id && e->stream == ctx->stream) b = e.get();
+            if (e->capture == 0 && (!idle || e->bytes < idle->bytes)) idle = e.get();
+        }
+        if (!b) {
+            b = idle;
+            if (!b)
+                if (int status = new_block(s, s.captured, bytes, bytes, &b)) return status;
+            auto held = std::make_unique<Held>(Held{ctx->stream_scratch, b});
+            cudaUserObject_t object = nullptr;
+            LC_CUDA(cudaUserObjectCreate(&object, held.get(), release_held, 1, cudaUserObjectNoDestructorSync));
+            held.release();  // by release_held now
+            b->capture = id, b->stream = ctx->stream;
+            const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+            if (e != cudaSuccess) {
+                cudaUserObjectRelease(object, 1);
+                return lc_fail(LC_ERR_CUDA, "scratch: cudaGraphRetainUserObject: %s", cudaGetErrorString(e));
+            }
+        }
+    }
+    s.called = true;
+    *out = b->p;
+    return LC_OK;
+}
+
+}  // namespace
+
+int lc_scratch_here(lc_ctx *ctx, size_t bytes, void **out) {
+    try {
+        return scratch_here(ctx, bytes, out);
+    } catch (const std::exception &) {
+        return lc_fail(LC_ERR_OOM, "scratch: no host memory");
+    }
 }
 
 // ---- buffers ---------------------------------------------------------------

@@ -411,3 +411,124 @@ def test_a_dominant_first_key_keeps_the_others(ctx, dev, dst, hd, prefix, cap, c
             err = (got - o).abs()
             assert (err <= tol).all(), (i, h, float((err / o.abs()).max()), float((tol / o.abs()).max()))
         at += c
+
+
+def busy_batches(dev):
+    """Two batches that keep the GPU some tens of microseconds, with many states each, and their results."""
+    import torch
+
+    a = Batch(dev, "bf16", "f32", 8, 2, 128, 6000, 300, [1] * 24, [(29 * i) % 300 + 1 for i in range(24)], seed=21)
+    b = Batch(dev, "f16", "f16", 16, 4, 64, 9000, 200, [2] * 17, [(31 * i) % 199 + 2 for i in range(17)], seed=22)
+    c = lc.Context(0)
+    for x in (a, b):
+        c.set_stream(torch.cuda.current_stream())
+        x.run(c)
+        x.check()
+    c.close()
+    return a, b, a.out.clone(), b.out.clone()
+
+
+def test_streams_of_one_context_at_the_same_time(ctx, dev):
+    """Calls of one context in turn on two streams that nothing orders: neither meets the other's states."""
+    import torch
+
+    a, b, want_a, want_b = busy_batches(dev)
+    c, streams = lc.Context(0), [torch.cuda.Stream() for _ in range(2)]
+    for x in (a, b):
+        x.out.fill_(77.0)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for x, s in zip((a, b), streams):
+            c.set_stream(s)
+            x.run(c)
+            with torch.cuda.stream(s):
+                outs.append((x, x.out.clone()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, want_a if x is a else want_b) for x, got in outs)
+    c.device_status()
+    c.close()
+
+
+def test_graphs_of_one_context_at_the_same_time(ctx, dev):
+    """Two graphs captured on one stream of one context, replayed on two streams beside eager calls on a third."""
+    import torch
+
+    a, b, want_a, want_b = busy_batches(dev)
+    e = Batch(dev, "bf16", "bf16", 8, 8, 64, 5000, 100, [1] * 30, [50] * 30, seed=23)
+    c, streams = lc.Context(0), [torch.cuda.Stream() for _ in range(4)]
+    c.set_stream(streams[3])
+    e.run(c)
+    e.check()
+    want_e, graphs = e.out.clone(), []
+    for x in (a, b):
+        x.out.fill_(77.0)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=streams[3]):
+            for _ in range(3):
+                x.run(c)
+        graphs.append(g)
+    for _ in range(10):
+        for x, g, s in zip((a, b), graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        c.set_stream(streams[2])
+        e.run(c)
+    torch.cuda.synchronize()
+    assert torch.equal(a.out, want_a) and torch.equal(b.out, want_b) and torch.equal(e.out, want_e)
+    c.device_status()
+    del graphs, g
+    c.close()
+
+
+def test_capture_after_a_call_that_needed_no_scratch(ctx, dev):
+    """A large prompt is written out by whole items, a single row needs states: captured all the same."""
+    import torch
+
+    big = Batch(dev, "bf16", "bf16", 32, 8, 128, 1024, 2048, [2048], [2048], seed=31, garbage=False)
+    one = Batch(dev, "bf16", "bf16", 32, 8, 128, 8192, 64, [1], [9], seed=32)
+    c, s = lc.Context(0), torch.cuda.Stream()
+    c.set_stream(s)
+    torch.cuda.synchronize()
+    big.run(c)
+    torch.cuda.synchronize()
+    assert c.scratch_bytes() == 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        one.run(c)
+    g.replay()
+    one.check()
+    del g
+    c.close()
+
+
+def test_captured_scratch_is_used_again(ctx, dev):
+    """The scratch of a destroyed graph goes to the next one."""
+    import gc
+    import time
+
+    import torch
+
+    b = Batch(dev, "f16", "f32", 8, 2, 64, 3000, 64, [1] * 5, [3, 9, 27, 40, 1], seed=33)
+    c, s = lc.Context(0), torch.cuda.Stream()
+    c.set_stream(s)
+    torch.cuda.synchronize()
+    b.run(c)
+    torch.cuda.synchronize()
+    held = []
+    for _ in range(6):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            b.run(c)
+            b.run(c)
+        b.out.fill_(77.0)
+        torch.cuda.synchronize()
+        g.replay()
+        b.check()
+        held.append(c.scratch_bytes())
+        del g
+        gc.collect()
+        time.sleep(0.05)  # the release comes from a thread of the driver
+    assert held[0] == held[-1], held
+    c.close()
