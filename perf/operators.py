@@ -7,6 +7,7 @@ Head counts, hidden sizes and vocabularies are those of the benchmark's decoder,
 generic ones.
 """
 import math
+import threading
 
 import numpy as np
 import torch
@@ -216,14 +217,14 @@ _ctx = {}
 
 
 def _context():
-    """The library's context on the current device, enqueuing on torch's current stream."""
+    """This thread's library context on the current device, enqueuing on torch's current stream."""
     from laguna_raw_halo_strix_b200 import lc
 
-    d = torch.cuda.current_device()
-    if d not in _ctx:
-        _ctx[d] = lc.Context(d)
-    _ctx[d].set_stream(torch.cuda.current_stream())
-    return lc, _ctx[d]
+    at = threading.get_ident(), torch.cuda.current_device()
+    if at not in _ctx:
+        _ctx[at] = lc.Context(at[1])
+    _ctx[at].set_stream(torch.cuda.current_stream())
+    return lc, _ctx[at]
 
 
 def run(state):
