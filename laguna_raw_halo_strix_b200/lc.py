@@ -196,6 +196,38 @@ class TargetHParams(C.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+_i32 = _f32 = None  # torch's types, once a tensor has been given
+
+
+def _check_lists(ints, floats, what: str) -> None:
+    """Lists that the library reads as packed int32 and float32: tensors have to be that (addresses and None pass)."""
+    try:
+        for t in ints:
+            if t is not None and not (t.dtype is _i32 and t.is_contiguous()):
+                break
+        else:
+            for t in floats:
+                if t is not None and not (t.dtype is _f32 and t.is_contiguous()):
+                    break
+            else:
+                return
+    except AttributeError:  # an address
+        pass
+    _find_bad_list(ints, floats, what)
+
+
+def _find_bad_list(ints, floats, what: str) -> None:
+    global _i32, _f32
+    import torch
+
+    _i32, _f32 = torch.int32, torch.float32
+    for lists, dtypes in ((ints, (_i32, torch.uint32)), (floats, (_f32,))):
+        for t in lists:
+            if hasattr(t, "dtype") and (t.dtype not in dtypes or not t.is_contiguous()):
+                raise LagunaError(LC_ERR_INVALID, f"{what}: a list of {t.dtype} with shape {tuple(t.shape)} and strides "
+                                                  f"{tuple(t.stride())} is read as packed {dtypes[0]}")
+
+
 class PrefixKV(C.Structure):
     """lc_prefix_kv (include/laguna_cuda.h): the shared prefix and the sequences' own K/V rows.  Holds the tensors."""
 
@@ -205,6 +237,7 @@ class PrefixKV(C.Structure):
 
     def __init__(self, k_prefix, v_prefix, prefix_len, k_own, v_own, own_cap, own_len, seq_start, n_seqs, ld_prefix=0,
                  ld_own=0, own_stride=0):
+        _check_lists((own_len, seq_start), (), "PrefixKV")
         super().__init__(ptr(k_prefix), ptr(v_prefix), ld_prefix, prefix_len, own_cap, ptr(k_own), ptr(v_own), ld_own,
                          own_stride, ptr(own_len), ptr(seq_start), n_seqs)
         self.held = (k_prefix, v_prefix, k_own, v_own, own_len, seq_start)
@@ -213,7 +246,8 @@ class PrefixKV(C.Structure):
 class LogitsRules(C.Structure):
     """lc_logits_rules (include/laguna_cuda.h), from tensors: the lengths of the
     lists and the shape of the masks [n_masks, words] are read off them (a list
-    given as an int address needs its length beside it).  Holds the tensors."""
+    given as an int address needs its length beside it).  Lists are packed int32
+    or float32 tensors, masks rows of packed 32-bit words.  Holds the tensors."""
 
     _fields_ = [("hist", _vp), ("hist_start", _vp), ("gen_start", _vp), ("hist_len", _u64),
                 ("repetition", _vp), ("frequency", _vp), ("presence", _vp),
@@ -227,8 +261,16 @@ class LogitsRules(C.Structure):
             hist_len = 0 if hist is None else hist.numel()
         if bias_len is None:
             bias_len = 0 if bias_tok is None else bias_tok.numel()
+            if bias_len and hasattr(bias, "numel") and bias.numel() < bias_len:
+                raise LagunaError(LC_ERR_INVALID, f"LogitsRules: {bias.numel()} biases for {bias_len} tokens")
         if mask is not None and (mask_ld is None or n_masks is None):
+            if mask.ndim != 2 or mask.stride(1) != 1 or (mask.dtype is not _i32 and
+                                                         str(mask.dtype) not in ("torch.int32", "torch.uint32")):
+                raise LagunaError(LC_ERR_INVALID, f"LogitsRules: mask of {mask.dtype} with shape {tuple(mask.shape)} and "
+                                                  f"strides {mask.stride()} is read as rows of packed 32-bit words")
             n_masks, mask_ld = mask.shape[0], mask.stride(0)
+        _check_lists((hist, hist_start, gen_start, bias_tok, bias_start, mask_row),
+                     (repetition, frequency, presence, bias), "LogitsRules")
         super().__init__(ptr(hist), ptr(hist_start), ptr(gen_start), hist_len, ptr(repetition), ptr(frequency),
                          ptr(presence), ptr(bias_tok), ptr(bias), ptr(bias_start), bias_len, ptr(mask), ptr(mask_row),
                          mask_ld or 0, n_masks or 0)
@@ -405,6 +447,7 @@ class Context:
     def rope(self, dtype, out_dtype, layout, q, q_out, n_q_heads, k, k_out, n_kv_heads, pos, freq, m, head_dim,
              rope_dim, scale=1.0, ldq=0, ldq_out=0, ldk=0, ldk_out=0):
         """lc_rope: q and k (either may be None with 0 heads) rotated at pos[row]; strides in elements, 0 = packed."""
+        _check_lists((pos,), (freq,), "rope")
         status = self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k),
                                 ldk, ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale)
         if status:

@@ -64,3 +64,33 @@ def test_restatement_by_hand():
     # 0: seen twice, generated once; 1: prompt only; 2: the later bias; 3: masked; 4: bias
     assert out[0].tolist() == [2 / 2 - 0.25 - 0.5, -4.0, 1.5, -np.inf, 1.5]
     assert best[0] == 4  # the larger of two equal ones
+
+
+def test_lists_of_another_type_or_with_gaps_are_refused():
+    import torch
+
+    good = dict(hist=torch.zeros(8, dtype=torch.int32), hist_start=torch.zeros(4, dtype=torch.int32),
+                gen_start=torch.zeros(3, dtype=torch.int32), repetition=torch.ones(3), frequency=torch.ones(3),
+                presence=torch.ones(3), bias_tok=torch.zeros(5, dtype=torch.int32), bias=torch.ones(5),
+                bias_start=torch.zeros(4, dtype=torch.int32), mask=torch.zeros(2, 6, dtype=torch.int32)[:, :5],
+                mask_row=torch.zeros(3, dtype=torch.int32))
+    r = lc.LogitsRules(**good)
+    assert (r.hist_len, r.bias_len, r.n_masks, r.mask_ld) == (8, 5, 2, 6)
+    assert r.hist == good["hist"].data_ptr() and r.presence == good["presence"].data_ptr()
+    for name, t in good.items():
+        wrong = t.long() if t.dtype == torch.int32 else t.double()
+        gaps = torch.stack([t, t], -1)[..., 0]
+        assert torch.equal(gaps, t) and not gaps.is_contiguous()
+        half = t.short() if t.dtype == torch.int32 else t.bfloat16()
+        for bad in (wrong, gaps, half):
+            with pytest.raises(lc.LagunaError, match="read as") as e:
+                lc.LogitsRules(**{**good, name: bad})
+            assert e.value.status == lc.LC_ERR_INVALID
+    with pytest.raises(lc.LagunaError, match="biases for"):
+        lc.LogitsRules(**{**good, "bias": torch.ones(4)})
+    with pytest.raises(lc.LagunaError, match="read as"):
+        lc.LogitsRules(**{**good, "mask": torch.zeros(5, dtype=torch.int32)})
+    # addresses, unsigned words and missing rules pass
+    lc.LogitsRules(hist=0x1000, hist_start=good["hist_start"], hist_len=3, mask=0x2000, mask_ld=4, n_masks=2)
+    lc.LogitsRules(mask=torch.zeros(2, 6, dtype=torch.uint32), hist=torch.zeros(3, dtype=torch.uint32))
+    lc.LogitsRules()

@@ -50,3 +50,17 @@ def test_nothing_to_do_and_null_context():
     s = lc.PrefixKV(None, None, 0, None, None, 0, None, None, 0)
     assert lc.lib().lc_prefix_attn(None, lc.F16, lc.F16, None, 0, C.byref(s), None, 0, 1, 8, 8, 64, 1.0, 1) == \
         lc.LC_ERR_INVALID
+
+
+def test_lengths_of_another_type_or_with_gaps_are_refused():
+    import torch
+
+    good = dict(own_len=torch.zeros(3, dtype=torch.int32), seq_start=torch.zeros(4, dtype=torch.int32))
+    args = dict(k_prefix=0x1000, v_prefix=0x2000, prefix_len=4, k_own=0x3000, v_own=0x4000, own_cap=5, n_seqs=3)
+    assert lc.PrefixKV(**args, **good).own_len == good["own_len"].data_ptr()
+    lc.PrefixKV(**args, own_len=0x5000, seq_start=0x6000)
+    for name, t in good.items():
+        for bad in (t.long(), t.float(), torch.stack([t, t], -1)[:, 0]):
+            with pytest.raises(lc.LagunaError, match="read as") as e:
+                lc.PrefixKV(**args, **{**good, name: bad})
+            assert e.value.status == lc.LC_ERR_INVALID

@@ -106,3 +106,22 @@ def test_nothing_to_do_and_null_context():
     assert call(n_q=0, n_kv=0, q=None, k=None, q_out=None, k_out=None) == lc.LC_OK
     assert lc.lib().lc_rope(None, 0, 0, 0, None, 0, None, 0, 0, None, 0, None, 0, 0, None, None, 1, 128, 128,
                             1.0) == lc.LC_ERR_INVALID
+
+
+def test_positions_of_another_type_or_with_gaps_are_refused():
+    import torch
+
+    c = lc.Context.__new__(lc.Context)  # without a device: lc_rope refuses its null context
+    c.L, c.h = lc.lib(), None
+    good = dict(pos=torch.zeros(3, dtype=torch.int32), freq=torch.ones(4))
+
+    def call(pos, freq):
+        c.rope(lc.F32, lc.F32, lc.ROPE_HALF, 0x1000, 0x1000, 1, None, None, 0, pos, freq, 3, 8, 8)
+
+    with pytest.raises(lc.LagunaError, match="null ctx"):
+        call(**good)
+    for name, t in good.items():
+        for bad in (t.long(), t.double(), torch.stack([t, t], -1)[:, 0]):
+            with pytest.raises(lc.LagunaError, match="read as") as e:
+                call(**{**good, name: bad})
+            assert e.value.status == lc.LC_ERR_INVALID
