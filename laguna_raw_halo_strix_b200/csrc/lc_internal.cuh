@@ -107,10 +107,17 @@ int lc_use_device(lc_ctx *ctx);
 // driver again.
 int lc_set_smem_attr(const void *kernel, size_t bytes);
 
-// Do the m rows of wa bytes, pa apart, at a share a byte with the m rows of wb
-// bytes, pb apart, at b?  Exact for equal pitches (columns of one buffer);
-// otherwise whole extents are compared.
-bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m);
+// Rows of `width` bytes, `pitch` apart.
+struct LcRows {
+    const void *at;
+    uint64_t pitch, width, rows;
+};
+// Do the rows of a share a byte with those of b?  Exact for equal pitches (columns of one
+// buffer) or a single row; otherwise whole extents are compared.
+bool lc_rows_meet(LcRows a, LcRows b);
+inline bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
+    return lc_rows_meet({a, pa, wa, m}, {b, pb, wb, m});
+}
 
 #define LC_REQUIRE(cond, code, ...)             \
     do {                                        \

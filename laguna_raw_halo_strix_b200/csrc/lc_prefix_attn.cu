@@ -1165,8 +1165,23 @@ extern "C" int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void 
                    (((uintptr_t)kv->seq_start | (uintptr_t)kv->own_len) & 3) == 0,
                LC_ERR_INVALID, "lc_prefix_attn: rows must start on 16-byte boundaries");
     const uint64_t bo = out_dtype == LC_F32 ? 4 : 2;
+    const LcRows out_rows = {out, ldo * bo, wq * bo, rows};
     LC_REQUIRE(!lc_rows_meet(q, ldq * 2, wq * 2, out, ldo * bo, wq * bo, rows), LC_ERR_INVALID,
                "lc_prefix_attn: out overlaps q");
+    for (const void *p : {kv->k_prefix, kv->v_prefix})
+        LC_REQUIRE(!lc_rows_meet({p, ldp * 2, wk * 2, kv->prefix_len}, out_rows), LC_ERR_INVALID,
+                   "lc_prefix_attn: out overlaps the prefix");
+    for (const void *p : {kv->k_own, kv->v_own}) {
+        // the sequences' extents against out's, then (columns of one buffer) row by row
+        const uint64_t extent = kv->own_cap ? ((kv->own_cap - 1) * ldw + wk) * 2 : 0;
+        if (!lc_rows_meet({p, seq_ld * 2, extent, kv->n_seqs}, {out, 0, (rows - 1) * ldo * bo + wq * bo, 1})) continue;
+        for (uint32_t i = 0; i < kv->n_seqs; i++)
+            LC_REQUIRE(!lc_rows_meet({(const char *)p + i * seq_ld * 2, ldw * 2, wk * 2, kv->own_cap}, out_rows),
+                       LC_ERR_INVALID, "lc_prefix_attn: out overlaps the own rows of sequence %u", i);
+    }
+    LC_REQUIRE(!lc_rows_meet({kv->seq_start, 0, 4 * (kv->n_seqs + 1ull), 1}, out_rows) &&
+                   (!kv->own_cap || !lc_rows_meet({kv->own_len, 0, 4ull * kv->n_seqs, 1}, out_rows)),
+               LC_ERR_INVALID, "lc_prefix_attn: out overlaps lengths or starts");
     if (int s = lc_use_device(ctx)) return s;
 
     PaArgs a = {};

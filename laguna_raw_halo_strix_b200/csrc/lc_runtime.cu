@@ -170,20 +170,23 @@ int lc_set_smem_attr(const void *kernel, size_t bytes) {
     return LC_OK;
 }
 
-bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
-    const intptr_t d = (intptr_t)b - (intptr_t)a;
-    if (pa != pb || m == 1) {
-        const uint64_t ea = (m - 1) * pa + wa, eb = (m - 1) * pb + wb;
-        return d < (intptr_t)ea && -d < (intptr_t)eb;
+bool lc_rows_meet(LcRows a, LcRows b) {
+    if (!a.rows || !b.rows || !a.width || !b.width) return false;
+    if (a.rows == 1) a.pitch = b.pitch;
+    if (b.rows == 1) b.pitch = a.pitch;
+    using Wide = __int128;
+    const Wide d = (Wide)(uintptr_t)b.at - (Wide)(uintptr_t)a.at;
+    if (a.pitch != b.pitch || !a.pitch) {
+        const Wide ea = (Wide)(a.rows - 1) * a.pitch + a.width, eb = (Wide)(b.rows - 1) * b.pitch + b.width;
+        return d < ea && -d < eb;
     }
-    // row i of a and row i + j of b start d + j * pa apart: overlap if that is in (-wb, wa)
-    const intptr_t p = (intptr_t)pa;
-    const intptr_t j0 = d >= 0 ? -(d / p) : (-d + p - 1) / p;  // d + j0 * p in [0, p)
-    for (intptr_t j = j0 - 1; j <= j0; j++) {
-        const intptr_t at = d + j * p;
-        if (j < (intptr_t)m && -j < (intptr_t)m && at < (intptr_t)wa && -at < (intptr_t)wb) return true;
-    }
-    return false;
+    // row i of a and row i + j of b start d + j * pitch apart: they meet if that is in
+    // (-b.width, a.width)
+    const Wide p = a.pitch;
+    auto down = [&](Wide v) { return v >= 0 ? v / p : -((-v + p - 1) / p); };
+    const Wide first = std::max(down(-(Wide)b.width - d) + 1, -(Wide)(a.rows - 1));
+    const Wide last = std::min(down((Wide)a.width - d - 1), (Wide)(b.rows - 1));
+    return first <= last;
 }
 
 int lc_after_launch(lc_ctx *ctx, const char *what) {

@@ -1,6 +1,8 @@
 """lc_prefix_attn without a GPU: its refusals, decided from the arguments alone
 before it looks into the context, so a blank one will do."""
 import ctypes as C
+import struct
+import sys
 
 import pytest
 
@@ -64,3 +66,40 @@ def test_lengths_of_another_type_or_with_gaps_are_refused():
             with pytest.raises(lc.LagunaError, match="read as") as e:
                 lc.PrefixKV(**args, **{**good, name: bad})
             assert e.value.status == lc.LC_ERR_INVALID
+
+
+@pytest.mark.parametrize("over", [
+    dict(out=0x300000), dict(out=0x400000 + 99 * 256), dict(out=0x300000 - 3 * 1024 - 16), dict(out=0x500000),
+    dict(out=0x600000 + 3 * 50 * 256 - 16), dict(out=0x600000 - 16), dict(out=0x700000), dict(out=0x7ff010),
+    dict(out=0x800000),
+    dict(kv=dict(ld_prefix=640), ldo=640, out=0x300000 + 3 * 1280 + 240),    # columns that reach into k
+    dict(kv=dict(ld_own=640), ldo=640, out=0x500000 + 2 * 1280 + 240),
+    dict(kv=dict(own_stride=51200), out=0x500000 + 2 * 102400 - 1024),      # the next sequence's first row
+], ids=str)
+def test_out_over_what_is_read_is_refused(over):
+    assert call(**over) == lc.LC_ERR_INVALID
+    assert "overlaps" in lc.last_error()
+
+
+def meet_by_bytes(a, b):
+    """Rows (at, pitch, width, rows) that share a byte, byte by byte."""
+    def cells(r):
+        return {r[0] + i * r[1] + j for i in range(r[3]) for j in range(r[2])}
+    return bool(cells(a) & cells(b))
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_out_beside_what_is_read_passes_the_check(monkeypatch, own):
+    """Out moved through the rows of a buffer that also holds k: refused exactly where a byte is shared.  (The
+    others get as far as the context's device, which does not exist.)"""
+    monkeypatch.setattr(sys.modules[__name__], "BLANK", C.create_string_buffer(struct.pack("i", 1 << 20), 4096))
+    refused = passed = 0
+    for at in range(-2560, 4 * 1280 + 1, 80):
+        base = 0x500000 if own else 0x300000
+        kv = dict(ld_own=640, prefix_len=0) if own else dict(ld_prefix=640, own_cap=0)
+        rows = (3 * 50, 1280, 256) if own else (100, 1280, 256)
+        s = call(rows=2, n_q=2, n_kv=2, hd=64, ldo=640, out=base + at, kv=kv)
+        meets = meet_by_bytes((0, rows[1], rows[2], 6), (at, 1280, 256, 2))
+        assert s == (lc.LC_ERR_INVALID if meets else lc.LC_ERR_CUDA) and ("overlaps" in lc.last_error()) == meets, at
+        refused, passed = refused + meets, passed + (not meets)
+    assert refused and passed
