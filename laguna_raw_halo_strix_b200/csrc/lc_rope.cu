@@ -355,6 +355,11 @@ extern "C" int lc_rope(lc_ctx *ctx, int dtype, int out_dtype, int layout, const 
                         lc_rows_meet(q, ldq * bi, wq * bi, k_out, ldk_out * bo, wk * bo, m) ||
                         lc_rows_meet(k, ldk * bi, wk * bi, q_out, ldq_out * bo, wq * bo, m)));
     LC_REQUIRE(!meet, LC_ERR_INVALID, "lc_rope: an output overlaps another tensor (only y = x in place is possible)");
+    const LcRows outs[2] = {{q_out, ldq_out * bo, wq * bo, m}, {k_out, ldk_out * bo, wk * bo, m}};
+    if (rope_dim)
+        for (const LcRows &y : outs)
+            LC_REQUIRE(!lc_rows_meet({pos, 0, 4ull * m, 1}, y) && !lc_rows_meet({freq, 0, 2ull * rope_dim, 1}, y),
+                       LC_ERR_INVALID, "lc_rope: an output overlaps pos or freq");
     RpArgs a = {};
     a.x[0] = q, a.x[1] = k, a.y[0] = q_out, a.y[1] = k_out;
     a.ldx[0] = ldq, a.ldx[1] = ldk, a.ldy[0] = ldq_out, a.ldy[1] = ldk_out;

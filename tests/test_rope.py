@@ -125,3 +125,24 @@ def test_positions_of_another_type_or_with_gaps_are_refused():
             with pytest.raises(lc.LagunaError, match="read as") as e:
                 call(**{**good, name: bad})
             assert e.value.status == lc.LC_ERR_INVALID
+
+
+@pytest.mark.parametrize("over", [
+    dict(pos=0x20000 + 2044), dict(pos=0x20000 - 12), dict(pos=0x40000 + 256 * 3), dict(freq=0x20000 + 512),
+    dict(freq=0x40000 - 4 * 31), dict(ldq_out=200, pos=0x20000 + 800 * 3 + 508), dict(n_q=0, freq=0x40000),
+    dict(n_kv=0, pos=0x20000)], ids=str)
+def test_outputs_over_positions_or_frequencies_are_refused(over):
+    assert call(**over) == lc.LC_ERR_INVALID
+    assert "pos or freq" in lc.last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(pos=0x20000 + 2048), dict(pos=0x20000 - 16), dict(ldq_out=200, pos=0x20000 + 512),
+    dict(ldq_out=200, freq=0x20000 + 800 + 512), dict(rope_dim=0, pos=0x20000, freq=0x40000)], ids=str)
+def test_positions_beside_outputs_pass_the_check(monkeypatch, over):
+    """They get as far as the context's device, which does not exist."""
+    import struct
+    import sys
+
+    monkeypatch.setattr(sys.modules[__name__], "BLANK", C.create_string_buffer(struct.pack("i", 1 << 20), 4096))
+    assert call(**over) == lc.LC_ERR_CUDA
