@@ -373,8 +373,8 @@ typedef struct {
  * the row's best token, beside lc_argmax_rows; in this order, each operation
  * rounded once to f32: repetition, frequency * count, presence, bias, masked
  * tokens to -inf.  ld / ld_out: floats between rows (0: n).  out may be logits
- * itself (same stride), or NULL when only keys are wanted; other overlaps are
- * LC_ERR_INVALID.  keys[m] (optional) get lc_pack_key(max, token), ties to the
+ * itself (same stride), or NULL when only keys are wanted; other overlaps of out
+ * or keys with anything are LC_ERR_INVALID.  keys[m] (optional) get lc_pack_key(max, token), ties to the
  * larger token; a row with every token masked has (-inf, its last token).
  * Vocab shards: the rows hold tokens row_offset .. row_offset + n - 1; token ids
  * in lists and mask bits stay global, ids outside the shard are skipped, and

@@ -622,6 +622,23 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     LC_REQUIRE(!out || (out == logits && ld == ld_out) ||
                    !lc_rows_meet(logits, ld * 4, n * 4ull, out, ld_out * 4, n * 4ull, m),
                LC_ERR_INVALID, "lc_logits_process: out overlaps logits (only out = logits in place is possible)");
+    const LcRows key_span = {keys, 0, keys ? 8ull * m : 0, 1}, out_rows = {out, ld_out * 4, out ? n * 4ull : 0, m};
+    LC_REQUIRE(!lc_rows_meet(key_span, {logits, ld * 4, n * 4ull, m}) && !lc_rows_meet(key_span, out_rows),
+               LC_ERR_INVALID, "lc_logits_process: keys overlap the logits");
+    const struct {
+        const void *at;
+        uint64_t entries;
+    } read[] = {{r.hist, r.hist_len}, {r.hist_start, m + 1ull}, {r.gen_start, m}, {r.repetition, m}, {r.frequency, m},
+                {r.presence, m}, {r.bias_tok, r.bias_len}, {r.bias, r.bias_len}, {r.bias_start, m + 1ull},
+                {r.mask_row, m}};
+    for (const auto &l : read) {
+        const LcRows span = {l.at, 0, l.at ? 4 * l.entries : 0, 1};
+        LC_REQUIRE(!lc_rows_meet(span, out_rows) && !lc_rows_meet(span, key_span), LC_ERR_INVALID,
+                   "lc_logits_process: an output overlaps a list");
+    }
+    const LcRows masks = {r.mask, r.mask_ld * 4, r.mask ? words * 4 : 0, r.n_masks};
+    LC_REQUIRE(!lc_rows_meet(masks, out_rows) && !lc_rows_meet(masks, key_span), LC_ERR_INVALID,
+               "lc_logits_process: an output overlaps the masks");
     if (int s = lc_use_device(ctx)) return s;
     LgArgs a = {};
     a.x = logits, a.y = out, a.ldx = ld, a.ldy = ld_out, a.m = m, a.n = n, a.row_offset = row_offset;

@@ -94,3 +94,40 @@ def test_lists_of_another_type_or_with_gaps_are_refused():
     lc.LogitsRules(hist=0x1000, hist_start=good["hist_start"], hist_len=3, mask=0x2000, mask_ld=4, n_masks=2)
     lc.LogitsRules(mask=torch.zeros(2, 6, dtype=torch.uint32), hist=torch.zeros(3, dtype=torch.uint32))
     lc.LogitsRules()
+
+
+LISTS = dict(hist=0x400000, hist_start=0x410000, hist_len=10, gen_start=0x420000, repetition=0x430000, frequency=0x440000,
+             presence=0x450000, bias_tok=0x460000, bias=0x470000, bias_start=0x480000, bias_len=7, mask=0x490000,
+             mask_row=0x4a0000, mask_ld=4, n_masks=3)
+
+
+@pytest.mark.parametrize("name", [k for k, v in LISTS.items() if v > 1000])
+@pytest.mark.parametrize("output", ["out", "keys"])
+def test_outputs_over_lists_are_refused(name, output):
+    entries = {"hist": 10, "hist_start": 5, "bias_start": 5, "bias_tok": 7, "bias": 7, "mask": 12}.get(name, 4)
+    last = LISTS[name] + 4 * entries - 4
+    if output == "keys":
+        last &= ~7
+    for at in (LISTS[name], last):
+        assert call(rules=LISTS, **{output: at}) == lc.LC_ERR_INVALID
+        assert "overlaps" in lc.last_error()
+
+
+@pytest.mark.parametrize("over", [dict(keys=0x100000), dict(keys=0x200000 + 1592), dict(keys=0x100000 - 24),
+                                  dict(ld=120, keys=0x100000 + 480 * 3 + 392), dict(keys=0x200000 - 8, out=0x200010)],
+                         ids=str)
+def test_keys_over_logits_are_refused(over):
+    assert call(**over) == lc.LC_ERR_INVALID
+    assert "keys overlap" in lc.last_error()
+
+
+@pytest.mark.parametrize("over", [dict(keys=0x100000 - 32), dict(keys=0x200000 + 1600), dict(ld=120, m=2, keys=0x100000 + 400),
+                                  dict(out=0x400028, keys=None), dict(out=0x410014), dict(out=None, keys=0x490030),
+                                  dict(out=0x100000)], ids=str)
+def test_outputs_beside_what_is_read_pass_the_check(monkeypatch, over):
+    """They get as far as the context's device, which does not exist."""
+    import struct
+    import sys
+
+    monkeypatch.setattr(sys.modules[__name__], "BLANK", C.create_string_buffer(struct.pack("i", 1 << 20), 4096))
+    assert call(rules=LISTS, **over) == lc.LC_ERR_CUDA
