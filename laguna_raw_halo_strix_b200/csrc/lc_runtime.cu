@@ -176,10 +176,9 @@ bool lc_rows_meet(LcRows a, LcRows b) {
     if (b.rows == 1) b.pitch = a.pitch;
     using Wide = __int128;
     const Wide d = (Wide)(uintptr_t)b.at - (Wide)(uintptr_t)a.at;
-    if (a.pitch != b.pitch || !a.pitch) {
-        const Wide ea = (Wide)(a.rows - 1) * a.pitch + a.width, eb = (Wide)(b.rows - 1) * b.pitch + b.width;
-        return d < ea && -d < eb;
-    }
+    const Wide ea = (Wide)(a.rows - 1) * a.pitch + a.width, eb = (Wide)(b.rows - 1) * b.pitch + b.width;
+    if (d >= ea || -d >= eb) return false;
+    if (a.pitch != b.pitch || !a.pitch) return true;
     // row i of a and row i + j of b start d + j * pitch apart: they meet if that is in
     // (-b.width, a.width)
     const Wide p = a.pitch;
