@@ -224,3 +224,66 @@ def test_captured_among_copies_and_forks(dev):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,n", [(6, 9000), (400, 3001)])
+@pytest.mark.parametrize("forked", [False, True])
+def test_rules_that_the_node_before_writes(dev, rows, n, forked):
+    """Every list and the logits are filled by the nodes right before the rules' kernel, on its stream and on
+    another one, from what each replay finds; against the restatement."""
+    import torch
+
+    rng = np.random.default_rng(rows)
+    sizes = rng.integers(0, 60, rows)
+    start = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    words = (n + 31) // 32
+
+    def inputs(seed):
+        r = np.random.default_rng(seed)
+        return dict(x=(3 * r.standard_normal((rows, n))).astype(np.float32),
+                    hist=r.integers(0, n, start[-1]).astype(np.int32), hist_start=start,
+                    gen_start=(start[:-1] + r.integers(0, sizes + 1)).astype(np.int32),
+                    repetition=r.uniform(0.7, 1.5, rows).astype(np.float32),
+                    frequency=r.uniform(-0.5, 1, rows).astype(np.float32),
+                    presence=r.uniform(-0.5, 1, rows).astype(np.float32),
+                    bias_tok=r.integers(0, n, start[-1]).astype(np.int32), bias_start=start,
+                    bias=r.standard_normal(start[-1]).astype(np.float32),
+                    mask=r.integers(0, 2 ** 32, (3, words), dtype=np.uint32).view(np.int32),
+                    mask_row=r.integers(-1, 3, rows).astype(np.int32))
+
+    given = {k: to_dev(v, dev) for k, v in inputs(0).items()}
+    held = {k: torch.zeros_like(v) for k, v in given.items()}
+    out, keys = torch.empty(rows, n, device=dev), torch.empty(rows, device=dev, dtype=torch.int64)
+    rules = lc.LogitsRules(**{k: v for k, v in held.items() if k != "x"})
+    c, main, side = lc.Context(0), torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step():
+        mine = torch.cuda.current_stream()
+        late = side if forked else mine
+        for k in held:
+            held[k].zero_()  # what a kernel that ran too early would find
+        late.wait_stream(mine)
+        with torch.cuda.stream(late):
+            for k in held:
+                held[k].copy_(given[k])
+        mine.wait_stream(late)
+        c.set_stream(mine)
+        c.logits_process(held["x"], rules, out, keys, rows, n)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        step()
+    for seed in range(1, 5):
+        new = inputs(seed)
+        for k, v in new.items():
+            given[k].copy_(torch.from_numpy(v))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        x, new["mask"] = new.pop("x"), new["mask"].view(np.uint32)
+        want, _, best = logits_ref.process(x, **new)
+        assert np.array_equal(out.cpu().numpy().view(np.uint32), want.view(np.uint32))
+        assert [lc.key_index(int(k)) for k in keys] == best.tolist()
+    del graph
+    c.close()
