@@ -199,33 +199,28 @@ class TargetHParams(C.Structure):
 _i32 = _f32 = None  # torch's types, once a tensor has been given
 
 
-def _check_lists(ints, floats, what: str) -> None:
-    """Lists that the library reads as packed int32 and float32: tensors have to be that (addresses and None pass)."""
+def _lists(ints, floats, what: str):
+    """Addresses of lists that the library reads as packed int32 and float32: tensors have to be that (addresses and
+    None pass)."""
     try:
-        for t in ints:
-            if t is not None and not (t.dtype is _i32 and t.is_contiguous()):
-                break
-        else:
-            for t in floats:
-                if t is not None and not (t.dtype is _f32 and t.is_contiguous()):
-                    break
-            else:
-                return
-    except AttributeError:  # an address
-        pass
-    _find_bad_list(ints, floats, what)
+        return [0 if t is None else t.data_ptr() if t.dtype is _i32 and t.is_contiguous() else _list(t, 0, what)
+                for t in ints] + \
+               [0 if t is None else t.data_ptr() if t.dtype is _f32 and t.is_contiguous() else _list(t, 1, what)
+                for t in floats]
+    except AttributeError:  # an address among them
+        return [_list(t, 0, what) for t in ints] + [_list(t, 1, what) for t in floats]
 
 
-def _find_bad_list(ints, floats, what: str) -> None:
+def _list(t, kind: int, what: str):
     global _i32, _f32
     import torch
 
     _i32, _f32 = torch.int32, torch.float32
-    for lists, dtypes in ((ints, (_i32, torch.uint32)), (floats, (_f32,))):
-        for t in lists:
-            if hasattr(t, "dtype") and (t.dtype not in dtypes or not t.is_contiguous()):
-                raise LagunaError(LC_ERR_INVALID, f"{what}: a list of {t.dtype} with shape {tuple(t.shape)} and strides "
-                                                  f"{tuple(t.stride())} is read as packed {dtypes[0]}")
+    good = ((_i32, torch.uint32), (_f32,))[kind]
+    if hasattr(t, "dtype") and (t.dtype not in good or not t.is_contiguous()):
+        raise LagunaError(LC_ERR_INVALID, f"{what}: a list of {t.dtype} with shape {tuple(t.shape)} and strides "
+                                          f"{tuple(t.stride())} is read as packed {good[0]}")
+    return ptr(t)
 
 
 class PrefixKV(C.Structure):
@@ -237,9 +232,8 @@ class PrefixKV(C.Structure):
 
     def __init__(self, k_prefix, v_prefix, prefix_len, k_own, v_own, own_cap, own_len, seq_start, n_seqs, ld_prefix=0,
                  ld_own=0, own_stride=0):
-        _check_lists((own_len, seq_start), (), "PrefixKV")
         super().__init__(ptr(k_prefix), ptr(v_prefix), ld_prefix, prefix_len, own_cap, ptr(k_own), ptr(v_own), ld_own,
-                         own_stride, ptr(own_len), ptr(seq_start), n_seqs)
+                         own_stride, *_lists((own_len, seq_start), (), "PrefixKV"), n_seqs)
         self.held = (k_prefix, v_prefix, k_own, v_own, own_len, seq_start)
 
 
@@ -264,16 +258,16 @@ class LogitsRules(C.Structure):
             if bias_len and hasattr(bias, "numel") and bias.numel() < bias_len:
                 raise LagunaError(LC_ERR_INVALID, f"LogitsRules: {bias.numel()} biases for {bias_len} tokens")
         if mask is not None and (mask_ld is None or n_masks is None):
-            if mask.ndim != 2 or mask.stride(1) != 1 or (mask.dtype is not _i32 and
-                                                         str(mask.dtype) not in ("torch.int32", "torch.uint32")):
-                raise LagunaError(LC_ERR_INVALID, f"LogitsRules: mask of {mask.dtype} with shape {tuple(mask.shape)} and "
-                                                  f"strides {mask.stride()} is read as rows of packed 32-bit words")
-            n_masks, mask_ld = mask.shape[0], mask.stride(0)
-        _check_lists((hist, hist_start, gen_start, bias_tok, bias_start, mask_row),
-                     (repetition, frequency, presence, bias), "LogitsRules")
-        super().__init__(ptr(hist), ptr(hist_start), ptr(gen_start), hist_len, ptr(repetition), ptr(frequency),
-                         ptr(presence), ptr(bias_tok), ptr(bias), ptr(bias_start), bias_len, ptr(mask), ptr(mask_row),
-                         mask_ld or 0, n_masks or 0)
+            shape, strides, dtype = mask.shape, mask.stride(), mask.dtype
+            if len(shape) != 2 or strides[1] != 1 or (dtype is not _i32 and
+                                                      str(dtype) not in ("torch.int32", "torch.uint32")):
+                raise LagunaError(LC_ERR_INVALID, f"LogitsRules: mask of {dtype} with shape {tuple(shape)} and strides "
+                                                  f"{strides} is read as rows of packed 32-bit words")
+            n_masks, mask_ld = shape[0], strides[0]
+        at = _lists((hist, hist_start, gen_start, bias_tok, bias_start, mask_row),
+                    (repetition, frequency, presence, bias), "LogitsRules")
+        super().__init__(at[0], at[1], at[2], hist_len, at[6], at[7], at[8], at[3], at[9], at[4], bias_len, ptr(mask),
+                         at[5], mask_ld or 0, n_masks or 0)
         self.held = (hist, hist_start, gen_start, repetition, frequency, presence, bias_tok, bias, bias_start, mask,
                      mask_row)
 
@@ -447,9 +441,9 @@ class Context:
     def rope(self, dtype, out_dtype, layout, q, q_out, n_q_heads, k, k_out, n_kv_heads, pos, freq, m, head_dim,
              rope_dim, scale=1.0, ldq=0, ldq_out=0, ldk=0, ldk_out=0):
         """lc_rope: q and k (either may be None with 0 heads) rotated at pos[row]; strides in elements, 0 = packed."""
-        _check_lists((pos,), (freq,), "rope")
         status = self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k),
-                                ldk, ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale)
+                                ldk, ptr(k_out), ldk_out, n_kv_heads, *_lists((pos,), (freq,), "rope"), m, head_dim,
+                                rope_dim, scale)
         if status:
             check(status, "lc_rope")
 
