@@ -26,9 +26,13 @@ namespace {
 
 constexpr int kRpThreads = 128;
 // Items a thread has in flight (and loads before the table is ready): 8192 rows of
-// 40 bf16 heads take 34 us with two in 8 CTAs an SM (4.9 TB/s), 5 us more with three in
-// 6; more of narrower ones gained nothing.
+// 40 bf16 heads take 34.2 us with two in 8 CTAs an SM (4.9 TB/s), 39.8 with three in 6;
+// more of narrower ones gained nothing.
 constexpr int kRpItems = 2;
+// CTAs an SM: narrow pieces of heads with copied dims need few registers and are bound
+// by what is under way (8192 rows of 16 bf16 heads, 20 of 80 dims rotated: 24.7 us with
+// 10 CTAs, 26.6 with the 9 that 53 registers leave).
+constexpr int rp_ctas(bool pairs, int v, bool copies) { return !copies || v > 4 || (v == 4 && !pairs) ? 8 : v == 4 ? 9 : 10; }
 constexpr uint32_t kRpMaxDim = 8192;  // a row's table of 32 KB
 constexpr double kRpTurn = 0.15915494309189533577, kRpTurnLost = -9.8393383375912435e-18;  // 1 / (2 pi), its rounding
 
@@ -112,7 +116,7 @@ struct RpArgs {
 // for the last where as many are left (a kernel of its own, for the copies' code costs
 // rows that are all rotated a quarter of their speed).
 template <class TI, class TO, bool PAIRS, int V, bool VEC, bool COPIES>
-__global__ void __launch_bounds__(kRpThreads, 8) rope_kernel(const RpArgs a) {
+__global__ void __launch_bounds__(kRpThreads, rp_ctas(PAIRS, V, COPIES)) rope_kernel(const RpArgs a) {
     extern __shared__ float2 cs_rows[];  // [rows][rope_dim / 2]
     const size_t row0 = (size_t)blockIdx.x * a.rows_per_cta;
     const int rows = (int)min((size_t)a.rows_per_cta, a.m - row0);
