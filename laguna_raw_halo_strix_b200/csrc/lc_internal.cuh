@@ -114,7 +114,17 @@ struct LcRows {
 };
 // Do the rows of a share a byte with those of b?  Exact for equal pitches (columns of one
 // buffer) or a single row; otherwise whole extents are compared.
-bool lc_rows_meet(LcRows a, LcRows b);
+bool lc_extents_meet(LcRows a, LcRows b);  // the answer where the extents do
+inline bool lc_rows_meet(LcRows a, LcRows b) {
+    if (!a.rows || !b.rows || !a.width || !b.width) return false;
+    auto end = [](const LcRows &r) {  // the last byte; past all memory where that does not fit
+        uint64_t e;
+        const bool out = __builtin_mul_overflow(r.rows - 1, r.pitch, &e) || __builtin_add_overflow(e, r.width - 1, &e) ||
+                         __builtin_add_overflow(e, (uint64_t)(uintptr_t)r.at, &e);
+        return out ? ~0ull : e;
+    };
+    return end(a) >= (uintptr_t)b.at && end(b) >= (uintptr_t)a.at && lc_extents_meet(a, b);
+}
 inline bool lc_rows_meet(const void *a, uint64_t pa, uint64_t wa, const void *b, uint64_t pb, uint64_t wb, uint64_t m) {
     return lc_rows_meet({a, pa, wa, m}, {b, pb, wb, m});
 }

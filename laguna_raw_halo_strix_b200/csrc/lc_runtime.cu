@@ -170,15 +170,12 @@ int lc_set_smem_attr(const void *kernel, size_t bytes) {
     return LC_OK;
 }
 
-bool lc_rows_meet(LcRows a, LcRows b) {
-    if (!a.rows || !b.rows || !a.width || !b.width) return false;
+bool lc_extents_meet(LcRows a, LcRows b) {
     if (a.rows == 1) a.pitch = b.pitch;
     if (b.rows == 1) b.pitch = a.pitch;
+    if (a.pitch != b.pitch || !a.pitch) return true;
     using Wide = __int128;
     const Wide d = (Wide)(uintptr_t)b.at - (Wide)(uintptr_t)a.at;
-    const Wide ea = (Wide)(a.rows - 1) * a.pitch + a.width, eb = (Wide)(b.rows - 1) * b.pitch + b.width;
-    if (d >= ea || -d >= eb) return false;
-    if (a.pitch != b.pitch || !a.pitch) return true;
     // row i of a and row i + j of b start d + j * pitch apart: they meet if that is in
     // (-b.width, a.width)
     const Wide p = a.pitch;
