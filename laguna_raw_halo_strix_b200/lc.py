@@ -444,9 +444,14 @@ class Context:
     def rope(self, dtype, out_dtype, layout, q, q_out, n_q_heads, k, k_out, n_kv_heads, pos, freq, m, head_dim,
              rope_dim, scale=1.0, ldq=0, ldq_out=0, ldk=0, ldk_out=0):
         """lc_rope: q and k (either may be None with 0 heads) rotated at pos[row]; strides in elements, 0 = packed."""
+        try:
+            checked = pos.dtype is _i32 and freq.dtype is _f32 and pos.is_contiguous() and freq.is_contiguous()
+        except AttributeError:  # None or addresses
+            checked = False
+        if not checked:
+            _lists((pos,), (freq,), "rope")
         status = self.L.lc_rope(self.h, dtype, out_dtype, layout, ptr(q), ldq, ptr(q_out), ldq_out, n_q_heads, ptr(k),
-                                ldk, ptr(k_out), ldk_out, n_kv_heads, *_lists((pos,), (freq,), "rope"), m, head_dim,
-                                rope_dim, scale)
+                                ldk, ptr(k_out), ldk_out, n_kv_heads, ptr(pos), ptr(freq), m, head_dim, rope_dim, scale)
         if status:
             check(status, "lc_rope")
 
