@@ -269,7 +269,9 @@ typedef struct {
  * are in out.  Lengths and starts are read on the device, so a captured call
  * can be replayed as sequences grow up to own_cap.  head_dim 64 or 128, scale
  * positive, at most 128 query heads to a KV head, ldq / ldo elements between
- * rows (0: packed), 16-byte aligned rows.  out shares no byte with q, k, v, the
+ * rows (0: packed), 16-byte aligned rows.  At most 2^20 sequences, and 2^22 work
+ * items: a KV head of a sequence is one or more (LC_ERR_UNSUPPORTED above, as with
+ * 2^20 sequences of 8 KV heads).  out shares no byte with q, k, v, the
  * lengths or the starts (LC_ERR_INVALID).
  * Partial states live in scratch of the context, a block for each stream that
  * calls it and one for each captured graph (which holds it until it is

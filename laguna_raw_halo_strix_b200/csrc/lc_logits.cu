@@ -258,10 +258,12 @@ __device__ __forceinline__ void lg_touch(const LgArgs &a, const LgLists &l, cons
 
 // Rows by the CTAs of a cluster, a part of each a CTA.  Three CTAs an SM keep 48 KB of
 // loads under way, which the 56 registers allow as long as none are spilled: shared
-// memory leaves so little L1 that a spilled one comes back from L2 (three words made
-// 256 rows of 128256 take 158 us instead of 94).  Without lists those rows take 49 us,
-// 5.4 TB/s; what lists add, to 74 us with 4096 tokens of history, 300 biases and masks
-// a row, is the list warps' time where a slice of theirs takes longer than the stream's.
+// memory leaves so little L1 that a spilled one comes back from L2 (three words took 256
+// rows of 128256 in an earlier form from 94 to 158 us).  Without lists those rows take
+// 49 us, 5.4 TB/s; what lists add, to 74 us with up to 4096 tokens of history, 100 biases
+// and masks a row (77 with 300), is the list warps' time where a slice of theirs takes
+// longer than the stream's.  Tokens that are not spread over the vocabulary cost more: 99
+// us where most have low ids, for a slice whose group has no room counts the whole history.
 __global__ void __launch_bounds__(kLgAll, 3) logits_kernel(const __grid_constant__ LgArgs a) {
     extern __shared__ __align__(16) uint32_t lg_smem[];
     __shared__ long long best_of[2][16 * kLgThreads / 32];  // of rank 0, by the row's parity
@@ -648,7 +650,8 @@ extern "C" int lc_logits_process(lc_ctx *ctx, const float *logits, uint64_t ld, 
     // Few rows, a slice a CTA and all at a time, as many CTAs a row as that allows but
     // at least 4096 tokens each (one row of 128256: 7.9 us against 11.5 in the other
     // kernel, 37 of 50021: 9.1 against 12.8; with clusters that wait for others to end
-    // 15.0; 16 rows of 32000 with 2048 each 7.4 us, with 4096 7.2).  Rows of one slice
+    // 15.0; 16 rows of 32000 with 2048 each 7.4 us, with 4096 7.2).  16 slices end at 131072
+    // tokens: one row of 151936 goes the other way, in 11.7 us.  Rows of one slice
     // with a history above an eighth of it too, which all of the CTA's threads count then
     // (512 rows of 4495 with 2000 tokens: 20 against 37; with 50 tokens on 3000, 41 against 24).
     const bool long_lists = r.hist_len > (uint64_t)m * n / 8;

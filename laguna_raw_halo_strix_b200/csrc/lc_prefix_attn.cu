@@ -20,8 +20,8 @@
 // hand-out of work, 9 loads of V, 10 issues S, 11 issues O.  K, V and S have two
 // stages: the next tile's scores are formed while the softmax warps work on this
 // one's, so that these, the longest link, do not wait (with one stage of 128 keys
-// a tile's products and softmax alternated; now 900 to 1040 TFLOP/s on a long prefix, 4
-// prompts of 512 tokens on 4096 keys in 133 us).  Two CTAs share an
+// a tile's products and softmax alternated; now 890 TFLOP/s with 4 prompts of 512 tokens on
+// 4096 f16 keys, 133 us, and 930 with one of 2048 on 32768).  Two CTAs share an
 // SM (256 TMEM columns and 100 KB each).  CTAs stay for several items: the next
 // one's Q and K are loaded while the last one's values and results are worked on.
 #include <float.h>
@@ -440,9 +440,9 @@ __global__ void __launch_bounds__(kPaThreads, 2)
     // own 32 scores, and the third, where there is one, takes the second stage's place
     constexpr int kStages = kPlanes < 3 ? 2 : 1;
     // Tiles whose products are summed in TMEM.  The tensor cores' f32 sums drop what lies
-    // below the last bit, 1.7e-8 of O a product, so for f32 outputs O is added to a sum in
-    // memory after that many (998 rows of 8 heads on 5884 + 431 bf16 keys: 9e-7 off and
-    // 238 us; with 25 tiles in one sum 5.3e-6 and 212 us)
+    // below the last bit, always downwards, so for f32 outputs O is added to a sum in
+    // memory after that many (998 rows of 8/8 heads of 128 on 5884 + 431 bf16 keys: 9.6e-7
+    // off and 131 us; with an item's tiles in one sum 5.2e-6 and 113 us)
     constexpr int kRun = kPlanes > 1 ? 4 : 1 << 30;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
