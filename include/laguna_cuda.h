@@ -277,7 +277,8 @@ typedef struct {
  * calls it and one for each captured graph (which holds it until it is
  * destroyed, and no longer than the context): calls on several streams, and
  * replays of several graphs, may run at the same time; one graph not beside
- * itself.  A context's first call is not captured (LC_ERR_UNSUPPORTED where it
+ * itself, nor clones of it, and a graph that an executable one was updated from
+ * is kept as long as that.  A context's first call is not captured (LC_ERR_UNSUPPORTED where it
  * needs scratch).  The reference attends one sequence at a time
  * (kernels/mha_attn.comp:31-72). */
 int lc_prefix_attn(lc_ctx *ctx, int dtype, int out_dtype, const void *q, uint64_t ldq, const lc_prefix_kv *kv,

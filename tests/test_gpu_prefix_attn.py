@@ -532,3 +532,45 @@ def test_captured_scratch_is_used_again(ctx, dev):
         time.sleep(0.05)  # the release comes from a thread of the driver
     assert held[0] == held[-1], held
     c.close()
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+def test_one_long_prompt_beside_single_tokens(ctx, dev, src, dst):
+    """Rows by the mean fill tiles, so that every sequence runs over the whole axis; the long one goes round."""
+    b = Batch(dev, src, dst, 8, 2, 64, 300, 1000, [1, 900, 1, 1, 0, 1], [5, 950, 1000, 1, 7, 64], seed=41, extra=2)
+    b.run(ctx)
+    b.check()
+    ctx.device_status()
+
+
+def test_context_closed_before_its_graph(ctx, dev):
+    """The graph is not replayed any more; that it goes later must not touch what the context freed."""
+    import gc
+    import time
+
+    import torch
+
+    b = Batch(dev, "bf16", "f32", 8, 2, 64, 3000, 64, [1] * 5, [3, 9, 27, 40, 1], seed=42)
+    c, s = lc.Context(0), torch.cuda.Stream()
+    c.set_stream(s)
+    torch.cuda.synchronize()
+    b.run(c)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        b.run(c)
+    c.close()
+    del g
+    gc.collect()
+    time.sleep(0.05)
+    b.run(ctx)
+    b.check()
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+@pytest.mark.parametrize("prefix,cap,counts,lens", [(500, 60, [3, 1, 20], [60, 9, 33]), (0, 300, [200], [300]),
+                                                    (4000, 20, [1] * 12, [20] * 12)])
+def test_without_the_causal_limit_at_any_stride(ctx, dev, src, dst, prefix, cap, counts, lens):
+    b = Batch(dev, src, dst, 8, 4, 64, prefix, cap, counts, lens, seed=43, extra=1, gap=40)
+    b.run(ctx, causal=0)
+    b.check(causal=0)
