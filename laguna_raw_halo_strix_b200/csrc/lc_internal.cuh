@@ -19,11 +19,13 @@
 // memory is freed by lc_destroy.
 struct LcStreamScratch {
     struct Block {
-        void *p;
-        size_t bytes;
-        cudaStream_t stream;
-        std::atomic<unsigned long long> capture;  // its id; 0: of a stream, or of no graph any more (set by
-    };                                            // the thread that destroys the graph)
+        void *p = nullptr;
+        size_t bytes = 0;
+        cudaStream_t stream = nullptr;
+        // The capture's id; 0: of a stream, or of no graph any more (set by the thread that
+        // destroys the graph).
+        std::atomic<unsigned long long> capture{0};
+    };
     std::vector<std::unique_ptr<Block>> eager, captured;
     bool called = false;  // a call has been made outside captures, or needed no block
     size_t bytes = 0;
